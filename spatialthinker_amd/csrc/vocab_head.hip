@@ -1,0 +1,715 @@
+// vocab_head.hip — losses of the vocabulary head straight from the hidden states, for gfx950: no (rows x vocabulary) logits in memory.
+//
+//   z[t][v] = (h_t . w_v) / temperature,   lse_t = log sum_v exp z[t][v]
+//   log-prob of given tokens:          logp_t = z[t][label_t] - lse_t
+//   distillation from top log-probs:   kl_t = sum_k p_tk (log p_tk - (z[t][id_tk] - lse_t)),  p from the teacher's k log-probs of the row
+// Both gradients have one form: d[t][v] = c_t exp(z[t][v] - lse_t) + (sparse targets), dh = d W, dW = d^T h, so both share every product:
+//   forward   head_tile_kernel<STATS>   z tile in registers -> per row (max, sum 2^(z - max)) of 128 columns; then head_lse_kernel
+//   backward  per piece of the vocabulary: head_tile_kernel<DLOGITS> recomputes the tile and writes d (bf16) into a bounded workspace,
+//             head_dh_kernel adds d W into fp32 slabs, head_dw_kernel writes d^T h
+// d is rounded to bf16 because it is the operand of two bf16 matrix products: half a bf16 step (2^-8 relative) per element, the size of the
+// rounding of the bf16 gradients themselves.  Logits, softmax statistics and every sum stay in fp32.
+// What bounds them: the matrix pipe (2 T V H flop forward, 6 T V H backward) from a few hundred rows on, the weight stream (2 V H bytes) below.
+#include "gemm_asm4_core.h"
+#include <algorithm>
+
+#define VH_LOG2E 1.4426950408889634f
+#define VH_LN2 0.6931471805599453f
+
+__device__ __forceinline__ float vh_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// workgroup -> tile: each XCD walks a contiguous range of tiles in groups of 8 tile-rows (A and B panels shared in its L2)
+__device__ __forceinline__ void vh_tile(int bid, int tiles_m, int tiles_n, int& tm, int& tn) {
+    const int nb = tiles_m * tiles_n;
+    const int xcd = bid & 7, idx = bid >> 3, q = nb >> 3, r = nb & 7;
+    bid = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+    const int per_group = 8 * tiles_n;
+    const int group = bid / per_group, in_g = bid % per_group;
+    const int first_m = group * 8;
+    const int gsz = min(tiles_m - first_m, 8);
+    tm = first_m + in_g % gsz;
+    tn = in_g / gsz;
+}
+
+// a row of the backward: d = c * 2^(z2 - lse2), at the label's column hot instead; c == 0 and hot == 0: the row takes no part (d = 0 whatever z is)
+struct alignas(16) VhRow { float c, lse2, hot; int label; };
+
+// targets of the forward: list[start[tm][tn] .. start[tm][tn + 1]) = those in row tile tm and column tile tn; z2 (T, K) takes their logits
+struct VhTargets { const int* start; const uint32_t* list; float* z2; int K; };
+
+// the bf16 tile image of the store epilogues: 256 rows x 256 columns, rows padded by 16 bytes
+#define VH_ROWB (256 * 2 + 16)
+#define VH_SMEM (256 * VH_ROWB)                                      // 135 168 B >= the two 64-KiB operand slots
+
+// one thread's share of the image -> rows of a bf16 matrix; columns in whole 16-byte chunks (cols % 8 == 0, ldc % 8 == 0)
+__device__ __forceinline__ void vh_store_image(const char* smem, uint16_t* __restrict__ C, int64_t ldc, int rows, int cols) {
+    const int t = threadIdx.x, c = t & 31;
+    if (c * 8 >= cols) return;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+        uint4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const uint4*>(smem + ((h * 8 + i) * 8 + (t >> 5)) * VH_ROWB + c * 16);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = (h * 8 + i) * 8 + (t >> 5);
+            if (row < rows) *reinterpret_cast<uint4*>(C + (int64_t)row * ldc + c * 8) = v[i];
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------
+// Logit tile of 256 rows x 256 vocabulary columns.  A lane owns 8 rows (mi*16 + (lane & 15)) and, of each, 4 columns of every 16-column
+// tile ni, so row statistics reduce inside the lane first and over the four lanes of a row last.
+// STATS: part[tn*2 + wn][m] = (max, sum) in base 2 of the 128 columns of a wave; zlab[m] = the label's logit, or z2[m][k] = the logit of target k
+// from the tile's list of targets (head_bucket_kernel): from the same accumulators as the statistics, so that a target that is its row's maximum
+// has exactly the maximum's value.
+// DLOGITS: d[m][n] (bf16, pitch ldd, zero in columns [V, ldd) and rows [T, T64)).
+// ------------------------------------------------------------------------------------------------------------------------------------
+template <bool DLOGITS>
+__global__ __launch_bounds__(256) void head_tile_kernel(const uint16_t* __restrict__ h, int64_t ldh, const uint16_t* __restrict__ w, int64_t ldw, int T,
+                                                       int V, int H, int tiles_m, int tiles_n, float sc, const int64_t* __restrict__ labels,
+                                                       float2* __restrict__ part, float* __restrict__ zlab, VhTargets tg, const VhRow* __restrict__ rows, int v0,
+                                                       uint16_t* __restrict__ d, int64_t ldd, int T64) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 1, wn = wave & 1;
+    int tm, tn;
+    vh_tile(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    const int m0 = tm * A4_BM, n0 = tn * A4_BN;
+    f32x4 acc[8][8];
+    a4_mainloop<false, false, false>(smem, h, ldh, w, ldw, m0, n0, T, V, 0, H / 64, H, acc);
+    const int col0 = n0 + wn * 128 + (lane >> 4) * 4;                // column of (ni, r): col0 + ni*16 + r
+    const bool inside = n0 + A4_BN <= V;
+    if constexpr (!DLOGITS) {
+        const int e0 = tg.start ? tg.start[tm * (tiles_n + 1) + tn] : 0, e1 = tg.start ? tg.start[tm * (tiles_n + 1) + tn + 1] : 0;
+        if (e1 > e0) {                                               // the tile through LDS, 128 columns (64 of each wave pair) at a time
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                __syncthreads();
+#pragma unroll
+                for (int nl = 0; nl < 4; ++nl)
+#pragma unroll
+                    for (int mi = 0; mi < 8; ++mi)
+                        *reinterpret_cast<f32x4*>(smem + (wm * 128 + mi * 16 + (lane & 15)) * VH_ROWB + (wn * 64 + nl * 16 + (lane >> 4) * 4) * 4) = acc[p * 4 + nl][mi];
+                __syncthreads();
+                for (int e = e0 + threadIdx.x; e < e1; e += 256) {
+                    const uint32_t it = tg.list[e];                  // row (8 bits), column (8 bits), k
+                    const int row = it & 255, col = (it >> 8) & 255;
+                    if (((col >> 6) & 1) == p)
+                        tg.z2[(int64_t)(m0 + row) * tg.K + (it >> 16)] =
+                            sc * *reinterpret_cast<const float*>(smem + row * VH_ROWB + ((col >> 7) * 64 + (col & 63)) * 4);
+                }
+            }
+        }
+#pragma unroll
+        for (int mi = 0; mi < 8; ++mi) {
+            const int m = m0 + wm * 128 + mi * 16 + (lane & 15);
+            if (!inside) {
+#pragma unroll
+                for (int ni = 0; ni < 8; ++ni)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[ni][mi][r] = col0 + ni * 16 + r < V ? acc[ni][mi][r] : -INFINITY;
+            }
+            float mx = acc[0][mi][0];
+#pragma unroll
+            for (int ni = 0; ni < 8; ++ni)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[ni][mi][r]);
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float m2 = mx * sc;                                // sc > 0
+            const float sub = m2 == -INFINITY ? 0.f : m2;            // nothing but -inf: every term is 2^-inf = 0
+            float s = 0.f;
+#pragma unroll
+            for (int ni = 0; ni < 8; ++ni)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s += vh_exp2(fmaf(acc[ni][mi][r], sc, -sub));
+            s += __shfl_xor(s, 16, 64);
+            s += __shfl_xor(s, 32, 64);
+            if (m < T) {
+                if (lane < 16) part[(int64_t)(tn * 2 + wn) * T + m] = make_float2(m2, s);
+                if (labels) {
+                    const int64_t lab = labels[m] - (n0 + wn * 128);
+                    if (lab >= 0 && lab < 128) {                     // one lane of the row owns the label's column
+#pragma unroll
+                        for (int ni = 0; ni < 8; ++ni)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (lab == ni * 16 + (lane >> 4) * 4 + r && col0 + ni * 16 + r < V) zlab[m] = acc[ni][mi][r] * sc;
+                    }
+                }
+            }
+        }
+    } else {
+        __syncthreads();                                             // every wave is done with the operand slots
+#pragma unroll
+        for (int mi = 0; mi < 8; ++mi) {
+            const int row = wm * 128 + mi * 16 + (lane & 15), m = m0 + row;
+            VhRow ri = {0.f, 0.f, 0.f, -1};
+            if (m < T) ri = rows[m];
+            const int lab = ri.label - v0 - col0;                    // column of the label relative to this lane's first
+            const bool live = ri.c != 0.f || ri.hot != 0.f;          // (NaN coefficients are live)
+#pragma unroll
+            for (int ni = 0; ni < 8; ++ni) {
+                float o[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float x = ri.c * vh_exp2(fmaf(acc[ni][mi][r], sc, -ri.lse2));
+                    if (lab == ni * 16 + r) x = ri.hot;
+                    o[r] = live && (inside || col0 + ni * 16 + r < V) ? x : 0.f;
+                }
+                uint2 pk;
+                pk.x = f2bf2(o[0], o[1]); pk.y = f2bf2(o[2], o[3]);
+                *reinterpret_cast<uint2*>(smem + row * VH_ROWB + (wn * 128 + ni * 16 + (lane >> 4) * 4) * 2) = pk;
+            }
+        }
+        __syncthreads();
+        vh_store_image(smem, d + (int64_t)m0 * ldd + n0, ldd, T64 - m0, (int)ldd - n0);
+    }
+}
+
+// (max, sum) partials -> lse (natural log), stat = (max, log2 sum); logp = label logit - lse for rows with a label inside the vocabulary, 0 for the others.
+// 16 rows x 64 slices per workgroup: 16 consecutive lanes read 128 contiguous bytes of one partial row.
+__global__ __launch_bounds__(1024) void head_lse_kernel(const float2* __restrict__ part, int n_parts, const float* __restrict__ zlab,
+                                                       const int64_t* __restrict__ labels, float* __restrict__ logp, float* __restrict__ lse, float2* __restrict__ stat,
+                                                       int T, int V) {
+    __shared__ float2 red[64][17];
+    const int r = threadIdx.x & 15, sl = threadIdx.x >> 4;
+    const int row = blockIdx.x * 16 + r;
+    float m = -INFINITY, s = 0.f;
+    if (row < T)
+        for (int p = sl; p < n_parts; p += 64) {
+            const float2 v = part[(int64_t)p * T + row];
+            const float mn = fmaxf(m, v.x);
+            if (mn != -INFINITY) s = s * vh_exp2(m - mn) + v.y * vh_exp2(v.x - mn);
+            else s += v.y;                                           // 0, or NaN kept
+            m = mn;
+        }
+    red[sl][r] = make_float2(m, s);
+    __syncthreads();
+    for (int o = 32; o > 0; o >>= 1) {
+        if (sl < o) {
+            const float2 a = red[sl][r], b = red[sl + o][r];
+            const float mn = fmaxf(a.x, b.x);
+            red[sl][r] = make_float2(mn, mn != -INFINITY ? a.y * vh_exp2(a.x - mn) + b.y * vh_exp2(b.x - mn) : a.y + b.y);
+        }
+        __syncthreads();
+    }
+    if (sl == 0 && row < T) {
+        const float2 v = red[0][r];
+        const float ls = log2f(v.y);
+        lse[row] = (v.x + ls) * VH_LN2;
+        if (stat) stat[row] = make_float2(v.x, ls);
+        if (labels) {                                                // (z - max) - log sum: exact where the label is the maximum, so a log-prob near 0
+            const int64_t lab = labels[row];                         // keeps its digits; z - lse would lose them in lse's rounding
+            logp[row] = lab >= 0 && lab < V ? ((zlab[row] - v.x) - ls) * VH_LN2 : 0.f;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------
+// Backward: row coefficients and the packed hidden states.  A row of d is held as scale_t * d', with d' in the workspace and the scale in
+// hz[t][:] = bf16(scale_t h[t][:]) (for dW) and in the finish of dh.  Where one target dominates a row the scale is that target's gradient: its d' is
+// 1, exact in bf16, and dh does not get that one rounding in all of its elements.  Otherwise the scale is 1 and hz = h.
+// hz is 0 for rows without a gradient and for the padding rows [T, T64): what such rows of h hold (also infinities and NaN) cannot reach dW
+// through 0 * x.
+// ------------------------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void vh_pack_row(const uint16_t* __restrict__ h, int64_t ldh, uint16_t* __restrict__ hz, int t, bool live, float scale, int H) {
+    for (int i = threadIdx.x * 8; i < H; i += blockDim.x * 8) {
+        uint4 o = make_uint4(0, 0, 0, 0);
+        if (live) {
+            float f[8];
+            unpack8(*reinterpret_cast<const uint4*>(h + (int64_t)t * ldh + i), f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] *= scale;
+            o = pack8(f);
+        }
+        *reinterpret_cast<uint4*>(hz + (int64_t)t * H + i) = o;
+    }
+}
+
+__global__ __launch_bounds__(128) void head_rows_label_kernel(const uint16_t* __restrict__ h, int64_t ldh, const int64_t* __restrict__ labels,
+                                                             const float* __restrict__ logp, const float* __restrict__ lse,
+                                                             const float* __restrict__ g, float inv_temp, VhRow* __restrict__ rows,
+                                                             float* __restrict__ scale, uint16_t* __restrict__ hz, int T, int V, int H) {
+    const int t = blockIdx.x;
+    VhRow ri = {0.f, 0.f, 0.f, -1};
+    float sc = 1.f;
+    if (t < T) {
+        const int64_t lab = labels[t];
+        if (lab >= 0 && lab < V) {
+            const float e = expm1f(logp[t]), hot = -e * g[t] * inv_temp;                 // g/temperature (1 - q), q the label's probability
+            if (hot != 0.f) {                                        // (NaN is not 0)
+                sc = hot;
+                ri.c = 1.f / e; ri.hot = 1.f; ri.label = (int)lab; ri.lse2 = lse[t] * VH_LOG2E;
+            }
+        }
+        if (threadIdx.x == 0) { rows[t] = ri; scale[t] = sc; }
+    }
+    vh_pack_row(h, ldh, hz, t, ri.hot != 0.f, sc, H);
+}
+
+// slab[s][m][n] (+)= sum over the K-slice s of d[m][:] w[:][n]: w is contraction-major as stored; `kv` of the ldd columns of d are vocabulary
+template <bool ACCUM>
+__global__ __launch_bounds__(256) void head_dh_kernel(const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ w, int64_t ldw, int T,
+                                                     int kv, int H, int tiles_m, int tiles_n, int split, float* __restrict__ slab) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 1, wn = wave & 1;
+    const int nb = tiles_m * tiles_n, slice = blockIdx.x / nb;
+    int tm, tn;
+    vh_tile(blockIdx.x % nb, tiles_m, tiles_n, tm, tn);
+    const int m0 = tm * A4_BM, n0 = tn * A4_BN;
+    const int nkt = (kv + 63) / 64, per = (nkt + split - 1) / split, kt0 = slice * per;
+    const int nk = min(nkt - kt0, per);                              // >= 1: the host gives no slice without K-tiles
+    f32x4 acc[8][8];
+    a4_mainloop<false, true, false, 0, true>(smem, d, ldd, w, ldw, m0, n0, T, H, kt0, nk, kv, acc);
+    float* out = slab + (int64_t)slice * T * H;
+#pragma unroll
+    for (int mi = 0; mi < 8; ++mi) {
+        const int m = m0 + wm * 128 + mi * 16 + (lane & 15);
+        if (m >= T) continue;
+#pragma unroll
+        for (int ni = 0; ni < 8; ++ni) {
+            const int n = n0 + wn * 128 + ni * 16 + (lane >> 4) * 4;
+            if (n >= H) continue;
+            float4* p = reinterpret_cast<float4*>(out + (int64_t)m * H + n);
+            float4 o = make_float4(acc[ni][mi][0], acc[ni][mi][1], acc[ni][mi][2], acc[ni][mi][3]);
+            if constexpr (ACCUM) { const float4 c = *p; o.x += c.x; o.y += c.y; o.z += c.z; o.w += c.w; }
+            *p = o;
+        }
+    }
+}
+
+// dh = bf16(row scale * sum of the slabs, in slice order)
+__global__ __launch_bounds__(256) void head_dh_finish_kernel(const float* __restrict__ slab, int split, const float* __restrict__ scale, uint16_t* __restrict__ dh, int64_t lddh, int T, int H) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= (int64_t)T * H) return;
+    float4 a = *reinterpret_cast<const float4*>(slab + i);
+    for (int s = 1; s < split; ++s) {
+        const float4 b = *reinterpret_cast<const float4*>(slab + (int64_t)s * T * H + i);
+        a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+    }
+    const float sc = scale[i / H];                                   // H % 64 == 0: the four values are of one row
+    uint2 o;
+    o.x = f2bf2(sc * a.x, sc * a.y); o.y = f2bf2(sc * a.z, sc * a.w);
+    *reinterpret_cast<uint2*>(dh + (i / H) * lddh + i % H) = o;
+}
+
+// dw[v][n] = sum_t d[t][v] hz[t][n]: both operands contraction-major as they lie in memory.  bf16 result, or fp32 (+=).
+template <bool OUT_BF16, bool ACCUM>
+__global__ __launch_bounds__(256) void head_dw_kernel(const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ hz, int T64, int kv, int H,
+                                                     int tiles_m, int tiles_n, uint16_t* __restrict__ dwb, float* __restrict__ dwf, int64_t lddw) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 1, wn = wave & 1;
+    int tm, tn;
+    vh_tile(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    const int m0 = tm * A4_BM, n0 = tn * A4_BN;
+    f32x4 acc[8][8];
+    a4_mainloop<true, true, false, 0, false, !OUT_BF16>(smem, d, ldd, hz, H, m0, n0, (int)ldd, H, 0, T64 / 64, T64, acc);
+    if constexpr (OUT_BF16) {
+        __syncthreads();
+#pragma unroll
+        for (int mi = 0; mi < 8; ++mi) {
+            const int row = wm * 128 + mi * 16 + (lane & 15);
+#pragma unroll
+            for (int ni = 0; ni < 8; ++ni) {
+                uint2 pk;
+                pk.x = f2bf2(acc[ni][mi][0], acc[ni][mi][1]); pk.y = f2bf2(acc[ni][mi][2], acc[ni][mi][3]);
+                *reinterpret_cast<uint2*>(smem + row * VH_ROWB + (wn * 128 + ni * 16 + (lane >> 4) * 4) * 2) = pk;
+            }
+        }
+        __syncthreads();
+        vh_store_image(smem, dwb + (int64_t)m0 * lddw + n0, lddw, kv - m0, H - n0);
+    } else {
+#pragma unroll
+        for (int mi = 0; mi < 8; ++mi) {
+            const int m = m0 + wm * 128 + mi * 16 + (lane & 15);
+            if (m >= kv) continue;
+#pragma unroll
+            for (int ni = 0; ni < 8; ++ni) {
+                const int n = n0 + wn * 128 + ni * 16 + (lane >> 4) * 4;
+                if (n >= H) continue;
+                float4* p = reinterpret_cast<float4*>(dwf + (int64_t)m * lddw + n);
+                float4 o = make_float4(acc[ni][mi][0], acc[ni][mi][1], acc[ni][mi][2], acc[ni][mi][3]);
+                if constexpr (ACCUM) { const float4 c = *p; o.x += c.x; o.y += c.y; o.z += c.z; o.w += c.w; }
+                *p = o;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------
+// Distillation from k teacher log-probs per row.
+// ------------------------------------------------------------------------------------------------------------------------------------
+#define VH_MAX_K 1024
+#define VH_MAX_V (1 << 22)                                           // column tiles fit the counters of head_bucket_kernel
+
+// teacher probabilities of one row, by one wave: p_k of present entries (0 <= id < V), 0 for the others; log p_k = a_k - shift
+struct VhTeacher { float shift, total; };
+__device__ __forceinline__ VhTeacher vh_teacher(const int32_t* __restrict__ ids, const float* __restrict__ a, int K, int V, bool renorm, int lane) {
+    VhTeacher r = {0.f, 0.f};
+    if (renorm) {                                                    // log p = a - log sum_k exp a over the present entries
+        float m = -INFINITY, s = 0.f;
+        for (int k = lane; k < K; k += 64) if (ids[k] >= 0 && ids[k] < V) m = fmaxf(m, a[k]);
+        m = wave_max(m);
+        if (m == -INFINITY) return r;                                // nothing present (or only zero probabilities): the row takes no part
+        for (int k = lane; k < K; k += 64) if (ids[k] >= 0 && ids[k] < V) s += vh_exp2((a[k] - m) * VH_LOG2E);
+        s = wave_sum(s);
+        r.shift = m + log2f(s) * VH_LN2;
+        r.total = 1.f;
+        return r;
+    }
+    float s = 0.f;
+    for (int k = lane; k < K; k += 64) if (ids[k] >= 0 && ids[k] < V) s += vh_exp2(a[k] * VH_LOG2E);
+    r.total = wave_sum(s);
+    return r;
+}
+
+// The targets of each 256-row tile, sorted by 256-column tile (counting sort in LDS): one workgroup per row tile.  The order inside a list depends on
+// LDS atomics, its use does not: every entry writes a place of its own.  Absent entries get z2 = 0 here.
+__global__ __launch_bounds__(1024) void head_bucket_kernel(const int32_t* __restrict__ ids, int K, int* __restrict__ start, uint32_t* __restrict__ list,
+                                                          float* __restrict__ z2, int T, int V, int tiles_n) {
+    extern __shared__ int bin[];                                     // tiles_n counters, then 16 wave totals
+    int* wave_total = bin + tiles_n;
+    const int r0 = blockIdx.x * 256, n = min(256, T - r0) * K, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    ids += (int64_t)r0 * K; z2 += (int64_t)r0 * K;
+    start += (int64_t)blockIdx.x * (tiles_n + 1);
+    const int base = blockIdx.x * 256 * K;                           // <= 2^31: T * K is checked on the host
+    for (int i = threadIdx.x; i < tiles_n; i += 1024) bin[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += 1024) {
+        const int32_t id = ids[i];
+        if (id >= 0 && id < V) atomicAdd(&bin[id >> 8], 1);
+        else z2[i] = 0.f;
+    }
+    __syncthreads();
+    // exclusive prefix sums, 1024 bins at a time
+    int run = base;
+    for (int b0 = 0; b0 < tiles_n; b0 += 1024) {
+        const int b = b0 + threadIdx.x, c = b < tiles_n ? bin[b] : 0;
+        int x = c;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const int y = __shfl_up(x, o, 64); x += lane >= o ? y : 0; }
+        if (lane == 63) wave_total[wave] = x;
+        __syncthreads();
+        int before = run, total = 0;
+#pragma unroll
+        for (int wv = 0; wv < 16; ++wv) { before += wv < wave ? wave_total[wv] : 0; total += wave_total[wv]; }
+        if (b < tiles_n) { bin[b] = before + x - c; start[b] = before + x - c; }
+        run += total;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) start[tiles_n] = run;
+    for (int i = threadIdx.x; i < n; i += 1024) {
+        const int32_t id = ids[i];
+        if (id >= 0 && id < V) list[atomicAdd(&bin[id >> 8], 1)] = (uint32_t)(i / K) | (uint32_t)(id & 255) << 8 | (uint32_t)(i % K) << 16;
+    }
+}
+
+// kl and log q of every row, one wave per row: logq[t][k] (in: z2 of the target, out: natural log q; 0 for absent entries)
+__global__ __launch_bounds__(256) void head_kl_kernel(const int32_t* __restrict__ ids, const float* __restrict__ a, int K, int renorm,
+                                                     const float2* __restrict__ stat, float* __restrict__ logq, float* __restrict__ kl, int T, int V) {
+    const int lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (t >= T) return;
+    ids += (int64_t)t * K; a += (int64_t)t * K; logq += (int64_t)t * K;
+    const VhTeacher th = vh_teacher(ids, a, K, V, renorm, lane);
+    const float2 st = stat[t];
+    float s = 0.f;
+    for (int k = lane; k < K; k += 64) {
+        const bool have = ids[k] >= 0 && ids[k] < V;
+        const float q = have ? ((logq[k] - st.x) - st.y) * VH_LN2 : 0.f;
+        logq[k] = q;
+        const float lp = a[k] - th.shift, p = have && th.total != 0.f ? vh_exp2(lp * VH_LOG2E) : 0.f;
+        if (p != 0.f) s += p * (lp - q);                             // a zero probability contributes nothing, whatever its logarithm
+    }
+    s = wave_sum(s);
+    if (lane == 0) kl[t] = s;
+}
+
+__global__ __launch_bounds__(128) void head_rows_kl_kernel(const uint16_t* __restrict__ h, int64_t ldh, const int32_t* __restrict__ ids,
+                                                          const float* __restrict__ a, int K, int renorm, const float* __restrict__ lse,
+                                                          const float* __restrict__ logq, const float* __restrict__ g, float inv_temp,
+                                                          VhRow* __restrict__ rows, float* __restrict__ scale, uint16_t* __restrict__ hz, int T, int V, int H) {
+    const int t = blockIdx.x, lane = threadIdx.x & 63;
+    VhRow ri = {0.f, 0.f, 0.f, -1};
+    float sc = 1.f;
+    if (t < T) {
+        ids += (int64_t)t * K; a += (int64_t)t * K; logq += (int64_t)t * K;
+        const VhTeacher th = vh_teacher(ids, a, K, V, renorm, lane);
+        const float gt = g[t] * inv_temp;
+        if (th.total != 0.f && gt != 0.f) {
+            float top = 0.f, val = 0.f, energy = 0.f;                // the target with the largest gradient, and the sum of the squares
+            for (int k = lane; k < K; k += 64)
+                if (ids[k] >= 0 && ids[k] < V) {
+                    const float x = gt * (th.total * vh_exp2(logq[k] * VH_LOG2E) - vh_exp2((a[k] - th.shift) * VH_LOG2E));
+                    energy += x * x;
+                    if (fabsf(x) > top) { top = fabsf(x); val = x; }
+                }
+            energy = wave_sum(energy);
+            const float most = wave_max(top);
+            const unsigned long long who = __ballot(top == most);
+            val = __shfl(val, who ? __ffsll(who) - 1 : 0, 64);
+            if (most * most > 0.5f * energy && most < INFINITY) sc = val;
+            ri.c = gt * th.total / sc;
+            ri.lse2 = lse[t] * VH_LOG2E;
+        }
+        if (threadIdx.x == 0) { rows[t] = ri; scale[t] = sc; }
+    }
+    vh_pack_row(h, ldh, hz, t, ri.c != 0.f, sc, H);
+}
+
+// d' at the targets of a piece [v0, v0 + kv): overwritten with the whole value (c / P) (P q - sum of the p of this id), from the fp32
+// log q of the forward pass.  An id that a row holds twice gets the sum of its probabilities from both entries: the same value twice.
+__global__ __launch_bounds__(256) void head_sparse_kernel(const int32_t* __restrict__ ids, const float* __restrict__ a, int K, int renorm,
+                                                         const float* __restrict__ logq, const VhRow* __restrict__ rows, int v0, int kv,
+                                                         uint16_t* __restrict__ d, int64_t ldd, int T, int V) {
+    const int lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (t >= T) return;
+    ids += (int64_t)t * K; a += (int64_t)t * K; logq += (int64_t)t * K;
+    const VhTeacher th = vh_teacher(ids, a, K, V, renorm, lane);
+    const float c = rows[t].c;                                       // g/temperature P / scale
+    if (c == 0.f) return;                                            // the row's d is zero
+    const float r = c / th.total;
+    for (int k = lane; k < K; k += 64) {
+        const int32_t id = ids[k];
+        if (id < v0 || id >= v0 + kv) continue;
+        float p = 0.f;
+        for (int j = 0; j < K; ++j) if (ids[j] == id) p += vh_exp2((a[j] - th.shift) * VH_LOG2E);
+        d[(int64_t)t * ldd + id - v0] = f2bf(r * (th.total * vh_exp2(logq[k] * VH_LOG2E) - p));
+    }
+}
+
+__global__ __launch_bounds__(256) void head_zero_kernel(char* __restrict__ p, int64_t pitch_bytes, int64_t row_bytes) {
+    for (int64_t i = threadIdx.x * 8; i < row_bytes; i += 256 * 8) *reinterpret_cast<uint2*>(p + (int64_t)blockIdx.x * pitch_bytes + i) = make_uint2(0, 0);
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------------------------------------------
+namespace {
+struct Plan {                                                        // workspace layout (byte offsets) and piece / slice counts of one call
+    int T64, pieces, piece, split;
+    int64_t part, zlab, stat, start, list, fwd_bytes;
+    int64_t rows, scale, hz, d, slab, bwd_bytes;
+};
+int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
+
+Plan head_plan(int T, int V, int H, int K) {                         // K: targets per row of the distillation, 0: labels
+    Plan p;
+    p.T64 = (int)up(T, 64);
+    const int64_t n_parts = 2 * (int64_t)st_cdiv(V, 256);
+    p.part = 0;
+    p.zlab = up(n_parts * T * 8, 256);
+    p.stat = p.zlab + up((int64_t)T * 4, 256);
+    p.start = p.stat + up((int64_t)T * 8, 256);
+    p.list = p.start + (K ? up((int64_t)st_cdiv(T, 256) * (st_cdiv(V, 256) + 1) * 4, 256) : 0);
+    p.fwd_bytes = p.list + up((int64_t)T * K * 4, 256);
+    // d of one piece: at most 512 MiB
+    const int64_t max_cols = std::max<int64_t>(256, ((int64_t)512 << 20) / 2 / p.T64 / 256 * 256);
+    p.pieces = st_cdiv(V, max_cols);
+    p.piece = (int)up(st_cdiv(V, p.pieces), 256);
+    p.pieces = st_cdiv(V, p.piece);
+    // dh: K-slices so that few row tiles still fill the CUs (whole rounds of a tile's K-steps + ~14 of prologue / epilogue)
+    const int tiles = st_cdiv(T, 256) * st_cdiv(H, 256), ncu = st_num_cus(), nkt = st_cdiv(std::min(V, p.piece), 64);
+    p.split = 1;
+    int64_t best = INT64_MAX;
+    for (int s = 1; s <= 32; ++s) {
+        if (s > 1 && (nkt / s < 8 || (int64_t)s * T * H * 4 > ((int64_t)512 << 20))) break;
+        const int64_t cost = (int64_t)st_cdiv((int64_t)tiles * s, ncu) * (st_cdiv(nkt, s) + 14) + 2 * s;
+        if (cost < best) { best = cost; p.split = s; }
+    }
+    p.rows = 0;
+    p.scale = up((int64_t)T * (int64_t)sizeof(VhRow), 256);
+    p.hz = p.scale + up((int64_t)T * 4, 256);
+    p.d = p.hz + up((int64_t)p.T64 * H * 2, 256);
+    p.slab = p.d + up((int64_t)p.T64 * p.piece * 2, 256);
+    p.bwd_bytes = p.slab + up((int64_t)p.split * T * H * 4, 256);
+    return p;
+}
+
+bool operands_ok(const void* h, int64_t ldh, const void* w, int64_t ldw, int T, int V, int H, float inv_temp) {
+    return h && w && T >= 0 && V > 0 && V <= VH_MAX_V && H > 0 && H % 64 == 0 && !(ldh & 7) && !(ldw & 7) && ldh >= H && ldw >= H && ldh < (1 << 22) && ldw < (1 << 22) &&
+           !(((uintptr_t)h) & 15) && !(((uintptr_t)w) & 15) && inv_temp > 0.f && inv_temp < INFINITY && (int64_t)st_cdiv(T, 256) * st_cdiv(V, 256) < (1 << 30);
+}
+
+// one attribute per kernel and device, set before its first launch there
+template <auto KERN> void allow_lds() {
+    static bool done[64] = {};
+    int dev = 0;
+    hipGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !done[dev]) {
+        hipFuncSetAttribute((const void*)KERN, hipFuncAttributeMaxDynamicSharedMemorySize, VH_SMEM);
+        if (dev >= 0 && dev < 64) done[dev] = true;
+    }
+}
+
+int head_stats(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, const int64_t* labels, float sc, float* logp, float* lse, VhTargets tg,
+               char* ws, const Plan& p, int T, int V, int H, hipStream_t s) {
+    const int tm = st_cdiv(T, 256), tn = st_cdiv(V, 256);
+    float2* part = (float2*)(ws + p.part);
+    float* zlab = (float*)(ws + p.zlab);
+    allow_lds<head_tile_kernel<false>>();
+    hipLaunchKernelGGL((head_tile_kernel<false>), dim3(tm * tn), dim3(256), VH_SMEM, s, h, ldh, w, ldw, T, V, H, tm, tn, sc, labels, part, zlab, tg,
+                       (const VhRow*)nullptr, 0, (uint16_t*)nullptr, (int64_t)0, 0);
+    ST_CHECK_LAUNCH();
+    hipLaunchKernelGGL(head_lse_kernel, dim3(st_cdiv(T, 16)), dim3(1024), 0, s, part, 2 * tn, zlab, labels, logp, lse, (float2*)(ws + p.stat), T, V);
+    ST_CHECK_LAUNCH();
+    return 0;
+}
+
+// the pieces of a backward pass behind the row coefficients; `sparse(v0, kv, ldd)` finishes d at the targets of a piece
+template <class F>
+int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, float sc, uint16_t* dh, int64_t lddh, uint16_t* dwb, float* dwf,
+                  int64_t lddw, int accumulate, char* ws, const Plan& p, int T, int V, int H, hipStream_t s, F&& sparse) {
+    const VhRow* rows = (const VhRow*)(ws + p.rows);
+    const uint16_t* hz = (const uint16_t*)(ws + p.hz);
+    uint16_t* d = (uint16_t*)(ws + p.d);
+    float* slab = (float*)(ws + p.slab);
+    const int tm = st_cdiv(T, 256), th = st_cdiv(H, 256);
+    allow_lds<head_tile_kernel<true>>();
+    allow_lds<head_dh_kernel<false>>(); allow_lds<head_dh_kernel<true>>();
+    allow_lds<head_dw_kernel<true, false>>(); allow_lds<head_dw_kernel<false, false>>(); allow_lds<head_dw_kernel<false, true>>();
+    for (int i = 0; i < p.pieces; ++i) {
+        const int v0 = i * p.piece, kv = std::min(p.piece, V - v0), tn = st_cdiv(kv, 256);
+        const int64_t ldd = up(kv, 64);
+        const uint16_t* wp = w + (int64_t)v0 * ldw;
+        hipLaunchKernelGGL((head_tile_kernel<true>), dim3(tm * tn), dim3(256), VH_SMEM, s, h, ldh, wp, ldw, T, kv, H, tm, tn, sc, (const int64_t*)nullptr,
+                           (float2*)nullptr, (float*)nullptr, VhTargets{}, rows, v0, d, ldd, p.T64);
+        ST_CHECK_LAUNCH();
+        const int rc = sparse(v0, kv, d, ldd);
+        if (rc) return rc;
+        if (dh) {
+            const int nkt = st_cdiv(kv, 64), per = st_cdiv(nkt, p.split), slices = st_cdiv(nkt, per);      // (a short last piece may fill fewer slices)
+            const dim3 grid(tm * th * slices);
+            if (i == 0) hipLaunchKernelGGL((head_dh_kernel<false>), grid, dim3(256), VH_SMEM, s, d, ldd, wp, ldw, T, kv, H, tm, th, p.split, slab);
+            else hipLaunchKernelGGL((head_dh_kernel<true>), grid, dim3(256), VH_SMEM, s, d, ldd, wp, ldw, T, kv, H, tm, th, p.split, slab);
+            ST_CHECK_LAUNCH();
+        }
+        if (dwb || dwf) {
+            const int tv = st_cdiv(kv, 256);
+            const dim3 grid(tv * th);
+            uint16_t* ob = dwb ? dwb + (int64_t)v0 * lddw : nullptr;
+            float* of = dwf ? dwf + (int64_t)v0 * lddw : nullptr;
+            if (dwb) hipLaunchKernelGGL((head_dw_kernel<true, false>), grid, dim3(256), VH_SMEM, s, d, ldd, hz, p.T64, kv, H, tv, th, ob, of, lddw);
+            else if (accumulate) hipLaunchKernelGGL((head_dw_kernel<false, true>), grid, dim3(256), VH_SMEM, s, d, ldd, hz, p.T64, kv, H, tv, th, ob, of, lddw);
+            else hipLaunchKernelGGL((head_dw_kernel<false, false>), grid, dim3(256), VH_SMEM, s, d, ldd, hz, p.T64, kv, H, tv, th, ob, of, lddw);
+            ST_CHECK_LAUNCH();
+        }
+    }
+    if (dh) {
+        const int nkt = st_cdiv(std::min(V, p.piece), 64), slices = st_cdiv(nkt, st_cdiv(nkt, p.split));
+        hipLaunchKernelGGL(head_dh_finish_kernel, dim3(st_cdiv((int64_t)T * H, 1024)), dim3(256), 0, s, slab, slices, (const float*)(ws + p.scale), dh, lddh, T, H);
+        ST_CHECK_LAUNCH();
+    }
+    return 0;
+}
+
+bool grads_ok(const void* dh, int64_t lddh, const void* dwb, const void* dwf, int64_t lddw, int accumulate, int H) {
+    if (dh && ((((uintptr_t)dh) & 7) || (lddh & 3) || lddh < H)) return false;
+    if (dwb && (dwf || accumulate || (((uintptr_t)dwb) & 15) || (lddw & 7) || lddw < H)) return false;
+    if (dwf && ((((uintptr_t)dwf) & 15) || (lddw & 3) || lddw < H)) return false;
+    return true;
+}
+
+// no rows: dW is a sum over nothing
+int empty_dw(uint16_t* dwb, float* dwf, int64_t lddw, int accumulate, int V, int H, hipStream_t s) {
+    if (accumulate || (!dwb && !dwf)) return 0;
+    const int64_t e = dwb ? 2 : 4;
+    hipLaunchKernelGGL(head_zero_kernel, dim3(V), dim3(256), 0, s, dwb ? (char*)dwb : (char*)dwf, lddw * e, (int64_t)H * e);
+    ST_CHECK_LAUNCH();
+    return 0;
+}
+}  // namespace
+
+extern "C" {
+
+int st_linear_head_workspace_bytes(int T, int V, int H, int K, int backward, int64_t* bytes_host, st_stream_t stream) {
+    (void)stream;
+    if (T < 0 || K < 0 || K > VH_MAX_K || V <= 0 || V > VH_MAX_V || H <= 0 || H % 64 || !bytes_host) return ST_EINVAL;
+    const Plan p = head_plan(std::max(T, 1), V, H, K);
+    *bytes_host = backward ? p.bwd_bytes : p.fwd_bytes;
+    return 0;
+}
+
+int st_linear_logprob_fwd(const st_bf16* hidden, int64_t ldh, const st_bf16* weight, int64_t ldw, const int64_t* labels, float inv_temperature,
+                          float* logp, float* lse, void* workspace, int64_t workspace_bytes, int T, int V, int H, st_stream_t stream) {
+    if (T == 0) return V > 0 && H > 0 && H % 64 == 0 ? 0 : ST_EINVAL;
+    if (!operands_ok(hidden, ldh, weight, ldw, T, V, H, inv_temperature) || !labels || !logp || !lse) return ST_EINVAL;
+    const Plan p = head_plan(T, V, H, 0);
+    if (!workspace || workspace_bytes < p.fwd_bytes) return ST_EINVAL;
+    return head_stats(hidden, ldh, weight, ldw, labels, inv_temperature * VH_LOG2E, logp, lse, VhTargets{}, (char*)workspace, p, T, V, H,
+                      (hipStream_t)stream);
+}
+
+int st_linear_logprob_bwd(const st_bf16* hidden, int64_t ldh, const st_bf16* weight, int64_t ldw, const int64_t* labels, const float* logp, const float* lse,
+                          const float* g, float inv_temperature, st_bf16* dhidden, int64_t lddh, st_bf16* dweight_bf16, float* dweight_f32, int64_t lddw, int accumulate,
+                          void* workspace, int64_t workspace_bytes, int T, int V, int H, st_stream_t stream) {
+    hipStream_t s = (hipStream_t)stream;
+    if (V <= 0 || H <= 0 || H % 64 || T < 0 || !grads_ok(dhidden, lddh, dweight_bf16, dweight_f32, lddw, accumulate, H)) return ST_EINVAL;
+    if (T == 0) return empty_dw(dweight_bf16, dweight_f32, lddw, accumulate, V, H, s);
+    if (!operands_ok(hidden, ldh, weight, ldw, T, V, H, inv_temperature) || !labels || !logp || !lse || !g) return ST_EINVAL;
+    const Plan p = head_plan(T, V, H, 0);
+    if (!workspace || workspace_bytes < p.bwd_bytes) return ST_EINVAL;
+    char* ws = (char*)workspace;
+    hipLaunchKernelGGL(head_rows_label_kernel, dim3(p.T64), dim3(128), 0, s, hidden, ldh, labels, logp, lse, g, inv_temperature, (VhRow*)(ws + p.rows),
+                       (float*)(ws + p.scale), (uint16_t*)(ws + p.hz), T, V, H);
+    ST_CHECK_LAUNCH();
+    return head_backward(hidden, ldh, weight, ldw, inv_temperature * VH_LOG2E, dhidden, lddh, dweight_bf16, dweight_f32, lddw, accumulate, ws, p, T, V, H, s,
+                         [](int, int, uint16_t*, int64_t) { return 0; });
+}
+
+int st_linear_topk_kl_fwd(const st_bf16* hidden, int64_t ldh, const st_bf16* weight, int64_t ldw, const int32_t* ids, const float* teacher_logp, int K,
+                          int renormalize, float inv_temperature, float* kl, float* lse, float* logq, void* workspace, int64_t workspace_bytes, int T,
+                          int V, int H, st_stream_t stream) {
+    if (K <= 0 || K > VH_MAX_K || (int64_t)T * K > INT32_MAX) return ST_EINVAL;
+    if (T == 0) return V > 0 && H > 0 && H % 64 == 0 ? 0 : ST_EINVAL;
+    if (!operands_ok(hidden, ldh, weight, ldw, T, V, H, inv_temperature) || !ids || !teacher_logp || !kl || !lse || !logq) return ST_EINVAL;
+    const Plan p = head_plan(T, V, H, K);
+    if (!workspace || workspace_bytes < p.fwd_bytes) return ST_EINVAL;
+    hipStream_t s = (hipStream_t)stream;
+    const float sc = inv_temperature * VH_LOG2E;
+    char* ws = (char*)workspace;
+    int* start = (int*)(ws + p.start);
+    uint32_t* list = (uint32_t*)(ws + p.list);
+    const int tn = st_cdiv(V, 256);
+    hipLaunchKernelGGL(head_bucket_kernel, dim3(st_cdiv(T, 256)), dim3(1024), (tn + 16) * 4, s, ids, K, start, list, logq, T, V, tn);
+    ST_CHECK_LAUNCH();
+    const int rc = head_stats(hidden, ldh, weight, ldw, nullptr, sc, nullptr, lse, VhTargets{start, list, logq, K}, ws, p, T, V, H, s);
+    if (rc) return rc;
+    hipLaunchKernelGGL(head_kl_kernel, dim3(st_cdiv(T, 4)), dim3(256), 0, s, ids, teacher_logp, K, renormalize,
+                       (const float2*)(ws + p.stat), logq, kl, T, V);
+    ST_CHECK_LAUNCH();
+    return 0;
+}
+
+int st_linear_topk_kl_bwd(const st_bf16* hidden, int64_t ldh, const st_bf16* weight, int64_t ldw, const int32_t* ids, const float* teacher_logp, int K,
+                          int renormalize, float inv_temperature, const float* lse, const float* logq, const float* g, st_bf16* dhidden, int64_t lddh,
+                          st_bf16* dweight_bf16, float* dweight_f32, int64_t lddw, int accumulate, void* workspace, int64_t workspace_bytes, int T, int V,
+                          int H, st_stream_t stream) {
+    hipStream_t s = (hipStream_t)stream;
+    if (K <= 0 || K > VH_MAX_K || V <= 0 || H <= 0 || H % 64 || T < 0 || !grads_ok(dhidden, lddh, dweight_bf16, dweight_f32, lddw, accumulate, H))
+        return ST_EINVAL;
+    if (T == 0) return empty_dw(dweight_bf16, dweight_f32, lddw, accumulate, V, H, s);
+    if (!operands_ok(hidden, ldh, weight, ldw, T, V, H, inv_temperature) || !ids || !teacher_logp || !lse || !logq || !g) return ST_EINVAL;
+    const Plan p = head_plan(T, V, H, 0);
+    if (!workspace || workspace_bytes < p.bwd_bytes) return ST_EINVAL;
+    char* ws = (char*)workspace;
+    hipLaunchKernelGGL(head_rows_kl_kernel, dim3(p.T64), dim3(128), 0, s, hidden, ldh, ids, teacher_logp, K, renormalize, lse, logq, g, inv_temperature,
+                       (VhRow*)(ws + p.rows), (float*)(ws + p.scale), (uint16_t*)(ws + p.hz), T, V, H);
+    ST_CHECK_LAUNCH();
+    return head_backward(hidden, ldh, weight, ldw, inv_temperature * VH_LOG2E, dhidden, lddh, dweight_bf16, dweight_f32, lddw, accumulate, ws, p, T, V, H, s,
+                         [&](int v0, int kv, uint16_t* d, int64_t ldd) -> int {
+                             hipLaunchKernelGGL(head_sparse_kernel, dim3(st_cdiv(T, 4)), dim3(256), 0, s, ids, teacher_logp, K, renormalize, logq,
+                                                (const VhRow*)(ws + p.rows), v0, kv, d, ldd, T, V);
+                             ST_CHECK_LAUNCH();
+                             return 0;
+                         });
+}
+
+}  // extern "C"

@@ -113,6 +113,173 @@ def grpo_advantage(rewards, mask, group, n_groups: int, eps: float = 1e-6):
     return adv, status
 
 
+# ------------------------------------------------------------------ vocabulary head without stored logits
+HEAD_MAX_TARGETS = 1024         # VH_MAX_K of the library
+HEAD_MAX_VOCAB = 1 << 22        # VH_MAX_V of the library
+TOPK_MAX = 256                  # TK_MAX_K of the library
+
+
+def _on(device, *named):
+    """Every tensor on `device` — the kernels run on the current stream of that device."""
+    for t, what in named:
+        if t is not None and t.device != device:
+            raise RuntimeError(f"{what}: on {t.device}, expected {device}")
+
+
+def _vec(t, dtype, shape, what):
+    if t.dtype != dtype:
+        raise TypeError(f"{what}: expected {dtype}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: must be contiguous")
+    return t
+
+
+def _head_operands(hidden, weight, temperature):
+    _chk(hidden, BF16, "hidden"); _chk(weight, BF16, "weight")
+    if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
+        raise ValueError(f"hidden (T, H) and weight (V, H): got {tuple(hidden.shape)} and {tuple(weight.shape)}")
+    T, H = hidden.shape
+    if weight.shape[0] == 0 or H == 0 or H % 64:
+        raise ValueError(f"the head needs at least one token and a width in multiples of 64, got {tuple(weight.shape)}")
+    if not (temperature > 0.0 and math.isfinite(temperature) and math.isfinite(1.0 / temperature)):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    for t, what in ((hidden, "hidden"), (weight, "weight")):
+        if t.shape[0] and (t.data_ptr() & 15 or t.stride(0) & 7 or t.stride(0) < H or t.stride(0) >= 1 << 22):
+            raise ValueError(f"{what}: rows must be 16-byte aligned and not overlap (stride {t.stride(0)})")
+    if not hidden.is_cuda:
+        _p(hidden)
+    _on(hidden.device, (weight, "weight"))
+    if weight.shape[0] > HEAD_MAX_VOCAB:
+        raise ValueError(f"vocabularies up to {HEAD_MAX_VOCAB} tokens, got {weight.shape[0]}")
+    return T, weight.shape[0], H
+
+
+def _head_workspace(T, V, H, K, backward, device):
+    """Scratch of one call, from torch's stream-ordered allocator (a captured graph gets its own from its pool)."""
+    import ctypes
+    n = ctypes.c_int64(0)
+    lib().st_linear_head_workspace_bytes(T, V, H, K, int(backward), ctypes.addressof(n), None)
+    return torch.empty(n.value, dtype=torch.uint8, device=device)
+
+
+def _head_grads(hidden, weight, want_dhidden, dweight, dweight_f32, accumulate):
+    """(dhidden or None) after the checks of the gradient outputs."""
+    if dweight is not None and (dweight_f32 is not None or accumulate):
+        raise ValueError("dweight: one of bf16 (overwritten) and fp32 (optionally accumulated)")
+    for t, dt, what in ((dweight, BF16, "dweight"), (dweight_f32, F32, "dweight_f32")):
+        if t is not None:
+            _chk(t, dt, what)
+            if t.shape != weight.shape or t.data_ptr() & 15 or t.stride(0) % (16 // t.element_size()) or t.stride(0) < t.shape[1]:
+                raise ValueError(f"{what}: expected {tuple(weight.shape)} with 16-byte aligned rows")
+            _on(hidden.device, (t, what))
+    return torch.empty(hidden.shape, dtype=BF16, device=hidden.device) if want_dhidden else None
+
+
+def _ld(t):
+    return t.stride(0) if t is not None else 0
+
+
+def linear_logprob_fwd(hidden, weight, labels, temperature: float = 1.0):
+    """hidden (T,H) bf16, weight (V,H) bf16, labels (T,) int64 -> (logp (T,) f32, lse (T,) f32) of z = hidden @ weight^T / temperature, whose
+    logits are never stored.  Labels outside [0, V): rows that are not scored (logp 0)."""
+    T, V, H = _head_operands(hidden, weight, temperature)
+    _vec(labels, I64, (T,), "labels"); _on(hidden.device, (labels, "labels"))
+    with torch.cuda.device(hidden.device):
+        logp = torch.empty(T, dtype=F32, device=hidden.device)
+        lse = torch.empty(T, dtype=F32, device=hidden.device)
+        if T:
+            ws = _head_workspace(T, V, H, 0, False, hidden.device)
+            lib().st_linear_logprob_fwd(_p(hidden), hidden.stride(0), _p(weight), weight.stride(0), _p(labels), 1.0 / temperature, _p(logp), _p(lse),
+                                        _p(ws), ws.numel(), T, V, H, _s())
+    return logp, lse
+
+
+def linear_logprob_bwd(hidden, weight, labels, logp, lse, g, temperature: float = 1.0, *, want_dhidden=True, dweight=None, dweight_f32=None, accumulate=False):
+    """Gradients of sum(g * logp): returns dhidden (T,H) bf16 (None unless wanted); dweight (bf16, overwritten) or dweight_f32 (fp32, accumulate:
+    added to) is filled in place."""
+    T, V, H = _head_operands(hidden, weight, temperature)
+    for t, dt, what in ((labels, I64, "labels"), (logp, F32, "logp"), (lse, F32, "lse"), (g, F32, "g")):
+        _vec(t, dt, (T,), what); _on(hidden.device, (t, what))
+    with torch.cuda.device(hidden.device):
+        dh = _head_grads(hidden, weight, want_dhidden, dweight, dweight_f32, accumulate)
+        ws = _head_workspace(T, V, H, 0, True, hidden.device)
+        lib().st_linear_logprob_bwd(_p(hidden), hidden.stride(0), _p(weight), weight.stride(0), _p(labels), _p(logp), _p(lse), _p(g), 1.0 / temperature,
+                                    _p(dh), _ld(dh), _p(dweight), _p(dweight_f32), _ld(dweight if dweight is not None else dweight_f32),
+                                    int(accumulate), _p(ws), ws.numel(), T, V, H, _s())
+    return dh
+
+
+def _topk_targets(hidden, ids, teacher_logp, T):
+    if ids.dim() != 2 or ids.shape[0] != T or not 1 <= ids.shape[1] <= HEAD_MAX_TARGETS:
+        raise ValueError(f"ids: expected ({T}, 1..{HEAD_MAX_TARGETS}), got {tuple(ids.shape)}")
+    if ids.numel() >= 1 << 31:
+        raise ValueError(f"ids: fewer than 2^31 entries, got {tuple(ids.shape)}")
+    _vec(ids, I32, ids.shape, "ids"); _vec(teacher_logp, F32, ids.shape, "teacher_logp")
+    _on(hidden.device, (ids, "ids"), (teacher_logp, "teacher_logp"))
+    return ids.shape[1]
+
+
+def linear_topk_kl_fwd(hidden, weight, ids, teacher_logp, temperature: float = 1.0, renormalize: bool = False):
+    """ids (T,K) int32, teacher_logp (T,K) f32 -> (kl (T,) f32, lse (T,) f32, logq (T,K) f32): kl = sum_k p_k (log p_k - log q[ids_k]) with
+    p = exp(teacher_logp), or its softmax over the row's entries; entries with an id outside [0, V) are absent (st_linear_topk_kl_fwd)."""
+    T, V, H = _head_operands(hidden, weight, temperature)
+    K = _topk_targets(hidden, ids, teacher_logp, T)
+    with torch.cuda.device(hidden.device):
+        kl = torch.empty(T, dtype=F32, device=hidden.device)
+        lse = torch.empty(T, dtype=F32, device=hidden.device)
+        logq = torch.empty(T, K, dtype=F32, device=hidden.device)
+        if T:
+            ws = _head_workspace(T, V, H, K, False, hidden.device)
+            lib().st_linear_topk_kl_fwd(_p(hidden), hidden.stride(0), _p(weight), weight.stride(0), _p(ids), _p(teacher_logp), K, int(renormalize),
+                                        1.0 / temperature, _p(kl), _p(lse), _p(logq), _p(ws), ws.numel(), T, V, H, _s())
+    return kl, lse, logq
+
+
+def linear_topk_kl_bwd(hidden, weight, ids, teacher_logp, lse, logq, g, temperature: float = 1.0, renormalize: bool = False, *, want_dhidden=True,
+                       dweight=None, dweight_f32=None, accumulate=False):
+    """Gradients of sum(g * kl); outputs as linear_logprob_bwd."""
+    T, V, H = _head_operands(hidden, weight, temperature)
+    K = _topk_targets(hidden, ids, teacher_logp, T)
+    for t, shape, what in ((lse, (T,), "lse"), (logq, (T, K), "logq"), (g, (T,), "g")):
+        _vec(t, F32, shape, what); _on(hidden.device, (t, what))
+    with torch.cuda.device(hidden.device):
+        dh = _head_grads(hidden, weight, want_dhidden, dweight, dweight_f32, accumulate)
+        ws = _head_workspace(T, V, H, K, True, hidden.device)
+        lib().st_linear_topk_kl_bwd(_p(hidden), hidden.stride(0), _p(weight), weight.stride(0), _p(ids), _p(teacher_logp), K, int(renormalize),
+                                    1.0 / temperature, _p(lse), _p(logq), _p(g), _p(dh), _ld(dh), _p(dweight), _p(dweight_f32),
+                                    _ld(dweight if dweight is not None else dweight_f32), int(accumulate), _p(ws), ws.numel(), T, V, H, _s())
+    return dh
+
+
+def topk_logprob(logits, k: int, temperature: float = 1.0):
+    """logits (T,V) bf16 -> (ids (T,k) int32, logp (T,k) f32, lse (T,) f32): the k largest log-probs of logits / temperature per row in falling
+    order, equal logits by rising id."""
+    import ctypes
+    _chk(logits, BF16, "logits")
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"logits: expected (T, V), got {tuple(logits.shape)}")
+    T, V = logits.shape
+    if not 1 <= k <= min(TOPK_MAX, V):
+        raise ValueError(f"k must be in 1..{min(TOPK_MAX, V)}, got {k}")
+    if T > 1 and logits.stride(0) < V:
+        raise ValueError(f"logits: rows overlap (stride {logits.stride(0)})")
+    if not (temperature > 0.0 and math.isfinite(temperature) and math.isfinite(1.0 / temperature)):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    _p(logits)
+    with torch.cuda.device(logits.device):
+        ids = torch.empty(T, k, dtype=I32, device=logits.device)
+        logp = torch.empty(T, k, dtype=F32, device=logits.device)
+        lse = torch.empty(T, dtype=F32, device=logits.device)
+        if T:
+            n = ctypes.c_int64(0)
+            lib().st_topk_logprob_workspace_bytes(T, V, k, ctypes.addressof(n), None)
+            ws = torch.empty(n.value, dtype=torch.uint8, device=logits.device) if n.value else None
+            lib().st_topk_logprob(_p(logits), max(logits.stride(0), V), k, 1.0 / temperature, _p(ids), _p(logp), _p(lse), _p(ws), n.value, T, V, _s())
+    return ids, logp, lse
+
+
 # ------------------------------------------------------------------ norms / rope / activations
 def rmsnorm_fwd(x, w, eps, want_rstd=True, out=None):
     _chk(x, BF16, "x"); _chk(w, BF16, "w")

@@ -1,0 +1,100 @@
+"""What the vocabulary-head operators refuse, without a GPU: the argument checks come before any launch."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+BF16 = torch.bfloat16
+
+
+def args(T=4, H=64, V=10, dtype=BF16):
+    return torch.zeros(T, H, dtype=dtype), torch.zeros(V, H, dtype=dtype), torch.zeros(T, dtype=torch.int64)
+
+
+def test_cpu_tensors_are_refused_not_computed_elsewhere():
+    from spatialthinker_amd import ops
+    from verl.utils import torch_functional as VF
+    h, w, lab = args()
+    with pytest.raises(RuntimeError, match="not on a GPU"):
+        ops.linear_logprob_fwd(h, w, lab)
+    with pytest.raises(RuntimeError, match="not on a GPU"):
+        VF.linear_log_probs(h, w, lab)
+    with pytest.raises(RuntimeError, match="not on a GPU"):
+        VF.linear_topk_kl(h, w, torch.zeros(4, 3, dtype=torch.int32), torch.zeros(4, 3))
+    with pytest.raises(RuntimeError, match="not on a GPU"):
+        VF.top_log_probs(torch.zeros(2, 50), 3)
+
+
+@pytest.mark.parametrize("temperature", [0.0, -1.0, math.inf, math.nan, 1e-320])
+def test_temperature(temperature):
+    from spatialthinker_amd import ops
+    h, w, lab = args()
+    with pytest.raises(ValueError, match="temperature"):
+        ops.linear_logprob_fwd(h, w, lab, temperature)
+    with pytest.raises(ValueError, match="temperature"):
+        ops.topk_logprob(w, 3, temperature)
+
+
+def test_types_and_shapes():
+    from spatialthinker_amd import ops
+    from verl.utils import torch_functional as VF
+    h, w, lab = args()
+    with pytest.raises(TypeError):
+        ops.linear_logprob_fwd(h.float(), w, lab)
+    with pytest.raises(TypeError):
+        ops.linear_logprob_fwd(h, w.half(), lab)
+    with pytest.raises(ValueError):
+        ops.linear_logprob_fwd(*args(H=72)[:2], lab)               # width not a multiple of 64
+    with pytest.raises(ValueError):
+        ops.linear_logprob_fwd(h, torch.zeros(10, 128, dtype=BF16), lab)
+    with pytest.raises(ValueError):
+        ops.linear_logprob_fwd(h, torch.zeros(0, 64, dtype=BF16), lab)
+    with pytest.raises(ValueError):                                # rows that are not 16-byte aligned
+        ops.linear_logprob_fwd(torch.zeros(4, 65, dtype=BF16)[:, :64], w, lab)
+    with pytest.raises(ValueError):
+        ops.linear_logprob_fwd(torch.zeros(1, 64, dtype=BF16).expand(4, 64), w, lab)       # rows that overlap
+    with pytest.raises(ValueError):
+        VF.linear_log_probs(h, w, lab[:3])
+    with pytest.raises(ValueError):
+        VF.linear_topk_kl(h, w, torch.zeros(4, 3, dtype=torch.int32), torch.zeros(4, 2))
+    with pytest.raises(ValueError):
+        VF.linear_topk_kl(h, w, torch.zeros(5, 3, dtype=torch.int32), torch.zeros(5, 3))
+    for k in (0, 11, -1):
+        with pytest.raises(ValueError):
+            ops.topk_logprob(torch.zeros(2, 10, dtype=BF16), k)
+    with pytest.raises(ValueError):
+        ops.topk_logprob(torch.zeros(2, 1000, dtype=BF16), 257)
+    with pytest.raises(TypeError):
+        ops.topk_logprob(torch.zeros(2, 1000), 2)
+    with pytest.raises(ValueError):
+        ops.topk_logprob(torch.zeros(1, 1000, dtype=BF16).expand(2, 1000), 2)
+
+
+def test_c_entries_return_einval_before_any_launch():
+    from spatialthinker_amd.lib import lib
+    L = lib()
+    n = ctypes.c_int64(0)
+    at = ctypes.addressof(n)
+    assert L.st_linear_head_workspace_bytes.raw(8, 1000, 64, 4, 1, at, None) == 0 and n.value > 0
+    small = n.value
+    assert L.st_linear_head_workspace_bytes.raw(8, 1000, 64, 4, 0, at, None) == 0 and n.value > 0
+    for T, V, H, K in ((-1, 10, 64, 0), (8, 0, 64, 0), (8, 10, 0, 0), (8, 10, 65, 0), (8, 10, 64, 1025), (8, 10, 64, -1), (8, (1 << 22) + 1, 64, 0)):
+        assert L.st_linear_head_workspace_bytes.raw(T, V, H, K, 1, at, None) == -22
+    p = 1 << 20                                                    # never touched: every call below is refused
+    fwd = lambda h=p, ldh=64, w=p, ldw=64, lab=p, it=1.0, ws=p, nb=1 << 40, T=8, V=1000, H=64: L.st_linear_logprob_fwd.raw(
+        h, ldh, w, ldw, lab, it, p, p, ws, nb, T, V, H, None)
+    for bad in (dict(h=None), dict(w=None), dict(lab=None), dict(ldh=63), dict(ldw=68), dict(ldh=56), dict(ldw=1 << 22), dict(h=p + 2), dict(w=p + 8),
+                dict(it=0.0), dict(it=-1.0), dict(it=math.inf), dict(it=math.nan), dict(ws=None), dict(nb=small // 1000), dict(T=-1), dict(V=0), dict(H=65)):
+        assert fwd(**bad) == -22, bad
+    bwd = lambda dh=p, lddh=64, db=None, df=None, lddw=64, acc=0, ws=p, nb=1 << 40: L.st_linear_logprob_bwd.raw(
+        p, 64, p, 64, p, p, p, p, 1.0, dh, lddh, db, df, lddw, acc, ws, nb, 8, 1000, 64, None)
+    for bad in (dict(dh=p + 2), dict(lddh=63), dict(lddh=60), dict(db=p, df=p), dict(db=p, acc=1), dict(db=p, lddw=66), dict(df=p, lddw=62), dict(df=p + 4),
+                dict(ws=None), dict(nb=small - 1)):
+        assert bwd(**bad) == -22, bad
+    kl = lambda K=4, ids=p, a=p, ws=p, T=8: L.st_linear_topk_kl_fwd.raw(p, 64, p, 64, ids, a, K, 0, 1.0, p, p, p, ws, 1 << 40, T, 1000, 64, None)
+    for bad in (dict(K=0), dict(K=1025), dict(ids=None), dict(a=None), dict(ws=None), dict(K=1024, T=1 << 21)):
+        assert kl(**bad) == -22, bad
+    top = lambda z=p, ldl=1000, k=5, it=1.0, ws=p, nb=1 << 40, T=8, V=1000: L.st_topk_logprob.raw(z, ldl, k, it, p, p, p, ws, nb, T, V, None)
+    for bad in (dict(z=None), dict(z=p + 1), dict(ldl=999), dict(k=0), dict(k=257), dict(k=6, V=5, ldl=5), dict(it=0.0), dict(T=-1), dict(V=0)):
+        assert top(**bad) == -22, bad

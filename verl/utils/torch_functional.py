@@ -122,6 +122,103 @@ def log_probs_from_logits_flash_attn(logits: torch.Tensor, labels: torch.Tensor)
     return log_probs_from_logits(logits, labels)
 
 
+class _LinearLogProbs(torch.autograd.Function):
+    """log-probs of given tokens from hidden states and head weight, the logits never stored (st_linear_logprob_fwd / _bwd).  The backward forms
+    the logits again, piece by piece of the vocabulary; only the gradients that autograd asks for are computed."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, labels, temperature):
+        from spatialthinker_amd import ops
+        logp, lse = ops.linear_logprob_fwd(hidden, weight, labels, temperature)
+        ctx.save_for_backward(hidden, weight, labels, logp, lse)
+        ctx.temperature = temperature
+        return logp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        from spatialthinker_amd import ops
+        hidden, weight, labels, logp, lse = ctx.saved_tensors
+        dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if ctx.needs_input_grad[1] else None
+        dh = ops.linear_logprob_bwd(hidden, weight, labels, logp, lse, grad_out.contiguous().float(), ctx.temperature,
+                                    want_dhidden=ctx.needs_input_grad[0], dweight=dw)
+        return dh, dw, None, None
+
+
+class _LinearTopkKL(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, ids, teacher, temperature, renormalize):
+        from spatialthinker_amd import ops
+        kl, lse, logq = ops.linear_topk_kl_fwd(hidden, weight, ids, teacher, temperature, renormalize)
+        ctx.save_for_backward(hidden, weight, ids, teacher, lse, logq)
+        ctx.temperature, ctx.renormalize = temperature, renormalize
+        return kl
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        from spatialthinker_amd import ops
+        hidden, weight, ids, teacher, lse, logq = ctx.saved_tensors
+        dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if ctx.needs_input_grad[1] else None
+        dh = ops.linear_topk_kl_bwd(hidden, weight, ids, teacher, lse, logq, grad_out.contiguous().float(), ctx.temperature, ctx.renormalize,
+                                    want_dhidden=ctx.needs_input_grad[0], dweight=dw)
+        return dh, dw, None, None, None, None
+
+
+def _head_rows(hidden: torch.Tensor, weight: torch.Tensor):
+    """(rows of hidden (T, H), weight) as the head kernels take them: bf16, rows contiguous and 16-byte aligned (a copy only where they are not).
+    Both casts are differentiable: fp32 inputs get fp32 gradients."""
+    def rows(t):
+        t = t.to(torch.bfloat16)
+        ok = t.shape[0] == 0 or (t.stride(-1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0)
+        return t if ok else t.clone(memory_format=torch.contiguous_format)
+    return rows(hidden.reshape(-1, hidden.shape[-1])), rows(weight)
+
+
+def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
+    """log_probs_from_logits(hidden @ weight^T / temperature, labels) without the logits: hidden (..., H), weight (V, H) (the head), labels (...)
+    -> (...) fp32, differentiable in hidden and weight.  At V = 152 064 the logits of 8192 rows are 2.5 GB; here the backward's workspace stays
+    within 0.5 GiB for one piece of the vocabulary and the logits stay in fp32.  A label outside [0, V) (padding, -100) marks a row that is not
+    scored: 0, and no gradient from it.  H must be a multiple of 64; GPU tensors only."""
+    h, w = _head_rows(hidden, weight)
+    if labels.shape != hidden.shape[:-1]:
+        raise ValueError(f"labels {tuple(labels.shape)} do not match hidden {tuple(hidden.shape)}")
+    lab = labels.to(device=h.device, dtype=torch.int64).contiguous().view(-1)
+    return _LinearLogProbs.apply(h, w, lab, float(temperature)).view(labels.shape)
+
+
+def linear_topk_kl(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor, teacher_log_probs: torch.Tensor, temperature: float = 1.0,
+                   renormalize: bool = False) -> torch.Tensor:
+    """Distillation from a teacher's top log-probs (top_log_probs), per row, without the student's logits:
+        kl[t] = sum_k p_k (log p_k - log softmax(hidden_t @ weight^T / temperature)[id_k]),   p = exp(teacher_log_probs)
+    hidden (..., H), weight (V, H), teacher_ids / teacher_log_probs (..., K) -> (...) fp32, differentiable in hidden and weight (the teacher is a
+    constant).  renormalize: p is scaled to sum 1 over the row's entries; without it the mass outside the teacher's top K counts for nothing.
+    Entries with an id outside [0, V) are absent; a row of such entries gives 0 and no gradient.  K <= 1024."""
+    h, w = _head_rows(hidden, weight)
+    if teacher_ids.shape[:-1] != hidden.shape[:-1] or teacher_ids.shape != teacher_log_probs.shape:
+        raise ValueError(f"teacher ids {tuple(teacher_ids.shape)} / log-probs {tuple(teacher_log_probs.shape)} do not match hidden {tuple(hidden.shape)}")
+    k = teacher_ids.shape[-1]
+    if teacher_ids.dtype != torch.int32:                         # int64 ids that int32 cannot hold must stay outside [0, V)
+        teacher_ids = teacher_ids.clamp(-1, 0x7fffffff).to(torch.int32)
+    ids = teacher_ids.to(h.device).contiguous().view(-1, k)
+    a = teacher_log_probs.detach().to(device=h.device, dtype=torch.float32).contiguous().view(-1, k)
+    return _LinearTopkKL.apply(h, w, ids, a, float(temperature), bool(renormalize)).view(hidden.shape[:-1])
+
+
+@torch.no_grad()
+def top_log_probs(logits: torch.Tensor, k: int, temperature: float = 1.0):
+    """The k largest log-probs of logits / temperature: logits (..., V) -> (ids (..., k) int32, log-probs (..., k) fp32, lse (...) fp32), in falling
+    order, equal logits by rising id.  What a teacher hands to linear_topk_kl.  bf16 logits (anything else is rounded to bf16 first, as
+    log_probs_from_logits does); k <= 256."""
+    batch_dim, vocab = logits.shape[:-1], logits.shape[-1]
+    z = logits.to(torch.bfloat16).reshape(-1, vocab)
+    if z.stride(-1) != 1:
+        z = z.contiguous()
+    from spatialthinker_amd import ops
+    ids, logp, lse = ops.topk_logprob(z, int(k), float(temperature))
+    return ids.view(*batch_dim, k), logp.view(*batch_dim, k), lse.view(batch_dim)
+
+
 def get_constant_schedule_with_warmup(optimizer: torch.optim.Optimizer, num_warmup_steps: int, last_epoch: int = -1):
     """:187-197 — lr * min(1, step / max(1, num_warmup_steps)); step 0 of a zero-warm-up schedule therefore trains at lr = 0
     (PolicyEngine.current_lr reproduces the same multiplier on its own counter)."""
