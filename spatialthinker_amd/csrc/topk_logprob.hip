@@ -8,9 +8,9 @@
 // per-thread maxima is reached by at least k values, so whatever lies below it can be dropped: this threshold rises as the maxima grow and
 // after the first segment only a few hundred of a row's 150 000 values pass it and go into a candidate list in LDS.  A list that would
 // overflow (values that rise along the row) is cut back to its k largest first, so the result does not depend on the order of the
-// values.  Values are ordered as whole numbers: bf16 bits mapped to a signed 16-bit order (-0 equals +0, NaN by its bits beyond the
-// infinities), the id below them in the 64-bit key, which makes every key different and ties go to the lower id.
-// The exponential sum runs over the same registers.
+// values.  The walk compares floats; candidates carry a 64-bit key of the value's order as a whole number (-0 equals +0) over the falling id,
+// which makes every key different and ties go to the lower id.  NaN passes no comparison; it makes the row's lse NaN, and such a row is
+// answered without its candidates.  The exponential sum runs over the same registers.
 #include "common.h"
 #include <algorithm>
 
@@ -21,16 +21,11 @@
 #define TK_SEG 4                               // loads per segment: the threshold is renewed once per segment
 #define TK_MAX_K 256
 #define TK_CAP (TK_CHUNK + TK_MAX_K)           // candidates: what is kept plus one whole chunk (+ the values in front of and behind the granules)
-#define TK_NONE (-32769)                       // below every value's order
+#define TK_NONE (-32640)                       // the order of -inf: every value passes
 
 __device__ __forceinline__ int tk_order(uint16_t b) {                    // bf16 bits -> signed order, -0 = +0
     const int mag = b & 0x7fff;
     return (b & 0x8000) ? -mag : mag;
-}
-typedef short tk_short2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ tk_short2 tk_order2(uint32_t w) {             // the same for two values at once (packed 16-bit integer instructions)
-    const tk_short2 sign = __builtin_bit_cast(tk_short2, w) >> (short)15, mag = __builtin_bit_cast(tk_short2, w & 0x7fff7fffu);
-    return (mag ^ sign) - sign;
 }
 __device__ __forceinline__ float tk_value(int order) {
     const int mag = order < 0 ? -order : order;
@@ -38,12 +33,15 @@ __device__ __forceinline__ float tk_value(int order) {
 }
 __device__ __forceinline__ uint64_t tk_key(int order, uint32_t id) { return ((uint64_t)(uint32_t)(order + 32768) << 32) | (0xffffffffu - id); }
 
+#define TK_BINS 1024                           // orders told apart below the largest candidate when the list is ranked
+
 struct TkShared {
     uint64_t cand[TK_CAP + 16];
-    uint64_t best[TK_MAX_K];
+    uint64_t best[2 * TK_MAX_K];
     int maxima[TK_THREADS];
     float2 red[TK_THREADS / 64];
     int count, thr, scan[TK_THREADS / 64];
+    int bins[TK_BINS];
 };
 
 // number of threads of the workgroup for which `p` holds, summed with `n` per thread; a barrier on both sides
@@ -81,12 +79,52 @@ __device__ __forceinline__ void tk_cut(TkShared& sh, int n, int k) {
     __syncthreads();
 }
 
-// the list's k largest in falling order -> best[0 .. k): n >= k
+// the list's k largest in falling order -> best[0 .. k), or all of them where n < k.  Counts per order value first: only what is at least the k-th
+// largest value is ranked (k and its ties) instead of all n candidates against each other.
 __device__ __forceinline__ void tk_rank(TkShared& sh, int n, int k) {
-    if (n > 2 * TK_THREADS) { tk_cut(sh, n, k); n = k; }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (n > 2 * k && n > 128) {
+        int most = 0;                                                    // the largest order (+32768)
+        for (int j = threadIdx.x; j < n; j += TK_THREADS) most = max(most, (int)(sh.cand[j] >> 32));
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+        if (lane == 0) sh.scan[wave] = most;
+        sh.bins[threadIdx.x] = 0; sh.bins[threadIdx.x + TK_THREADS] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TK_THREADS / 64; ++i) most = max(most, sh.scan[i]);
+        for (int j = threadIdx.x; j < n; j += TK_THREADS) atomicAdd(&sh.bins[min(most - (int)(sh.cand[j] >> 32), TK_BINS - 1)], 1);
+        __syncthreads();
+        // bin 0 holds the largest value: the first bin up to which at least k candidates lie
+        const int c0 = sh.bins[2 * threadIdx.x], c1 = sh.bins[2 * threadIdx.x + 1];
+        int x = c0 + c1;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const int y = __shfl_up(x, o, 64); x += lane >= o ? y : 0; }
+        if (lane == 63) sh.scan[wave] = x;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TK_THREADS / 64; ++i) x += i < wave ? sh.scan[i] : 0;
+        if (x >= k && x - c1 - c0 < k) { sh.maxima[0] = x - c1 >= k ? 2 * threadIdx.x : 2 * threadIdx.x + 1; sh.maxima[1] = x - c1 >= k ? x - c1 : x; }
+        __syncthreads();
+        const int last = sh.maxima[0], left = sh.maxima[1];
+        if (left <= 2 * TK_MAX_K) {
+            if (threadIdx.x == 0) sh.count = 0;
+            __syncthreads();
+            for (int j = threadIdx.x; j < n; j += TK_THREADS)
+                if (most - (int)(sh.cand[j] >> 32) <= last) sh.best[atomicAdd(&sh.count, 1)] = sh.cand[j];
+            __syncthreads();
+            for (int j = threadIdx.x; j < left; j += TK_THREADS) sh.cand[j] = sh.best[j];
+            n = left;
+        } else {                                                         // many equal values: the lowest ids among them, by bisection
+            tk_cut(sh, n, k);
+            n = k;
+        }
+        __syncthreads();
+    }
     for (int j = threadIdx.x; j < n; j += TK_THREADS) {
         const uint64_t key = sh.cand[j];
         int rank = 0;
+#pragma unroll 4
         for (int i = 0; i < n; ++i) rank += sh.cand[i] > key ? 1 : 0;
         if (rank < k) sh.best[rank] = key;
     }
@@ -113,8 +151,8 @@ __device__ __forceinline__ void tk_write(TkShared& sh, int k, float2 ms, float i
     const float l = (ms.x + log2f(ms.y)) * TK_LN2;
     if (threadIdx.x == 0) *lse = l;
     for (int j = threadIdx.x; j < k; j += TK_THREADS) {
-        const uint64_t key = sh.best[j];
-        ids[j] = (int32_t)(0xffffffffu - (uint32_t)key);
+        const uint64_t key = l == l ? sh.best[j] : 0;
+        ids[j] = l == l ? (int32_t)(0xffffffffu - (uint32_t)key) : j;
         logp[j] = tk_value((int)(key >> 32) - 32768) * inv_temp - l;
     }
 }
@@ -135,137 +173,206 @@ __global__ __launch_bounds__(TK_THREADS, 4) void topk_row_kernel(const uint16_t*
     const int back = n - front - granules * 8;
     const uint4* body = reinterpret_cast<const uint4*>(x + beg + front);
     if (threadIdx.x == 0) { sh.count = 0; sh.thr = TK_NONE; }
-    int thr = TK_NONE, top = TK_NONE;                                    // values <= thr are out; this thread's largest so far
-    float m = -INFINITY, s = 0.f;
+    int thr = TK_NONE;                                                   // values of a lower order are out
+    float top = -INFINITY, m = -INFINITY, s = 0.f;                       // this thread's largest so far; base-2 maximum and sum
+    bool any = false;                                                    // this thread has met a value
     __syncthreads();
     auto single = [&](int e) {                                           // one value outside the granules; the list has room for these
-        const uint16_t b = x[beg + e];
-        const int o = tk_order(b);
-        top = max(top, o);
-        if (o > thr) sh.cand[atomicAdd(&sh.count, 1)] = tk_key(o, (uint32_t)(beg + e));
-        const float f = bf2f(b);
+        const float f = bf2f(x[beg + e]);
+        any = true;
+        top = fmaxf(top, f);
+        if (f >= tk_value(thr)) sh.cand[atomicAdd(&sh.count, 1)] = tk_key(tk_order(x[beg + e]), (uint32_t)(beg + e));
         const float2 v = tk_join(make_float2(m, s), make_float2(f * sc, f == -INFINITY ? 0.f : f == f ? 1.f : f));
         m = v.x; s = v.y;
     };
     if ((int)threadIdx.x < front) single(threadIdx.x);
-    for (int g0 = 0; g0 < granules; g0 += TK_THREADS * TK_SEG) {
-        uint4 r[TK_SEG];
+    uint4 r[TK_SEG], ahead[TK_SEG];
+    auto fetch = [&](int g0) {                                           // unconditional loads (the waits can be counted): past the end the last granule
 #pragma unroll
-        for (int c = 0; c < TK_SEG; ++c) {
-            const int g = g0 + c * TK_THREADS + threadIdx.x;
-            r[c] = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);       // no granule: -inf adds nothing to the sum
-            if (g < granules) r[c] = body[g];
+        for (int c = 0; c < TK_SEG; ++c) ahead[c] = body[min(g0 + c * TK_THREADS + (int)threadIdx.x, granules - 1)];
+    };
+    if (granules) fetch(0);
+    for (int g0 = 0, seg = 0; g0 < granules; g0 += TK_THREADS * TK_SEG, ++seg) {
+#pragma unroll
+        for (int c = 0; c < TK_SEG; ++c) r[c] = ahead[c];
+        fetch(g0 + TK_THREADS * TK_SEG);                                 // the next segment flies while this one is worked on
+        if (g0 + TK_THREADS * TK_SEG > granules) {                       // no granule: -inf adds nothing to the sum
+#pragma unroll
+            for (int c = 0; c < TK_SEG; ++c)
+                if (g0 + c * TK_THREADS + (int)threadIdx.x >= granules) r[c] = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
         }
-        int cmax[TK_SEG];
+        float cmax[TK_SEG], most = -INFINITY;
 #pragma unroll
         for (int c = 0; c < TK_SEG; ++c) {
-            const tk_short2 mx = __builtin_elementwise_max(__builtin_elementwise_max(tk_order2(r[c].x), tk_order2(r[c].y)),
-                                                           __builtin_elementwise_max(tk_order2(r[c].z), tk_order2(r[c].w)));
-            cmax[c] = g0 + c * TK_THREADS + (int)threadIdx.x < granules ? max((int)mx.x, (int)mx.y) : TK_NONE;
-            top = max(top, cmax[c]);
             float f[8];
             unpack8(r[c], f);
-            float vm = f[0];
-#pragma unroll
-            for (int j = 1; j < 8; ++j) vm = fmaxf(vm, f[j]);
-            vm *= sc;                                                    // sc > 0
+            cmax[c] = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+            most = fmaxf(most, cmax[c]);
+        }
+        top = fmaxf(top, most);
+        any = any || g0 + (int)threadIdx.x < granules;
+        {   // the exponential sum of the segment's 8 * TK_SEG values, base 2
+            const float vm = most * sc;                                  // sc > 0
             if (vm > m) { s *= __builtin_amdgcn_exp2f(m - vm); m = vm; }
             const float sub = m == -INFINITY ? 0.f : m;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s += __builtin_amdgcn_exp2f(fmaf(f[j], sc, -sub));
+            for (int c = 0; c < TK_SEG; ++c) {
+                float f[8], a = 0.f;
+                unpack8(r[c], f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) a += __builtin_amdgcn_exp2f(fmaf(f[j], sc, -sub));
+                s += a;
+            }
         }
-        // the threshold: the k-th largest per-thread maximum (fewer than k threads with values: none yet).  One wave bisects the 16-bit order.
-        sh.maxima[threadIdx.x] = top;
-        __syncthreads();
-        if (threadIdx.x < 64) {
-            int mine[TK_THREADS / 64];
+        // the threshold: the k-th largest per-thread maximum (fewer than k threads with values: none yet), renewed in segments 0, 1, 3, 7, ...: by then the
+        // maxima have seen twice as many values.  One wave bisects the 16-bit order.
+        if ((seg & (seg + 1)) == 0) {
+            sh.maxima[threadIdx.x] = any ? tk_order((uint16_t)(__float_as_uint(top) >> 16)) : TK_NONE - 1;
+            __syncthreads();
+            if (threadIdx.x < 64) {
+                int mine[TK_THREADS / 64];
 #pragma unroll
-            for (int i = 0; i < TK_THREADS / 64; ++i) mine[i] = sh.maxima[lane + i * 64] + 32768;      // -1: no value
-            int t = 0, c0 = 0;
+                for (int i = 0; i < TK_THREADS / 64; ++i) mine[i] = sh.maxima[lane + i * 64] - TK_NONE;     // -1: no value
+                int c0 = 0, lo = 0x7fffffff, hi = -1;
 #pragma unroll
-            for (int i = 0; i < TK_THREADS / 64; ++i) c0 += __popcll(__ballot(mine[i] >= 0));
-            if (c0 >= want) {
+                for (int i = 0; i < TK_THREADS / 64; ++i) {
+                    c0 += __popcll(__ballot(mine[i] >= 0));
+                    lo = min(lo, mine[i]); hi = max(hi, mine[i]);
+                }
+                if (c0 >= want) {
+#pragma unroll
+                    for (int o = 32; o > 0; o >>= 1) { lo = min(lo, __shfl_xor(lo, o, 64)); hi = max(hi, __shfl_xor(hi, o, 64)); }
+                    lo = __builtin_amdgcn_readfirstlane(max(lo, 0)); hi = __builtin_amdgcn_readfirstlane(hi);
 #pragma unroll 1
-                for (int b = 15; b >= 0; --b) {
-                    int c = 0;
+                    while (lo < hi) {                                    // the largest value that at least `want` maxima reach is in [lo, hi]
+                        const int mid = (lo + hi + 1) >> 1;
+                        int c = 0;
 #pragma unroll
-                    for (int i = 0; i < TK_THREADS / 64; ++i) c += __popcll(__ballot(mine[i] >= (t | (1 << b))));
-                    if (c >= want) t |= 1 << b;
+                        for (int i = 0; i < TK_THREADS / 64; ++i) c += __popcll(__ballot(mine[i] >= mid));
+                        if (c >= want) lo = mid; else hi = mid - 1;
+                    }
+                    if (lane == 0) sh.thr = lo + TK_NONE;                // values equal to the k-th maximum stay
                 }
-                if (lane == 0) sh.thr = t - 32768 - 1;                   // values equal to the k-th maximum stay
             }
+            __syncthreads();
+            thr = max(thr, sh.thr);
         }
-        __syncthreads();
-        thr = max(thr, sh.thr);
+        const int have = sh.count;                                       // the same for every thread: appended to only behind the next barrier
+        float ge = tk_value(thr);
+        if (!__syncthreads_or(most >= ge && g0 + (int)threadIdx.x < granules)) continue;
+        auto there = [&](int c) { return cmax[c] >= ge && g0 + c * TK_THREADS + (int)threadIdx.x < granules; };
+        auto passing = [&](const uint4& w) {
+            float f[8];
+            unpack8(w, f);
+            int n = 0;
 #pragma unroll
-        for (int c = 0; c < TK_SEG; ++c) {
-            const int have = sh.count;                                   // the same for every thread: appended to only behind the next barrier
-            if (!__syncthreads_or(cmax[c] > thr)) continue;
-            const int e = front + (g0 + c * TK_THREADS + (int)threadIdx.x) * 8;
-            const uint32_t w[4] = {r[c].x, r[c].y, r[c].z, r[c].w};
-            if (have + TK_CHUNK > TK_CAP) {                              // a whole chunk might not fit: count what would be added
-                int mine = 0;
-                if (cmax[c] > thr)
+            for (int j = 0; j < 8; ++j) n += f[j] >= ge ? 1 : 0;
+            return n;
+        };
+        auto append = [&](int c, const uint4& w) {
+            const uint32_t id = (uint32_t)(beg + front + (g0 + c * TK_THREADS + (int)threadIdx.x) * 8);
+            float f[8];
+            unpack8(w, f);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) mine += tk_order((uint16_t)(w[j >> 1] >> ((j & 1) * 16))) > thr ? 1 : 0;
-                if (have + tk_block_sum(sh, mine) > TK_CAP) {
-                    // have > TK_MAX_K >= want here (a chunk adds <= TK_CHUNK): the k largest survive, the smallest of them is the new threshold
-                    tk_cut(sh, have, want);
-                    int lo = 0x7fffffff;
-                    for (int j = threadIdx.x; j < want; j += TK_THREADS) lo = min(lo, (int)(sh.cand[j] >> 32) - 32768);
+            for (int j = 0; j < 8; ++j)
+                if (f[j] >= ge) sh.cand[atomicAdd(&sh.count, 1)] = tk_key(tk_order((uint16_t)(__float_as_uint(f[j]) >> 16)), id + j);
+        };
+        int mine = 0;
+        if (most >= ge)
 #pragma unroll
-                    for (int o = 32; o > 0; o >>= 1) lo = min(lo, __shfl_xor(lo, o, 64));
-                    if (lane == 0) sh.scan[threadIdx.x >> 6] = lo;
-                    __syncthreads();
+            for (int c = 0; c < TK_SEG; ++c) if (there(c)) mine += passing(r[c]);
+        if (have + tk_block_sum(sh, mine) <= TK_CAP) {                   // the usual case
+            if (most >= ge)
 #pragma unroll
-                    for (int i = 0; i < TK_THREADS / 64; ++i) lo = min(lo, sh.scan[i]);
-                    thr = max(thr, lo);                                  // an equal value further on has a higher id: out
-                    __syncthreads();
-                }
+                for (int c = 0; c < TK_SEG; ++c) if (there(c)) append(c, r[c]);
+            __syncthreads();
+            continue;
+        }
+#pragma unroll 1
+        for (int c = 0; c < TK_SEG; ++c) {                               // load by load: ids rise from one to the next
+            const int g = g0 + c * TK_THREADS + (int)threadIdx.x;
+            const bool here = g < granules;
+            const uint4 w = body[min(g, granules - 1)];                  // once more from memory: a rare path must not hold the segment's registers
+            const int now = sh.count;
+            if (now + tk_block_sum(sh, here ? passing(w) : 0) > TK_CAP) {
+                // now > TK_MAX_K >= want here (a load adds <= TK_CHUNK): the k largest survive, the smallest of them is the new threshold
+                tk_cut(sh, now, want);
+                int lo = 0x7fffffff;
+                for (int j = threadIdx.x; j < want; j += TK_THREADS) lo = min(lo, (int)(sh.cand[j] >> 32) - 32768);
+#pragma unroll
+                for (int o = 32; o > 0; o >>= 1) lo = min(lo, __shfl_xor(lo, o, 64));
+                if (lane == 0) sh.scan[threadIdx.x >> 6] = lo;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < TK_THREADS / 64; ++i) lo = min(lo, sh.scan[i]);
+                thr = max(thr, lo + 1);                                  // an equal value further on has a higher id: out
+                ge = tk_value(thr);
+                __syncthreads();
             }
-            if (cmax[c] > thr) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int o = tk_order((uint16_t)(w[j >> 1] >> ((j & 1) * 16)));
-                    if (o > thr) sh.cand[atomicAdd(&sh.count, 1)] = tk_key(o, (uint32_t)(beg + e + j));
-                }
-            }
+            if (here) append(c, w);
             __syncthreads();
         }
     }
     if ((int)threadIdx.x < back) single(front + granules * 8 + threadIdx.x);
     const float2 ms = tk_block_join(sh, make_float2(m, s));
     __syncthreads();
+    const int got = min(want, sh.count);                                 // fewer than want: a row with NaN
     tk_rank(sh, sh.count, want);
     if (slices == 1) {
         tk_write(sh, k, ms, inv_temp, ids + (int64_t)row * k, logp + (int64_t)row * k, lse + row);
     } else {
         uint64_t* kp = keys + ((int64_t)row * slices + blockIdx.x) * k;
-        for (int j = threadIdx.x; j < k; j += TK_THREADS) kp[j] = j < want ? sh.best[j] : 0;
+        for (int j = threadIdx.x; j < k; j += TK_THREADS) kp[j] = j < got ? sh.best[j] : 0;
         if (threadIdx.x == 0) stats[(int64_t)row * slices + blockIdx.x] = ms;
     }
 }
 
-// one workgroup per row: the best of slices * k <= TK_CAP keys
+// One workgroup per row: the best of slices * k <= TK_CAP keys, each slice's in falling order (0 where it has fewer than k values).  The
+// ceil(k / slices)-th keys of the slices and the k-th key of any slice bound the row's k-th from below: only what reaches both bounds is ranked.
 __global__ __launch_bounds__(TK_THREADS) void topk_join_kernel(const uint64_t* __restrict__ keys, const float2* __restrict__ stats, int slices, int k,
                                                               float inv_temp, int32_t* __restrict__ ids, float* __restrict__ logp, float* __restrict__ lse) {
     __shared__ TkShared sh;
-    const int row = blockIdx.x;
-    for (int j = threadIdx.x; j < slices * k; j += TK_THREADS) sh.cand[j] = keys[(int64_t)row * slices * k + j];
+    __shared__ uint64_t floor_of[TK_THREADS / 64];
+    const int row = blockIdx.x, lane = threadIdx.x & 63;
+    const uint64_t* kp = keys + (int64_t)row * slices * k;
+    if (threadIdx.x == 0) sh.count = 0;
+    uint64_t lo = ~0ull, hi = 0;                                         // min over slices of the ceil(k/slices)-th key, max of the k-th
+    for (int j = threadIdx.x; j < slices; j += TK_THREADS) {
+        lo = min(lo, kp[(int64_t)j * k + (k + slices - 1) / slices - 1]);
+        hi = max(hi, kp[(int64_t)j * k + k - 1]);
+    }
     const float2 ms = tk_block_join(sh, threadIdx.x < (unsigned)slices ? stats[(int64_t)row * slices + threadIdx.x] : make_float2(-INFINITY, 0.f));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        lo = min(lo, (uint64_t)__shfl_xor((unsigned long long)lo, o, 64));
+        hi = max(hi, (uint64_t)__shfl_xor((unsigned long long)hi, o, 64));
+    }
+    if (lane == 0) { floor_of[threadIdx.x >> 6] = lo; sh.best[threadIdx.x >> 6] = hi; }
     __syncthreads();
-    // keys that are 0 (a slice shorter than k) never outrank a key: at least k are not
-    tk_rank(sh, slices * k, k);
+#pragma unroll
+    for (int i = 0; i < TK_THREADS / 64; ++i) { lo = min(lo, floor_of[i]); hi = max(hi, sh.best[i]); }
+    const uint64_t least = max(max(lo, hi), (uint64_t)1);
+    __syncthreads();
+    for (int j = threadIdx.x; j < slices * k; j += TK_THREADS) {
+        const uint64_t key = kp[j];
+        if (key >= least) sh.cand[atomicAdd(&sh.count, 1)] = key;
+    }
+    __syncthreads();
+    tk_rank(sh, sh.count, k);
     tk_write(sh, k, ms, inv_temp, ids + (int64_t)row * k, logp + (int64_t)row * k, lse + row);
 }
 
-// slices of a row: enough workgroups for the CUs when there are few rows; a slice keeps at least one segment of values, and the slices' keys
-// fit the join's list
+// Slices of a row: whole rounds of two workgroups per CU, each costing its slice plus about 32 K values' time of threshold, ranking and launch;
+// a slice keeps at least a load per thread, the slices' keys fit the join's list.
 static int topk_slices(int T, int V, int k) {
-    const int ncu = st_num_cus();
-    int s = std::min(st_cdiv(2 * ncu, std::max(T, 1)), st_cdiv(V, TK_CHUNK * TK_SEG / 2));
-    s = std::min(s, TK_CAP / k);
-    return std::max(s, 1);
+    const int slots = 2 * st_num_cus(), most = std::max(1, std::min({TK_CAP / k, st_cdiv(V, TK_CHUNK), 64}));
+    int best = 1;
+    int64_t cost = INT64_MAX;
+    for (int s = 1; s <= most; ++s) {
+        const int64_t c = (int64_t)st_cdiv((int64_t)T * s, slots) * (st_cdiv(V, s) + 32768) + (s > 1 ? 24576 + 256 * s : 0);
+        if (c < cost) { cost = c; best = s; }
+    }
+    return best;
 }
 
 extern "C" {
