@@ -170,6 +170,180 @@ __global__ __launch_bounds__(256) void head_tile_kernel(const uint16_t* __restri
     }
 }
 
+// ------------------------------------------------------------------------------------------------------------------------------------
+// The same logit tile for few rows (T <= 128): the launch is a stream of the head's weights, so the tile is small and several workgroups share a CU
+// to keep copies in flight: BT = 16 MT rows x 128 vocabulary columns, four waves of 32 columns each, K-steps of 64 through SLOTS LDS slots filled
+// by LDS-DMA (16-byte chunk c of a row at position c ^ (row & 7): conflict-free fragment reads), SLOTS - 1 steps in flight behind one barrier per
+// step.  Epilogues as head_tile_kernel; part[n0 / 128][m].  DLOGITS also leaves d transposed, dt[n][T64], for head_dw_few_kernel.
+// ------------------------------------------------------------------------------------------------------------------------------------
+template <int N> __device__ __forceinline__ void vh_wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+template <int MT, int SLOTS, bool DLOGITS>
+__global__ __launch_bounds__(256, 2) void head_few_kernel(const uint16_t* __restrict__ h, int64_t ldh, const uint16_t* __restrict__ w, int64_t ldw, int T, int V,
+                                                         int H, float sc, const int64_t* __restrict__ labels, float2* __restrict__ part,
+                                                         float* __restrict__ zlab, VhTargets tg, const VhRow* __restrict__ rows, int v0,
+                                                         uint16_t* __restrict__ d, int64_t ldd, uint16_t* __restrict__ dt, int T64) {
+    constexpr int BT = 16 * MT, SLOT = (128 + BT) * 128, HC = MT / 2;    // HC: 1-KiB copies of h per wave and step
+    static_assert(MT % 2 == 0, "every wave copies the same number of rows");
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * 128;
+    // copy j of a wave: 8 rows, lane -> row (lane >> 3), 16-byte chunk (lane & 7) ^ row
+    const int cr = lane >> 3, ch = ((lane & 7) ^ cr) * 8;
+    const uint16_t* wsrc[4];
+    const uint16_t* hsrc[HC];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) wsrc[j] = w + (int64_t)min(n0 + wave * 32 + j * 8 + cr, V - 1) * ldw + ch;
+#pragma unroll
+    for (int j = 0; j < HC; ++j) hsrc[j] = h + (int64_t)min(wave * 8 * HC + j * 8 + cr, T - 1) * ldh + ch;
+    auto stage = [&](int kt) {
+        char* dst = smem + (kt % SLOTS) * SLOT;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (DLOGITS) st_glds16(wsrc[j] + kt * 64, dst + (wave * 32 + j * 8) * 128);
+            else st_glds16_nt(wsrc[j] + kt * 64, dst + (wave * 32 + j * 8) * 128);
+        }
+#pragma unroll
+        for (int j = 0; j < HC; ++j) st_glds16(hsrc[j] + kt * 64, dst + (128 + wave * 8 * HC + j * 8) * 128);
+    };
+    f32x4 acc[2][MT];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const int nk = H / 64, fr = lane & 15, fk = lane >> 4;
+#pragma unroll
+    for (int s = 0; s < SLOTS - 1; ++s) if (s < nk) stage(s);
+    for (int kt = 0; kt < nk; ++kt) {
+        // this step's copies have landed; up to SLOTS - 2 younger steps stay in flight (the last steps have none to count)
+        if (kt + SLOTS - 2 < nk) vh_wait_vm<(SLOTS - 2) * (4 + HC)>(); else vh_wait_vm<0>();
+        __builtin_amdgcn_s_barrier();                                // ... for every wave, and every wave has read the slot that is filled next
+        asm volatile("" ::: "memory");
+        if (kt + SLOTS - 1 < nk) stage(kt + SLOTS - 1);
+        const char* lw = smem + (kt % SLOTS) * SLOT + wave * 32 * 128;
+        const char* lh = smem + (kt % SLOTS) * SLOT + 128 * 128;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int c = ((s * 4 + fk) ^ (fr & 7)) << 4;
+            bf16x8 wf[2], hf[MT];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) wf[i] = *reinterpret_cast<const bf16x8*>(lw + (i * 16 + fr) * 128 + c);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) hf[i] = *reinterpret_cast<const bf16x8*>(lh + (i * 16 + fr) * 128 + c);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < MT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[i], hf[j], acc[i][j], 0, 0, 0);
+        }
+    }
+    __syncthreads();                                                 // the slots are free
+    const int col0 = n0 + wave * 32 + fk * 4;                        // column of (i, r): col0 + i*16 + r
+    if constexpr (!DLOGITS) {
+        constexpr int ROWB = 128 * 4 + 16;
+        const int e0 = tg.start ? tg.start[n0 >> 8] : 0, e1 = tg.start ? tg.start[(n0 >> 8) + 1] : 0;
+        if (e1 > e0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(smem + (j * 16 + fr) * ROWB + (wave * 32 + i * 16 + fk * 4) * 4) = acc[i][j];
+            __syncthreads();
+            for (int e = e0 + threadIdx.x; e < e1; e += 256) {
+                const uint32_t it = tg.list[e];
+                const int row = it & 255, col = (it >> 8) & 255;
+                if ((col >> 7) == ((n0 >> 7) & 1))
+                    tg.z2[(int64_t)row * tg.K + (it >> 16)] = sc * *reinterpret_cast<const float*>(smem + row * ROWB + (col & 127) * 4);
+            }
+            __syncthreads();
+        }
+        float2* red = reinterpret_cast<float2*>(smem);               // [wave][row]
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            const int m = j * 16 + fr;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (col0 + i * 16 + r >= V) acc[i][j][r] = -INFINITY;
+                    mx = fmaxf(mx, acc[i][j][r]);
+                }
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float m2 = mx * sc, sub = m2 == -INFINITY ? 0.f : m2;
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s += vh_exp2(fmaf(acc[i][j][r], sc, -sub));
+            s += __shfl_xor(s, 16, 64);
+            s += __shfl_xor(s, 32, 64);
+            if (lane < 16) red[wave * BT + m] = make_float2(m2, s);
+            if (labels && m < T) {
+                const int64_t lab = labels[m] - col0;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (lab == i * 16 + r && col0 + i * 16 + r < V) zlab[m] = acc[i][j][r] * sc;
+            }
+        }
+        __syncthreads();
+        for (int m = threadIdx.x; m < min(BT, T); m += 256) {
+            float2 a = red[m];
+#pragma unroll
+            for (int wv = 1; wv < 4; ++wv) {
+                const float2 b = red[wv * BT + m];
+                const float mn = fmaxf(a.x, b.x);
+                a = make_float2(mn, mn != -INFINITY ? a.y * vh_exp2(a.x - mn) + b.y * vh_exp2(b.x - mn) : a.y + b.y);
+            }
+            part[(int64_t)blockIdx.x * T + m] = a;
+        }
+    } else {
+        // two bf16 images: [BT rows][128 columns] and [128 columns][BT rows]
+        constexpr int RB = 128 * 2 + 16, CB = BT * 2 + 16;
+        char* img_t = smem + BT * RB;
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            const int m = j * 16 + fr;
+            VhRow ri = {0.f, 0.f, 0.f, -1};
+            if (m < T) ri = rows[m];
+            const int lab = ri.label - v0 - col0;
+            const bool live = ri.c != 0.f || ri.hot != 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float o[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float x = ri.c * vh_exp2(fmaf(acc[i][j][r], sc, -ri.lse2));
+                    if (lab == i * 16 + r) x = ri.hot;
+                    o[r] = live && col0 + i * 16 + r < V ? x : 0.f;
+                }
+                uint2 pk;
+                pk.x = f2bf2(o[0], o[1]); pk.y = f2bf2(o[2], o[3]);
+                const int col = wave * 32 + i * 16 + fk * 4;
+                *reinterpret_cast<uint2*>(smem + m * RB + col * 2) = pk;
+                *reinterpret_cast<uint16_t*>(img_t + (col + 0) * CB + m * 2) = (uint16_t)pk.x;
+                *reinterpret_cast<uint16_t*>(img_t + (col + 1) * CB + m * 2) = (uint16_t)(pk.x >> 16);
+                *reinterpret_cast<uint16_t*>(img_t + (col + 2) * CB + m * 2) = (uint16_t)pk.y;
+                *reinterpret_cast<uint16_t*>(img_t + (col + 3) * CB + m * 2) = (uint16_t)(pk.y >> 16);
+            }
+        }
+        __syncthreads();
+        const int cols = min(128, (int)ldd - n0);                    // ldd % 64 == 0
+        for (int i = threadIdx.x; i < T64 * 16; i += 256) {
+            const int row = i >> 4, c = (i & 15) * 8;
+            if (c < cols)
+                *reinterpret_cast<uint4*>(d + (int64_t)row * ldd + n0 + c) = row < BT ? *reinterpret_cast<const uint4*>(smem + row * RB + c * 2) : make_uint4(0, 0, 0, 0);
+        }
+        const int per = T64 >> 3;                                    // 16-byte chunks of a row of dt
+        for (int i = threadIdx.x; i < cols * per; i += 256) {
+            const int col = i / per, c = (i - col * per) * 8;
+            *reinterpret_cast<uint4*>(dt + (int64_t)(n0 + col) * T64 + c) = c < BT ? *reinterpret_cast<const uint4*>(img_t + col * CB + c * 2) : make_uint4(0, 0, 0, 0);
+        }
+    }
+}
+
 // (max, sum) partials -> lse (natural log), stat = (max, log2 sum); logp = label logit - lse for rows with a label inside the vocabulary, 0 for the others.
 // 16 rows x 64 slices per workgroup: 16 consecutive lanes read 128 contiguous bytes of one partial row.
 __global__ __launch_bounds__(1024) void head_lse_kernel(const float2* __restrict__ part, int n_parts, const float* __restrict__ zlab,
@@ -344,10 +518,84 @@ __global__ __launch_bounds__(256) void head_dw_kernel(const uint16_t* __restrict
     }
 }
 
+// dw for few rows (T64 <= 128): the launch is the write of dw, V H elements, next to 2 KS products of 32 rows each.  Operands stand contraction-
+// contiguous (dt[v][T64], hzt[n][T64]), so fragments come straight from memory (dt once per workgroup, hzt from the caches).  A wave owns 64
+// vocabulary rows x 64 columns per step; row i of the MFMA's first operand is column (i >> 2)*16 + ni*4 + (i & 3) of the step, so a lane ends up with
+// 16 consecutive columns of a row: two 16-byte (fp32: four) stores, whole 128-byte lines per wave.
+template <int KS, bool OUT_BF16, bool ACCUM>
+__global__ __launch_bounds__(256) void head_dw_few_kernel(const uint16_t* __restrict__ dt, const uint16_t* __restrict__ hzt, int kv, int H, int cols_per,
+                                                         uint16_t* __restrict__ dwb, float* __restrict__ dwf, int64_t lddw) {
+    constexpr int T64 = KS * 32;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fk = lane >> 4;
+    const int r0 = blockIdx.x * 256 + wave * 64;
+    if (r0 >= kv) return;
+    bf16x8 df[4][KS];
+#pragma unroll
+    for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) df[mi][s] = *reinterpret_cast<const bf16x8*>(dt + (int64_t)min(r0 + mi * 16 + fr, kv - 1) * T64 + s * 32 + fk * 8);
+    const int c0 = blockIdx.y * cols_per, c1 = min(c0 + cols_per, H);
+    for (int c = c0; c < c1; c += 64) {
+        bf16x8 hf[4][KS];
+#pragma unroll
+        for (int ni = 0; ni < 4; ++ni)
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+                hf[ni][s] = *reinterpret_cast<const bf16x8*>(hzt + (int64_t)(c + (fr >> 2) * 16 + ni * 4 + (fr & 3)) * T64 + s * 32 + fk * 8);
+#pragma unroll
+        for (int mi = 0; mi < 4; ++mi) {
+            f32x4 acc[4];
+#pragma unroll
+            for (int ni = 0; ni < 4; ++ni) {
+                acc[ni] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < KS; ++s) acc[ni] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hf[ni][s], df[mi][s], acc[ni], 0, 0, 0);
+            }
+            const int v = r0 + mi * 16 + fr;
+            if (v >= kv) continue;
+            const int64_t at = (int64_t)v * lddw + c + fk * 16;
+            if constexpr (OUT_BF16) {
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    uint4 o;
+                    o.x = f2bf2(acc[2 * p][0], acc[2 * p][1]); o.y = f2bf2(acc[2 * p][2], acc[2 * p][3]);
+                    o.z = f2bf2(acc[2 * p + 1][0], acc[2 * p + 1][1]); o.w = f2bf2(acc[2 * p + 1][2], acc[2 * p + 1][3]);
+                    *reinterpret_cast<uint4*>(dwb + at + p * 8) = o;
+                }
+            } else {
+#pragma unroll
+                for (int ni = 0; ni < 4; ++ni) {
+                    float4* q = reinterpret_cast<float4*>(dwf + at + ni * 4);
+                    float4 o = make_float4(acc[ni][0], acc[ni][1], acc[ni][2], acc[ni][3]);
+                    if constexpr (ACCUM) { const float4 b = *q; o.x += b.x; o.y += b.y; o.z += b.z; o.w += b.w; }
+                    *q = o;
+                }
+            }
+        }
+    }
+}
+
+// hzt[n][t] = hz[t][n]: 64 x 64 elements per workgroup
+__global__ __launch_bounds__(256) void head_hzt_kernel(const uint16_t* __restrict__ hz, uint16_t* __restrict__ hzt, int T64, int H) {
+    __shared__ uint16_t tile[64][72];
+    const int n0 = blockIdx.x * 64, t0 = blockIdx.y * 64;
+    for (int i = threadIdx.x; i < 64 * 8; i += 256)
+        *reinterpret_cast<uint4*>(&tile[i >> 3][(i & 7) * 8]) = *reinterpret_cast<const uint4*>(hz + (int64_t)(t0 + (i >> 3)) * H + n0 + (i & 7) * 8);
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * 8; i += 256) {
+        const int n = i >> 3, c = (i & 7) * 8;
+        uint4 o;
+        o.x = tile[c][n] | (uint32_t)tile[c + 1][n] << 16; o.y = tile[c + 2][n] | (uint32_t)tile[c + 3][n] << 16;
+        o.z = tile[c + 4][n] | (uint32_t)tile[c + 5][n] << 16; o.w = tile[c + 6][n] | (uint32_t)tile[c + 7][n] << 16;
+        *reinterpret_cast<uint4*>(hzt + (int64_t)(n0 + n) * T64 + t0 + c) = o;
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------------------------------------
 // Distillation from k teacher log-probs per row.
 // ------------------------------------------------------------------------------------------------------------------------------------
 #define VH_MAX_K 1024
+#define VH_FEW 128                                                   // rows up to which the weight stream bounds the products
 #define VH_MAX_V (1 << 22)                                           // column tiles fit the counters of head_bucket_kernel
 
 // teacher probabilities of one row, by one wave: p_k of present entries (0 <= id < V), 0 for the others; log p_k = a_k - shift
@@ -468,7 +716,7 @@ __global__ __launch_bounds__(128) void head_rows_kl_kernel(const uint16_t* __res
 // log q of the forward pass.  An id that a row holds twice gets the sum of its probabilities from both entries: the same value twice.
 __global__ __launch_bounds__(256) void head_sparse_kernel(const int32_t* __restrict__ ids, const float* __restrict__ a, int K, int renorm,
                                                          const float* __restrict__ logq, const VhRow* __restrict__ rows, int v0, int kv,
-                                                         uint16_t* __restrict__ d, int64_t ldd, int T, int V) {
+                                                         uint16_t* __restrict__ d, int64_t ldd, uint16_t* __restrict__ dt, int T64, int T, int V) {
     const int lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (t >= T) return;
     ids += (int64_t)t * K; a += (int64_t)t * K; logq += (int64_t)t * K;
@@ -481,7 +729,9 @@ __global__ __launch_bounds__(256) void head_sparse_kernel(const int32_t* __restr
         if (id < v0 || id >= v0 + kv) continue;
         float p = 0.f;
         for (int j = 0; j < K; ++j) if (ids[j] == id) p += vh_exp2((a[j] - th.shift) * VH_LOG2E);
-        d[(int64_t)t * ldd + id - v0] = f2bf(r * (th.total * vh_exp2(logq[k] * VH_LOG2E) - p));
+        const uint16_t x = f2bf(r * (th.total * vh_exp2(logq[k] * VH_LOG2E) - p));
+        d[(int64_t)t * ldd + id - v0] = x;
+        if (dt) dt[(int64_t)(id - v0) * T64 + t] = x;
     }
 }
 
@@ -496,13 +746,15 @@ namespace {
 struct Plan {                                                        // workspace layout (byte offsets) and piece / slice counts of one call
     int T64, pieces, piece, split;
     int64_t part, zlab, stat, start, list, fwd_bytes;
-    int64_t rows, scale, hz, d, slab, bwd_bytes;
+    int64_t rows, scale, hz, hzt, d, dt, slab, bwd_bytes;
+    bool few;                                                        // the weight-streaming kernels
 };
 int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 
 Plan head_plan(int T, int V, int H, int K) {                         // K: targets per row of the distillation, 0: labels
     Plan p;
     p.T64 = (int)up(T, 64);
+    p.few = T <= VH_FEW;
     const int64_t n_parts = 2 * (int64_t)st_cdiv(V, 256);
     p.part = 0;
     p.zlab = up(n_parts * T * 8, 256);
@@ -527,8 +779,10 @@ Plan head_plan(int T, int V, int H, int K) {                         // K: targe
     p.rows = 0;
     p.scale = up((int64_t)T * (int64_t)sizeof(VhRow), 256);
     p.hz = p.scale + up((int64_t)T * 4, 256);
-    p.d = p.hz + up((int64_t)p.T64 * H * 2, 256);
-    p.slab = p.d + up((int64_t)p.T64 * p.piece * 2, 256);
+    p.hzt = p.hz + up((int64_t)p.T64 * H * 2, 256);
+    p.d = p.hzt + (p.few ? up((int64_t)p.T64 * H * 2, 256) : 0);
+    p.dt = p.d + up((int64_t)p.T64 * p.piece * 2, 256);
+    p.slab = p.dt + (p.few ? up((int64_t)p.T64 * p.piece * 2, 256) : 0);
     p.bwd_bytes = p.slab + up((int64_t)p.split * T * H * 4, 256);
     return p;
 }
@@ -539,14 +793,30 @@ bool operands_ok(const void* h, int64_t ldh, const void* w, int64_t ldw, int T, 
 }
 
 // one attribute per kernel and device, set before its first launch there
-template <auto KERN> void allow_lds() {
+template <auto KERN> void allow_lds(int bytes = VH_SMEM) {
     static bool done[64] = {};
     int dev = 0;
     hipGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !done[dev]) {
-        hipFuncSetAttribute((const void*)KERN, hipFuncAttributeMaxDynamicSharedMemorySize, VH_SMEM);
+        hipFuncSetAttribute((const void*)KERN, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
         if (dev >= 0 && dev < 64) done[dev] = true;
     }
+}
+
+// one launch of the few-row tile: T <= 32, 64 or 128 rows
+template <bool DLOGITS, class... A>
+int launch_few(int T, int V, hipStream_t s, A... args) {
+    const dim3 grid(st_cdiv(V, 128));
+    auto go = [&](auto kern, int smem) {
+        hipLaunchKernelGGL(kern, grid, dim3(256), smem, s, args...);
+        ST_CHECK_LAUNCH();
+        return 0;
+    };
+    constexpr int S32 = 4 * 160 * 128, S64 = 3 * 192 * 128, S128 = 2 * 256 * 128;
+    if (T <= 32) { allow_lds<head_few_kernel<2, 4, DLOGITS>>(S32); return go(head_few_kernel<2, 4, DLOGITS>, S32); }
+    if (T <= 64) { allow_lds<head_few_kernel<4, 3, DLOGITS>>(S64); return go(head_few_kernel<4, 3, DLOGITS>, S64); }
+    allow_lds<head_few_kernel<8, 2, DLOGITS>>(S128 + 8192);
+    return go(head_few_kernel<8, 2, DLOGITS>, S128 + 8192);          // (the two images of the d epilogue: 128 x 272 bytes each)
 }
 
 int head_stats(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, const int64_t* labels, float sc, float* logp, float* lse, VhTargets tg,
@@ -554,35 +824,55 @@ int head_stats(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, c
     const int tm = st_cdiv(T, 256), tn = st_cdiv(V, 256);
     float2* part = (float2*)(ws + p.part);
     float* zlab = (float*)(ws + p.zlab);
+    int n_parts = 2 * tn;
+    if (p.few) {
+        n_parts = st_cdiv(V, 128);
+        const int rc = launch_few<false>(T, V, s, h, ldh, w, ldw, T, V, H, sc, labels, part, zlab, tg, (const VhRow*)nullptr, 0, (uint16_t*)nullptr,
+                                         (int64_t)0, (uint16_t*)nullptr, 0);
+        if (rc) return rc;
+    } else {
     allow_lds<head_tile_kernel<false>>();
     hipLaunchKernelGGL((head_tile_kernel<false>), dim3(tm * tn), dim3(256), VH_SMEM, s, h, ldh, w, ldw, T, V, H, tm, tn, sc, labels, part, zlab, tg,
                        (const VhRow*)nullptr, 0, (uint16_t*)nullptr, (int64_t)0, 0);
     ST_CHECK_LAUNCH();
-    hipLaunchKernelGGL(head_lse_kernel, dim3(st_cdiv(T, 16)), dim3(1024), 0, s, part, 2 * tn, zlab, labels, logp, lse, (float2*)(ws + p.stat), T, V);
+    }
+    hipLaunchKernelGGL(head_lse_kernel, dim3(st_cdiv(T, 16)), dim3(1024), 0, s, part, n_parts, zlab, labels, logp, lse, (float2*)(ws + p.stat), T, V);
     ST_CHECK_LAUNCH();
     return 0;
 }
 
-// the pieces of a backward pass behind the row coefficients; `sparse(v0, kv, ldd)` finishes d at the targets of a piece
+// the pieces of a backward pass behind the row coefficients; `sparse` finishes d at the targets of a piece
 template <class F>
 int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, float sc, uint16_t* dh, int64_t lddh, uint16_t* dwb, float* dwf,
                   int64_t lddw, int accumulate, char* ws, const Plan& p, int T, int V, int H, hipStream_t s, F&& sparse) {
     const VhRow* rows = (const VhRow*)(ws + p.rows);
     const uint16_t* hz = (const uint16_t*)(ws + p.hz);
     uint16_t* d = (uint16_t*)(ws + p.d);
+    uint16_t* dt = p.few ? (uint16_t*)(ws + p.dt) : nullptr;
+    uint16_t* hzt = (uint16_t*)(ws + p.hzt);
     float* slab = (float*)(ws + p.slab);
     const int tm = st_cdiv(T, 256), th = st_cdiv(H, 256);
     allow_lds<head_tile_kernel<true>>();
     allow_lds<head_dh_kernel<false>>(); allow_lds<head_dh_kernel<true>>();
     allow_lds<head_dw_kernel<true, false>>(); allow_lds<head_dw_kernel<false, false>>(); allow_lds<head_dw_kernel<false, true>>();
+    if (p.few && (dwb || dwf)) {
+        hipLaunchKernelGGL(head_hzt_kernel, dim3(H / 64, p.T64 / 64), dim3(256), 0, s, hz, hzt, p.T64, H);
+        ST_CHECK_LAUNCH();
+    }
     for (int i = 0; i < p.pieces; ++i) {
         const int v0 = i * p.piece, kv = std::min(p.piece, V - v0), tn = st_cdiv(kv, 256);
         const int64_t ldd = up(kv, 64);
         const uint16_t* wp = w + (int64_t)v0 * ldw;
+        if (p.few) {
+            const int rc = launch_few<true>(T, kv, s, h, ldh, wp, ldw, T, kv, H, sc, (const int64_t*)nullptr, (float2*)nullptr, (float*)nullptr,
+                                            VhTargets{}, rows, v0, d, ldd, dt, p.T64);
+            if (rc) return rc;
+        } else {
         hipLaunchKernelGGL((head_tile_kernel<true>), dim3(tm * tn), dim3(256), VH_SMEM, s, h, ldh, wp, ldw, T, kv, H, tm, tn, sc, (const int64_t*)nullptr,
                            (float2*)nullptr, (float*)nullptr, VhTargets{}, rows, v0, d, ldd, p.T64);
         ST_CHECK_LAUNCH();
-        const int rc = sparse(v0, kv, d, ldd);
+        }
+        const int rc = sparse(v0, kv, d, ldd, dt);
         if (rc) return rc;
         if (dh) {
             const int nkt = st_cdiv(kv, 64), per = st_cdiv(nkt, p.split), slices = st_cdiv(nkt, per);      // (a short last piece may fill fewer slices)
@@ -596,7 +886,16 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
             const dim3 grid(tv * th);
             uint16_t* ob = dwb ? dwb + (int64_t)v0 * lddw : nullptr;
             float* of = dwf ? dwf + (int64_t)v0 * lddw : nullptr;
-            if (dwb) hipLaunchKernelGGL((head_dw_kernel<true, false>), grid, dim3(256), VH_SMEM, s, d, ldd, hz, p.T64, kv, H, tv, th, ob, of, lddw);
+            if (p.few) {
+                // columns per workgroup: about four workgroups per CU, so that loads, products and stores of several overlap
+                const int per = (int)up(st_cdiv(H, std::max(1, st_cdiv(4 * st_num_cus(), tv))), 64);
+                const dim3 few_grid(tv, st_cdiv(H, per));
+#define VH_DW_FEW(KS, OB, AC) hipLaunchKernelGGL((head_dw_few_kernel<KS, OB, AC>), few_grid, dim3(256), 0, s, dt, hzt, kv, H, per, ob, of, lddw)
+                if (p.T64 == 64) { if (dwb) VH_DW_FEW(2, true, false); else if (accumulate) VH_DW_FEW(2, false, true); else VH_DW_FEW(2, false, false); }
+                else { if (dwb) VH_DW_FEW(4, true, false); else if (accumulate) VH_DW_FEW(4, false, true); else VH_DW_FEW(4, false, false); }
+#undef VH_DW_FEW
+            }
+            else if (dwb) hipLaunchKernelGGL((head_dw_kernel<true, false>), grid, dim3(256), VH_SMEM, s, d, ldd, hz, p.T64, kv, H, tv, th, ob, of, lddw);
             else if (accumulate) hipLaunchKernelGGL((head_dw_kernel<false, true>), grid, dim3(256), VH_SMEM, s, d, ldd, hz, p.T64, kv, H, tv, th, ob, of, lddw);
             else hipLaunchKernelGGL((head_dw_kernel<false, false>), grid, dim3(256), VH_SMEM, s, d, ldd, hz, p.T64, kv, H, tv, th, ob, of, lddw);
             ST_CHECK_LAUNCH();
@@ -661,7 +960,7 @@ int st_linear_logprob_bwd(const st_bf16* hidden, int64_t ldh, const st_bf16* wei
                        (float*)(ws + p.scale), (uint16_t*)(ws + p.hz), T, V, H);
     ST_CHECK_LAUNCH();
     return head_backward(hidden, ldh, weight, ldw, inv_temperature * VH_LOG2E, dhidden, lddh, dweight_bf16, dweight_f32, lddw, accumulate, ws, p, T, V, H, s,
-                         [](int, int, uint16_t*, int64_t) { return 0; });
+                         [](int, int, uint16_t*, int64_t, uint16_t*) { return 0; });
 }
 
 int st_linear_topk_kl_fwd(const st_bf16* hidden, int64_t ldh, const st_bf16* weight, int64_t ldw, const int32_t* ids, const float* teacher_logp, int K,
@@ -704,9 +1003,9 @@ int st_linear_topk_kl_bwd(const st_bf16* hidden, int64_t ldh, const st_bf16* wei
                        (VhRow*)(ws + p.rows), (float*)(ws + p.scale), (uint16_t*)(ws + p.hz), T, V, H);
     ST_CHECK_LAUNCH();
     return head_backward(hidden, ldh, weight, ldw, inv_temperature * VH_LOG2E, dhidden, lddh, dweight_bf16, dweight_f32, lddw, accumulate, ws, p, T, V, H, s,
-                         [&](int v0, int kv, uint16_t* d, int64_t ldd) -> int {
+                         [&](int v0, int kv, uint16_t* d, int64_t ldd, uint16_t* dt) -> int {
                              hipLaunchKernelGGL(head_sparse_kernel, dim3(st_cdiv(T, 4)), dim3(256), 0, s, ids, teacher_logp, K, renormalize, logq,
-                                                (const VhRow*)(ws + p.rows), v0, kv, d, ldd, T, V);
+                                                (const VhRow*)(ws + p.rows), v0, kv, d, ldd, dt, p.T64, T, V);
                              ST_CHECK_LAUNCH();
                              return 0;
                          });
