@@ -200,10 +200,7 @@ __global__ __launch_bounds__(256, 2) void head_few_kernel(const uint16_t* __rest
     auto stage = [&](int kt) {
         char* dst = smem + (kt % SLOTS) * SLOT;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (DLOGITS) st_glds16(wsrc[j] + kt * 64, dst + (wave * 32 + j * 8) * 128);
-            else st_glds16_nt(wsrc[j] + kt * 64, dst + (wave * 32 + j * 8) * 128);
-        }
+        for (int j = 0; j < 4; ++j) st_glds16_nt(wsrc[j] + kt * 64, dst + (wave * 32 + j * 8) * 128);       // one workgroup reads a weight, once
 #pragma unroll
         for (int j = 0; j < HC; ++j) st_glds16(hsrc[j] + kt * 64, dst + (128 + wave * 8 * HC + j * 8) * 128);
     };
@@ -458,11 +455,104 @@ __global__ __launch_bounds__(256) void head_dh_kernel(const uint16_t* __restrict
     }
 }
 
+// The same for few rows (T64 <= 128): a stream of w, [32 vocabulary rows][256 columns] per step through SLOTS LDS slots, next to a [T64][32] tile of d.
+// w is contraction-major: its fragments are LDS transpose reads (image and swizzle as the contraction-major operands of gemm_asm4.hip).  Four
+// waves of 64 columns, all rows each; the vocabulary is cut into slices so that every CU has two workgroups.
+template <int MT, int SLOTS, bool ACCUM>
+__global__ __launch_bounds__(256, 2) void head_dh_few_kernel(const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ w, int64_t ldw, int T,
+                                                            int kv, int H, int tiles_n, int per, float* __restrict__ slab) {
+    constexpr int BT = 16 * MT, WB = 32 * 512, SLOT = WB + BT * 64, DC = BT / 64;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int slice = blockIdx.x / tiles_n, n0 = (blockIdx.x % tiles_n) * 256;
+    const int nkt = (kv + 31) / 32, kt0 = slice * per, nk = min(nkt - kt0, per);
+    // copies of w: two k-rows each, lane -> k-row (lane >> 5), 16-byte piece sl: the 32-byte chunk (sl >> 1) ^ g(k-row)
+    int wcol[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int kr = wave * 8 + j * 2 + (lane >> 5), sl = lane & 31, g = (kr & 3) | (((kr >> 3) & 1) << 2);
+        wcol[j] = n0 + min((((sl >> 1) ^ g) << 4) + (sl & 1) * 8, min(256, H - n0) - 8);
+    }
+    const uint16_t* dsrc[DC];
+#pragma unroll
+    for (int j = 0; j < DC; ++j) {                                   // copies of d: 16 rows of 64 bytes, 16-byte chunk (lane & 3) ^ (row >> 2)
+        const int row = (wave * DC + j) * 16 + (lane >> 2);
+        dsrc[j] = d + (int64_t)row * ldd + (((lane & 3) ^ ((row >> 2) & 3)) << 3);
+    }
+    auto stage = [&](int kt) {
+        char* dst = smem + (kt % SLOTS) * SLOT;
+        const int k0 = (kt0 + kt) * 32;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int kr = wave * 8 + j * 2 + (lane >> 5);           // k-rows beyond the vocabulary read its last one: d is zero there
+            st_glds16(w + (int64_t)min(k0 + kr, kv - 1) * ldw + wcol[j], dst + (wave * 4 + j) * 1024);
+        }
+#pragma unroll
+        for (int j = 0; j < DC; ++j) st_glds16(dsrc[j] + k0, dst + WB + (wave * DC + j) * 1024);
+    };
+    f32x4 acc[4][MT];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const int fr = lane & 15, fk = lane >> 4;
+    const uint32_t smem32 = (uint32_t)(uintptr_t)smem;
+    uint32_t tr[4];
+    {
+        const int g = ((lane >> 2) & 3) | ((fk & 1) << 2), row = fk * 8 + (fr >> 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tr[i] = smem32 + row * 512 + (((wave * 4 + i) ^ g) << 5) + (lane & 3) * 8;
+    }
+#pragma unroll
+    for (int s = 0; s < SLOTS - 1; ++s) if (s < nk) stage(s);
+    for (int kt = 0; kt < nk; ++kt) {
+        if (kt + SLOTS - 2 < nk) vh_wait_vm<(SLOTS - 2) * (4 + DC)>(); else vh_wait_vm<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (kt + SLOTS - 1 < nk) stage(kt + SLOTS - 1);
+        const uint32_t at = (kt % SLOTS) * SLOT;
+        const char* ld = smem + at + WB;
+        bf16x8 df[MT];
+#pragma unroll
+        for (int j = 0; j < MT; ++j) df[j] = *reinterpret_cast<const bf16x8*>(ld + (j * 16 + fr) * 64 + ((fk ^ ((fr >> 2) & 3)) << 4));
+        union Frag { bf16x8 v; s16x4_t h[2]; } wf[4];
+        // the transpose reads and the wait for them in one statement: the compiler neither sees the reads nor holds up the copies in flight
+        asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:2048\n\tds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:2048\n\t"
+                     "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:2048\n\tds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:2048\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(wf[0].h[0]), "=&v"(wf[0].h[1]), "=&v"(wf[1].h[0]), "=&v"(wf[1].h[1]), "=&v"(wf[2].h[0]), "=&v"(wf[2].h[1]), "=&v"(wf[3].h[0]),
+                       "=&v"(wf[3].h[1])
+                     : "v"(tr[0] + at), "v"(tr[1] + at), "v"(tr[2] + at), "v"(tr[3] + at)
+                     : "memory");
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[i].v, df[j], acc[i][j], 0, 0, 0);
+    }
+    float* out = slab + (int64_t)slice * T * H;
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        const int m = j * 16 + fr;
+        if (m >= T) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int n = n0 + wave * 64 + i * 16 + fk * 4;
+            if (n >= H) continue;
+            float4* q = reinterpret_cast<float4*>(out + (int64_t)m * H + n);
+            float4 o = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+            if constexpr (ACCUM) { const float4 c = *q; o.x += c.x; o.y += c.y; o.z += c.z; o.w += c.w; }
+            *q = o;
+        }
+    }
+}
+
 // dh = bf16(row scale * sum of the slabs, in slice order)
 __global__ __launch_bounds__(256) void head_dh_finish_kernel(const float* __restrict__ slab, int split, const float* __restrict__ scale, uint16_t* __restrict__ dh, int64_t lddh, int T, int H) {
     const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= (int64_t)T * H) return;
     float4 a = *reinterpret_cast<const float4*>(slab + i);
+#pragma unroll 8
     for (int s = 1; s < split; ++s) {
         const float4 b = *reinterpret_cast<const float4*>(slab + (int64_t)s * T * H + i);
         a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
@@ -519,58 +609,67 @@ __global__ __launch_bounds__(256) void head_dw_kernel(const uint16_t* __restrict
 }
 
 // dw for few rows (T64 <= 128): the launch is the write of dw, V H elements, next to 2 KS products of 32 rows each.  Operands stand contraction-
-// contiguous (dt[v][T64], hzt[n][T64]), so fragments come straight from memory (dt once per workgroup, hzt from the caches).  A wave owns 64
-// vocabulary rows x 64 columns per step; row i of the MFMA's first operand is column (i >> 2)*16 + ni*4 + (i & 3) of the step, so a lane ends up with
-// 16 consecutive columns of a row: two 16-byte (fp32: four) stores, whole 128-byte lines per wave.
+// contiguous (dt[v][T64], hzt[n][T64]), so fragments come straight from memory: dt once per workgroup, hzt from the caches, a step ahead.  A
+// workgroup owns 128 vocabulary rows and walks the columns 256 at a time, 64 per wave; the bf16 tile goes through LDS, because a row has to leave in
+// long runs: 64-byte pieces of 16 rows at a pitch of H elements meet in a few cache channels (V = 152 064, H = 3584: 292 us against 160 for a fill).
 template <int KS, bool OUT_BF16, bool ACCUM>
-__global__ __launch_bounds__(256) void head_dw_few_kernel(const uint16_t* __restrict__ dt, const uint16_t* __restrict__ hzt, int kv, int H, int cols_per,
+__global__ __launch_bounds__(256) void head_dw_few_kernel(const uint16_t* __restrict__ dt, const uint16_t* __restrict__ hzt, int kv, int H,
                                                          uint16_t* __restrict__ dwb, float* __restrict__ dwf, int64_t lddw) {
-    constexpr int T64 = KS * 32;
+    constexpr int T64 = KS * 32, MI = 8;                             // 16 MI vocabulary rows per workgroup
+    __shared__ __attribute__((aligned(16))) char img[OUT_BF16 ? 16 * MI * VH_ROWB : 16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fk = lane >> 4;
-    const int r0 = blockIdx.x * 256 + wave * 64;
-    if (r0 >= kv) return;
-    bf16x8 df[4][KS];
+    const int r0 = blockIdx.x * (16 * MI);
+    bf16x8 df[MI][KS], ahead[4][KS], hf[4][KS];
 #pragma unroll
-    for (int mi = 0; mi < 4; ++mi)
+    for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
         for (int s = 0; s < KS; ++s) df[mi][s] = *reinterpret_cast<const bf16x8*>(dt + (int64_t)min(r0 + mi * 16 + fr, kv - 1) * T64 + s * 32 + fk * 8);
-    const int c0 = blockIdx.y * cols_per, c1 = min(c0 + cols_per, H);
-    for (int c = c0; c < c1; c += 64) {
-        bf16x8 hf[4][KS];
+    auto fetch = [&](int c) {                                        // (columns beyond H: the last ones, never stored)
 #pragma unroll
         for (int ni = 0; ni < 4; ++ni)
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-                hf[ni][s] = *reinterpret_cast<const bf16x8*>(hzt + (int64_t)(c + (fr >> 2) * 16 + ni * 4 + (fr & 3)) * T64 + s * 32 + fk * 8);
+            for (int s = 0; s < KS; ++s) ahead[ni][s] = *reinterpret_cast<const bf16x8*>(hzt + (int64_t)min(c + ni * 16 + fr, H - 1) * T64 + s * 32 + fk * 8);
+    };
+    if constexpr (KS == 2) fetch(wave * 64);
+    for (int c0 = 0; c0 < H; c0 += 256) {
+        const int c = c0 + wave * 64;
+        if constexpr (KS > 2) fetch(c);                              // (no registers left to be a step ahead)
 #pragma unroll
-        for (int mi = 0; mi < 4; ++mi) {
-            f32x4 acc[4];
+        for (int ni = 0; ni < 4; ++ni)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) hf[ni][s] = ahead[ni][s];
+        if constexpr (KS == 2) fetch(c + 256);
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi) {
 #pragma unroll
             for (int ni = 0; ni < 4; ++ni) {
-                acc[ni] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int s = 0; s < KS; ++s) acc[ni] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hf[ni][s], df[mi][s], acc[ni], 0, 0, 0);
-            }
-            const int v = r0 + mi * 16 + fr;
-            if (v >= kv) continue;
-            const int64_t at = (int64_t)v * lddw + c + fk * 16;
-            if constexpr (OUT_BF16) {
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    uint4 o;
-                    o.x = f2bf2(acc[2 * p][0], acc[2 * p][1]); o.y = f2bf2(acc[2 * p][2], acc[2 * p][3]);
-                    o.z = f2bf2(acc[2 * p + 1][0], acc[2 * p + 1][1]); o.w = f2bf2(acc[2 * p + 1][2], acc[2 * p + 1][3]);
-                    *reinterpret_cast<uint4*>(dwb + at + p * 8) = o;
-                }
-            } else {
-#pragma unroll
-                for (int ni = 0; ni < 4; ++ni) {
-                    float4* q = reinterpret_cast<float4*>(dwf + at + ni * 4);
-                    float4 o = make_float4(acc[ni][0], acc[ni][1], acc[ni][2], acc[ni][3]);
+                for (int s = 0; s < KS; ++s) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hf[ni][s], df[mi][s], acc, 0, 0, 0);
+                if constexpr (OUT_BF16) {
+                    uint2 pk;
+                    pk.x = f2bf2(acc[0], acc[1]); pk.y = f2bf2(acc[2], acc[3]);
+                    *reinterpret_cast<uint2*>(img + (mi * 16 + fr) * VH_ROWB + (wave * 64 + ni * 16 + fk * 4) * 2) = pk;
+                } else {
+                    const int v = r0 + mi * 16 + fr, n = c + ni * 16 + fk * 4;
+                    if (v >= kv || n >= H) continue;
+                    float4* q = reinterpret_cast<float4*>(dwf + (int64_t)v * lddw + n);
+                    float4 o = make_float4(acc[0], acc[1], acc[2], acc[3]);
                     if constexpr (ACCUM) { const float4 b = *q; o.x += b.x; o.y += b.y; o.z += b.z; o.w += b.w; }
                     *q = o;
                 }
             }
+        }
+        if constexpr (OUT_BF16) {
+            __syncthreads();
+            const int col = (threadIdx.x & 31) * 8;
+#pragma unroll
+            for (int i = 0; i < 2 * MI; ++i) {
+                const int row = i * 8 + (threadIdx.x >> 5);
+                if (r0 + row < kv && c0 + col < H)
+                    __builtin_nontemporal_store(*reinterpret_cast<const f32x4*>(img + row * VH_ROWB + col * 2), reinterpret_cast<f32x4*>(dwb + (int64_t)(r0 + row) * lddw + c0 + col));
+            }
+            __syncthreads();
         }
     }
 }
@@ -770,8 +869,9 @@ Plan head_plan(int T, int V, int H, int K) {                         // K: targe
     // dh: K-slices so that few row tiles still fill the CUs (whole rounds of a tile's K-steps + ~14 of prologue / epilogue)
     const int tiles = st_cdiv(T, 256) * st_cdiv(H, 256), ncu = st_num_cus(), nkt = st_cdiv(std::min(V, p.piece), 64);
     p.split = 1;
+    if (p.few) p.split = std::max(1, std::min({2 * ncu / tiles, nkt / 8, 64}));       // two workgroups per CU, at least 16 steps of 32 each
     int64_t best = INT64_MAX;
-    for (int s = 1; s <= 32; ++s) {
+    for (int s = 1; s <= 32 && !p.few; ++s) {
         if (s > 1 && (nkt / s < 8 || (int64_t)s * T * H * 4 > ((int64_t)512 << 20))) break;
         const int64_t cost = (int64_t)st_cdiv((int64_t)tiles * s, ncu) * (st_cdiv(nkt, s) + 14) + 2 * s;
         if (cost < best) { best = cost; p.split = s; }
@@ -841,6 +941,24 @@ int head_stats(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, c
     return 0;
 }
 
+int launch_dh_few(const uint16_t* d, int64_t ldd, const uint16_t* w, int64_t ldw, int T, int kv, int H, int tiles_n, const Plan& p, bool accumulate,
+                  float* slab, hipStream_t s) {
+    const int nkt = st_cdiv(kv, 32), per = st_cdiv(nkt, p.split);
+    const dim3 grid(tiles_n * st_cdiv(nkt, per));
+    auto go = [&](auto kern, int smem) {
+        hipLaunchKernelGGL(kern, grid, dim3(256), smem, s, d, ldd, w, ldw, T, kv, H, tiles_n, per, slab);
+        ST_CHECK_LAUNCH();
+        return 0;
+    };
+    constexpr int S64 = 4 * (32 * 512 + 64 * 64), S128 = 3 * (32 * 512 + 128 * 64);
+    if (p.T64 == 64) {
+        allow_lds<head_dh_few_kernel<4, 4, false>>(S64); allow_lds<head_dh_few_kernel<4, 4, true>>(S64);
+        return accumulate ? go(head_dh_few_kernel<4, 4, true>, S64) : go(head_dh_few_kernel<4, 4, false>, S64);
+    }
+    allow_lds<head_dh_few_kernel<8, 3, false>>(S128); allow_lds<head_dh_few_kernel<8, 3, true>>(S128);
+    return accumulate ? go(head_dh_few_kernel<8, 3, true>, S128) : go(head_dh_few_kernel<8, 3, false>, S128);
+}
+
 // the pieces of a backward pass behind the row coefficients; `sparse` finishes d at the targets of a piece
 template <class F>
 int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, float sc, uint16_t* dh, int64_t lddh, uint16_t* dwb, float* dwf,
@@ -874,7 +992,10 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
         }
         const int rc = sparse(v0, kv, d, ldd, dt);
         if (rc) return rc;
-        if (dh) {
+        if (dh && p.few) {
+            const int rc = launch_dh_few(d, ldd, wp, ldw, T, kv, H, th, p, i > 0, slab, s);
+            if (rc) return rc;
+        } else if (dh) {
             const int nkt = st_cdiv(kv, 64), per = st_cdiv(nkt, p.split), slices = st_cdiv(nkt, per);      // (a short last piece may fill fewer slices)
             const dim3 grid(tm * th * slices);
             if (i == 0) hipLaunchKernelGGL((head_dh_kernel<false>), grid, dim3(256), VH_SMEM, s, d, ldd, wp, ldw, T, kv, H, tm, th, p.split, slab);
@@ -887,10 +1008,8 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
             uint16_t* ob = dwb ? dwb + (int64_t)v0 * lddw : nullptr;
             float* of = dwf ? dwf + (int64_t)v0 * lddw : nullptr;
             if (p.few) {
-                // columns per workgroup: about four workgroups per CU, so that loads, products and stores of several overlap
-                const int per = (int)up(st_cdiv(H, std::max(1, st_cdiv(4 * st_num_cus(), tv))), 64);
-                const dim3 few_grid(tv, st_cdiv(H, per));
-#define VH_DW_FEW(KS, OB, AC) hipLaunchKernelGGL((head_dw_few_kernel<KS, OB, AC>), few_grid, dim3(256), 0, s, dt, hzt, kv, H, per, ob, of, lddw)
+                const dim3 few_grid(st_cdiv(kv, 128));
+#define VH_DW_FEW(KS, OB, AC) hipLaunchKernelGGL((head_dw_few_kernel<KS, OB, AC>), few_grid, dim3(256), 0, s, dt, hzt, kv, H, ob, of, lddw)
                 if (p.T64 == 64) { if (dwb) VH_DW_FEW(2, true, false); else if (accumulate) VH_DW_FEW(2, false, true); else VH_DW_FEW(2, false, false); }
                 else { if (dwb) VH_DW_FEW(4, true, false); else if (accumulate) VH_DW_FEW(4, false, true); else VH_DW_FEW(4, false, false); }
 #undef VH_DW_FEW
@@ -902,7 +1021,7 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
         }
     }
     if (dh) {
-        const int nkt = st_cdiv(std::min(V, p.piece), 64), slices = st_cdiv(nkt, st_cdiv(nkt, p.split));
+        const int nkt = st_cdiv(std::min(V, p.piece), p.few ? 32 : 64), slices = st_cdiv(nkt, st_cdiv(nkt, p.split));
         hipLaunchKernelGGL(head_dh_finish_kernel, dim3(st_cdiv((int64_t)T * H, 1024)), dim3(256), 0, s, slab, slices, (const float*)(ws + p.scale), dh, lddh, T, H);
         ST_CHECK_LAUNCH();
     }
