@@ -5,6 +5,9 @@ kernels of libst_hip.so on torch's current stream and raises if a tensor is not 
 """
 from __future__ import annotations
 
+import contextlib
+import ctypes
+import functools
 import math
 
 import numpy as np
@@ -119,95 +122,113 @@ HEAD_MAX_VOCAB = 1 << 22        # VH_MAX_V of the library
 TOPK_MAX = 256                  # TK_MAX_K of the library
 
 
-def _on(device, *named):
-    """Every tensor on `device` — the kernels run on the current stream of that device."""
-    for t, what in named:
-        if t is not None and t.device != device:
-            raise RuntimeError(f"{what}: on {t.device}, expected {device}")
+def _current(device):
+    """Context in which `device` is the current one: the kernels run on its current stream (no context needed where it is current already)."""
+    return _NO_CONTEXT if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
-def _vec(t, dtype, shape, what):
+_NO_CONTEXT = contextlib.nullcontext()
+
+
+def _vec(t, dtype, shape, device, what):
+    """A contiguous tensor of this type and shape on `device`."""
     if t.dtype != dtype:
         raise TypeError(f"{what}: expected {dtype}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{what}: must be contiguous")
-    return t
+    if t.device != device:
+        raise RuntimeError(f"{what}: on {t.device}, expected {device}")
+
+
+def _positive(temperature):
+    if not (temperature > 0.0 and math.isfinite(temperature) and math.isfinite(1.0 / temperature)):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
 
 
 def _head_operands(hidden, weight, temperature):
+    """(T, V, H, row pitch of hidden, row pitch of weight) after the checks of a head's operands."""
     _chk(hidden, BF16, "hidden"); _chk(weight, BF16, "weight")
     if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
         raise ValueError(f"hidden (T, H) and weight (V, H): got {tuple(hidden.shape)} and {tuple(weight.shape)}")
     T, H = hidden.shape
-    if weight.shape[0] == 0 or H == 0 or H % 64:
-        raise ValueError(f"the head needs at least one token and a width in multiples of 64, got {tuple(weight.shape)}")
-    if not (temperature > 0.0 and math.isfinite(temperature) and math.isfinite(1.0 / temperature)):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
-    for t, what in ((hidden, "hidden"), (weight, "weight")):
-        if t.shape[0] and (t.data_ptr() & 15 or t.stride(0) & 7 or t.stride(0) < H or t.stride(0) >= 1 << 22):
-            raise ValueError(f"{what}: rows must be 16-byte aligned and not overlap (stride {t.stride(0)})")
+    V = weight.shape[0]
+    if not 0 < V <= HEAD_MAX_VOCAB or H == 0 or H % 64:
+        raise ValueError(f"the head needs 1..{HEAD_MAX_VOCAB} tokens and a width in multiples of 64, got {tuple(weight.shape)}")
+    _positive(temperature)
+    ldh, ldw = hidden.stride(0), weight.stride(0)
+    if T and (hidden.data_ptr() & 15 or ldh & 7 or not H <= ldh < 1 << 22):
+        raise ValueError(f"hidden: rows must be 16-byte aligned and not overlap (stride {ldh})")
+    if weight.data_ptr() & 15 or ldw & 7 or not H <= ldw < 1 << 22:
+        raise ValueError(f"weight: rows must be 16-byte aligned and not overlap (stride {ldw})")
     if not hidden.is_cuda:
         _p(hidden)
-    _on(hidden.device, (weight, "weight"))
-    if weight.shape[0] > HEAD_MAX_VOCAB:
-        raise ValueError(f"vocabularies up to {HEAD_MAX_VOCAB} tokens, got {weight.shape[0]}")
-    return T, weight.shape[0], H
+    if weight.device != hidden.device:
+        raise RuntimeError(f"weight: on {weight.device}, expected {hidden.device}")
+    return T, V, H, ldh, ldw
+
+
+@functools.lru_cache(maxsize=4096)
+def _head_workspace_bytes(T, V, H, K, backward):
+    n = ctypes.c_int64(0)
+    lib().st_linear_head_workspace_bytes(T, V, H, K, backward, ctypes.addressof(n), None)
+    return n.value
 
 
 def _head_workspace(T, V, H, K, backward, device):
     """Scratch of one call, from torch's stream-ordered allocator (a captured graph gets its own from its pool)."""
-    import ctypes
-    n = ctypes.c_int64(0)
-    lib().st_linear_head_workspace_bytes(T, V, H, K, int(backward), ctypes.addressof(n), None)
-    return torch.empty(n.value, dtype=torch.uint8, device=device)
+    return torch.empty(_head_workspace_bytes(T, V, H, K, backward), dtype=torch.uint8, device=device)
 
 
 def _head_grads(hidden, weight, want_dhidden, dweight, dweight_f32, accumulate):
-    """(dhidden or None) after the checks of the gradient outputs."""
+    """(dhidden or None, row pitch of the weight gradient) after the checks of the gradient outputs."""
     if dweight is not None and (dweight_f32 is not None or accumulate):
         raise ValueError("dweight: one of bf16 (overwritten) and fp32 (optionally accumulated)")
-    for t, dt, what in ((dweight, BF16, "dweight"), (dweight_f32, F32, "dweight_f32")):
+    pitch = 0
+    for t, dt, align, what in ((dweight, BF16, 8, "dweight"), (dweight_f32, F32, 4, "dweight_f32")):
         if t is not None:
             _chk(t, dt, what)
-            if t.shape != weight.shape or t.data_ptr() & 15 or t.stride(0) % (16 // t.element_size()) or t.stride(0) < t.shape[1]:
+            pitch = t.stride(0)
+            if t.shape != weight.shape or t.data_ptr() & 15 or pitch % align or pitch < t.shape[1]:
                 raise ValueError(f"{what}: expected {tuple(weight.shape)} with 16-byte aligned rows")
-            _on(hidden.device, (t, what))
-    return torch.empty(hidden.shape, dtype=BF16, device=hidden.device) if want_dhidden else None
+            if t.device != hidden.device:
+                raise RuntimeError(f"{what}: on {t.device}, expected {hidden.device}")
+    return torch.empty(hidden.shape, dtype=BF16, device=hidden.device) if want_dhidden else None, pitch
 
 
-def _ld(t):
-    return t.stride(0) if t is not None else 0
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def linear_logprob_fwd(hidden, weight, labels, temperature: float = 1.0):
     """hidden (T,H) bf16, weight (V,H) bf16, labels (T,) int64 -> (logp (T,) f32, lse (T,) f32) of z = hidden @ weight^T / temperature, whose
     logits are never stored.  Labels outside [0, V): rows that are not scored (logp 0)."""
-    T, V, H = _head_operands(hidden, weight, temperature)
-    _vec(labels, I64, (T,), "labels"); _on(hidden.device, (labels, "labels"))
-    with torch.cuda.device(hidden.device):
-        logp = torch.empty(T, dtype=F32, device=hidden.device)
-        lse = torch.empty(T, dtype=F32, device=hidden.device)
+    T, V, H, ldh, ldw = _head_operands(hidden, weight, temperature)
+    dev = hidden.device
+    _vec(labels, I64, (T,), dev, "labels")
+    with _current(dev):
+        logp = torch.empty(T, dtype=F32, device=dev)
+        lse = torch.empty(T, dtype=F32, device=dev)
         if T:
-            ws = _head_workspace(T, V, H, 0, False, hidden.device)
-            lib().st_linear_logprob_fwd(_p(hidden), hidden.stride(0), _p(weight), weight.stride(0), _p(labels), 1.0 / temperature, _p(logp), _p(lse),
-                                        _p(ws), ws.numel(), T, V, H, _s())
+            ws = _head_workspace(T, V, H, 0, 0, dev)
+            lib().st_linear_logprob_fwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, labels.data_ptr(), 1.0 / temperature, logp.data_ptr(), lse.data_ptr(),
+                                        ws.data_ptr(), ws.numel(), T, V, H, torch._C._cuda_getCurrentRawStream(dev.index))
     return logp, lse
 
 
 def linear_logprob_bwd(hidden, weight, labels, logp, lse, g, temperature: float = 1.0, *, want_dhidden=True, dweight=None, dweight_f32=None, accumulate=False):
     """Gradients of sum(g * logp): returns dhidden (T,H) bf16 (None unless wanted); dweight (bf16, overwritten) or dweight_f32 (fp32, accumulate:
     added to) is filled in place."""
-    T, V, H = _head_operands(hidden, weight, temperature)
-    for t, dt, what in ((labels, I64, "labels"), (logp, F32, "logp"), (lse, F32, "lse"), (g, F32, "g")):
-        _vec(t, dt, (T,), what); _on(hidden.device, (t, what))
-    with torch.cuda.device(hidden.device):
-        dh = _head_grads(hidden, weight, want_dhidden, dweight, dweight_f32, accumulate)
-        ws = _head_workspace(T, V, H, 0, True, hidden.device)
-        lib().st_linear_logprob_bwd(_p(hidden), hidden.stride(0), _p(weight), weight.stride(0), _p(labels), _p(logp), _p(lse), _p(g), 1.0 / temperature,
-                                    _p(dh), _ld(dh), _p(dweight), _p(dweight_f32), _ld(dweight if dweight is not None else dweight_f32),
-                                    int(accumulate), _p(ws), ws.numel(), T, V, H, _s())
+    T, V, H, ldh, ldw = _head_operands(hidden, weight, temperature)
+    dev = hidden.device
+    _vec(labels, I64, (T,), dev, "labels"); _vec(logp, F32, (T,), dev, "logp"); _vec(lse, F32, (T,), dev, "lse"); _vec(g, F32, (T,), dev, "g")
+    with _current(dev):
+        dh, lddw = _head_grads(hidden, weight, want_dhidden, dweight, dweight_f32, accumulate)
+        ws = _head_workspace(T, V, H, 0, 1, dev)
+        lib().st_linear_logprob_bwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, labels.data_ptr(), logp.data_ptr(), lse.data_ptr(), g.data_ptr(),
+                                    1.0 / temperature, _ptr(dh), H, _ptr(dweight), _ptr(dweight_f32), lddw, int(accumulate), ws.data_ptr(), ws.numel(),
+                                    T, V, H, torch._C._cuda_getCurrentRawStream(dev.index))
     return dh
 
 
@@ -216,67 +237,75 @@ def _topk_targets(hidden, ids, teacher_logp, T):
         raise ValueError(f"ids: expected ({T}, 1..{HEAD_MAX_TARGETS}), got {tuple(ids.shape)}")
     if ids.numel() >= 1 << 31:
         raise ValueError(f"ids: fewer than 2^31 entries, got {tuple(ids.shape)}")
-    _vec(ids, I32, ids.shape, "ids"); _vec(teacher_logp, F32, ids.shape, "teacher_logp")
-    _on(hidden.device, (ids, "ids"), (teacher_logp, "teacher_logp"))
+    _vec(ids, I32, ids.shape, hidden.device, "ids"); _vec(teacher_logp, F32, ids.shape, hidden.device, "teacher_logp")
     return ids.shape[1]
 
 
 def linear_topk_kl_fwd(hidden, weight, ids, teacher_logp, temperature: float = 1.0, renormalize: bool = False):
     """ids (T,K) int32, teacher_logp (T,K) f32 -> (kl (T,) f32, lse (T,) f32, logq (T,K) f32): kl = sum_k p_k (log p_k - log q[ids_k]) with
     p = exp(teacher_logp), or its softmax over the row's entries; entries with an id outside [0, V) are absent (st_linear_topk_kl_fwd)."""
-    T, V, H = _head_operands(hidden, weight, temperature)
+    T, V, H, ldh, ldw = _head_operands(hidden, weight, temperature)
     K = _topk_targets(hidden, ids, teacher_logp, T)
-    with torch.cuda.device(hidden.device):
-        kl = torch.empty(T, dtype=F32, device=hidden.device)
-        lse = torch.empty(T, dtype=F32, device=hidden.device)
-        logq = torch.empty(T, K, dtype=F32, device=hidden.device)
+    dev = hidden.device
+    with _current(dev):
+        kl = torch.empty(T, dtype=F32, device=dev)
+        lse = torch.empty(T, dtype=F32, device=dev)
+        logq = torch.empty(T, K, dtype=F32, device=dev)
         if T:
-            ws = _head_workspace(T, V, H, K, False, hidden.device)
-            lib().st_linear_topk_kl_fwd(_p(hidden), hidden.stride(0), _p(weight), weight.stride(0), _p(ids), _p(teacher_logp), K, int(renormalize),
-                                        1.0 / temperature, _p(kl), _p(lse), _p(logq), _p(ws), ws.numel(), T, V, H, _s())
+            ws = _head_workspace(T, V, H, K, 0, dev)
+            lib().st_linear_topk_kl_fwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, ids.data_ptr(), teacher_logp.data_ptr(), K, int(renormalize),
+                                        1.0 / temperature, kl.data_ptr(), lse.data_ptr(), logq.data_ptr(), ws.data_ptr(), ws.numel(), T, V, H,
+                                        torch._C._cuda_getCurrentRawStream(dev.index))
     return kl, lse, logq
 
 
 def linear_topk_kl_bwd(hidden, weight, ids, teacher_logp, lse, logq, g, temperature: float = 1.0, renormalize: bool = False, *, want_dhidden=True,
                        dweight=None, dweight_f32=None, accumulate=False):
     """Gradients of sum(g * kl); outputs as linear_logprob_bwd."""
-    T, V, H = _head_operands(hidden, weight, temperature)
+    T, V, H, ldh, ldw = _head_operands(hidden, weight, temperature)
     K = _topk_targets(hidden, ids, teacher_logp, T)
-    for t, shape, what in ((lse, (T,), "lse"), (logq, (T, K), "logq"), (g, (T,), "g")):
-        _vec(t, F32, shape, what); _on(hidden.device, (t, what))
-    with torch.cuda.device(hidden.device):
-        dh = _head_grads(hidden, weight, want_dhidden, dweight, dweight_f32, accumulate)
-        ws = _head_workspace(T, V, H, K, True, hidden.device)
-        lib().st_linear_topk_kl_bwd(_p(hidden), hidden.stride(0), _p(weight), weight.stride(0), _p(ids), _p(teacher_logp), K, int(renormalize),
-                                    1.0 / temperature, _p(lse), _p(logq), _p(g), _p(dh), _ld(dh), _p(dweight), _p(dweight_f32),
-                                    _ld(dweight if dweight is not None else dweight_f32), int(accumulate), _p(ws), ws.numel(), T, V, H, _s())
+    dev = hidden.device
+    _vec(lse, F32, (T,), dev, "lse"); _vec(logq, F32, (T, K), dev, "logq"); _vec(g, F32, (T,), dev, "g")
+    with _current(dev):
+        dh, lddw = _head_grads(hidden, weight, want_dhidden, dweight, dweight_f32, accumulate)
+        ws = _head_workspace(T, V, H, K, 1, dev)
+        lib().st_linear_topk_kl_bwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, ids.data_ptr(), teacher_logp.data_ptr(), K, int(renormalize),
+                                    1.0 / temperature, lse.data_ptr(), logq.data_ptr(), g.data_ptr(), _ptr(dh), H, _ptr(dweight), _ptr(dweight_f32), lddw,
+                                    int(accumulate), ws.data_ptr(), ws.numel(), T, V, H, torch._C._cuda_getCurrentRawStream(dev.index))
     return dh
+
+
+@functools.lru_cache(maxsize=4096)
+def _topk_workspace_bytes(T, V, k):
+    n = ctypes.c_int64(0)
+    lib().st_topk_logprob_workspace_bytes(T, V, k, ctypes.addressof(n), None)
+    return n.value
 
 
 def topk_logprob(logits, k: int, temperature: float = 1.0):
     """logits (T,V) bf16 -> (ids (T,k) int32, logp (T,k) f32, lse (T,) f32): the k largest log-probs of logits / temperature per row in falling
     order, equal logits by rising id."""
-    import ctypes
     _chk(logits, BF16, "logits")
     if logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError(f"logits: expected (T, V), got {tuple(logits.shape)}")
     T, V = logits.shape
     if not 1 <= k <= min(TOPK_MAX, V):
         raise ValueError(f"k must be in 1..{min(TOPK_MAX, V)}, got {k}")
-    if T > 1 and logits.stride(0) < V:
-        raise ValueError(f"logits: rows overlap (stride {logits.stride(0)})")
-    if not (temperature > 0.0 and math.isfinite(temperature) and math.isfinite(1.0 / temperature)):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    ldl = logits.stride(0)
+    if T > 1 and ldl < V:
+        raise ValueError(f"logits: rows overlap (stride {ldl})")
+    _positive(temperature)
     _p(logits)
-    with torch.cuda.device(logits.device):
-        ids = torch.empty(T, k, dtype=I32, device=logits.device)
-        logp = torch.empty(T, k, dtype=F32, device=logits.device)
-        lse = torch.empty(T, dtype=F32, device=logits.device)
+    dev = logits.device
+    with _current(dev):
+        ids = torch.empty(T, k, dtype=I32, device=dev)
+        logp = torch.empty(T, k, dtype=F32, device=dev)
+        lse = torch.empty(T, dtype=F32, device=dev)
         if T:
-            n = ctypes.c_int64(0)
-            lib().st_topk_logprob_workspace_bytes(T, V, k, ctypes.addressof(n), None)
-            ws = torch.empty(n.value, dtype=torch.uint8, device=logits.device) if n.value else None
-            lib().st_topk_logprob(_p(logits), max(logits.stride(0), V), k, 1.0 / temperature, _p(ids), _p(logp), _p(lse), _p(ws), n.value, T, V, _s())
+            n = _topk_workspace_bytes(T, V, k)
+            ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+            lib().st_topk_logprob(logits.data_ptr(), max(ldl, V), k, 1.0 / temperature, ids.data_ptr(), logp.data_ptr(), lse.data_ptr(), _ptr(ws), n, T, V,
+                                  torch._C._cuda_getCurrentRawStream(dev.index))
     return ids, logp, lse
 
 

@@ -122,6 +122,12 @@ def log_probs_from_logits_flash_attn(logits: torch.Tensor, labels: torch.Tensor)
     return log_probs_from_logits(logits, labels)
 
 
+def _once(ctx):
+    """Inside a backward, gradients are recorded only for a second derivative, which these operators do not have."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{type(ctx).__name__}: the head operators can be differentiated once (create_graph=True is not supported)")
+
+
 class _LinearLogProbs(torch.autograd.Function):
     """log-probs of given tokens from hidden states and head weight, the logits never stored (st_linear_logprob_fwd / _bwd).  The backward forms
     the logits again, piece by piece of the vocabulary; only the gradients that autograd asks for are computed."""
@@ -135,9 +141,9 @@ class _LinearLogProbs(torch.autograd.Function):
         return logp
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
         from spatialthinker_amd import ops
+        _once(ctx)
         hidden, weight, labels, logp, lse = ctx.saved_tensors
         dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if ctx.needs_input_grad[1] else None
         dh = ops.linear_logprob_bwd(hidden, weight, labels, logp, lse, grad_out.contiguous().float(), ctx.temperature,
@@ -155,9 +161,9 @@ class _LinearTopkKL(torch.autograd.Function):
         return kl
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
         from spatialthinker_amd import ops
+        _once(ctx)
         hidden, weight, ids, teacher, lse, logq = ctx.saved_tensors
         dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if ctx.needs_input_grad[1] else None
         dh = ops.linear_topk_kl_bwd(hidden, weight, ids, teacher, lse, logq, grad_out.contiguous().float(), ctx.temperature, ctx.renormalize,
@@ -165,14 +171,19 @@ class _LinearTopkKL(torch.autograd.Function):
         return dh, dw, None, None, None, None
 
 
-def _head_rows(hidden: torch.Tensor, weight: torch.Tensor):
-    """(rows of hidden (T, H), weight) as the head kernels take them: bf16, rows contiguous and 16-byte aligned (a copy only where they are not).
-    Both casts are differentiable: fp32 inputs get fp32 gradients."""
-    def rows(t):
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """t as (rows, width) bf16 with contiguous 16-byte aligned rows: itself where it is that, else a differentiable cast / view / copy."""
+    if t.dtype != torch.bfloat16:
         t = t.to(torch.bfloat16)
-        ok = t.shape[0] == 0 or (t.stride(-1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0)
-        return t if ok else t.clone(memory_format=torch.contiguous_format)
-    return rows(hidden.reshape(-1, hidden.shape[-1])), rows(weight)
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if t.shape[0] == 0 or (t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _flat(t: torch.Tensor, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    return t.to(device=device, dtype=dtype).contiguous().view(-1)
 
 
 def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
@@ -180,11 +191,10 @@ def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.T
     -> (...) fp32, differentiable in hidden and weight.  At V = 152 064 the logits of 8192 rows are 2.5 GB; here the backward's workspace stays
     within 0.5 GiB for one piece of the vocabulary and the logits stay in fp32.  A label outside [0, V) (padding, -100) marks a row that is not
     scored: 0, and no gradient from it.  H must be a multiple of 64; GPU tensors only."""
-    h, w = _head_rows(hidden, weight)
     if labels.shape != hidden.shape[:-1]:
         raise ValueError(f"labels {tuple(labels.shape)} do not match hidden {tuple(hidden.shape)}")
-    lab = labels.to(device=h.device, dtype=torch.int64).contiguous().view(-1)
-    return _LinearLogProbs.apply(h, w, lab, float(temperature)).view(labels.shape)
+    out = _LinearLogProbs.apply(_rows16(hidden), _rows16(weight), _flat(labels, torch.int64, hidden.device), float(temperature))
+    return out if labels.dim() == 1 else out.view(labels.shape)
 
 
 def linear_topk_kl(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor, teacher_log_probs: torch.Tensor, temperature: float = 1.0,
@@ -194,15 +204,15 @@ def linear_topk_kl(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torc
     hidden (..., H), weight (V, H), teacher_ids / teacher_log_probs (..., K) -> (...) fp32, differentiable in hidden and weight (the teacher is a
     constant).  renormalize: p is scaled to sum 1 over the row's entries; without it the mass outside the teacher's top K counts for nothing.
     Entries with an id outside [0, V) are absent; a row of such entries gives 0 and no gradient.  K <= 1024."""
-    h, w = _head_rows(hidden, weight)
     if teacher_ids.shape[:-1] != hidden.shape[:-1] or teacher_ids.shape != teacher_log_probs.shape:
         raise ValueError(f"teacher ids {tuple(teacher_ids.shape)} / log-probs {tuple(teacher_log_probs.shape)} do not match hidden {tuple(hidden.shape)}")
     k = teacher_ids.shape[-1]
     if teacher_ids.dtype != torch.int32:                         # int64 ids that int32 cannot hold must stay outside [0, V)
         teacher_ids = teacher_ids.clamp(-1, 0x7fffffff).to(torch.int32)
-    ids = teacher_ids.to(h.device).contiguous().view(-1, k)
-    a = teacher_log_probs.detach().to(device=h.device, dtype=torch.float32).contiguous().view(-1, k)
-    return _LinearTopkKL.apply(h, w, ids, a, float(temperature), bool(renormalize)).view(hidden.shape[:-1])
+    ids = _flat(teacher_ids, torch.int32, hidden.device).view(-1, k)
+    a = _flat(teacher_log_probs.detach(), torch.float32, hidden.device).view(-1, k)
+    out = _LinearTopkKL.apply(_rows16(hidden), _rows16(weight), ids, a, float(temperature), bool(renormalize))
+    return out if hidden.dim() == 2 else out.view(hidden.shape[:-1])
 
 
 @torch.no_grad()
@@ -210,12 +220,16 @@ def top_log_probs(logits: torch.Tensor, k: int, temperature: float = 1.0):
     """The k largest log-probs of logits / temperature: logits (..., V) -> (ids (..., k) int32, log-probs (..., k) fp32, lse (...) fp32), in falling
     order, equal logits by rising id.  What a teacher hands to linear_topk_kl.  bf16 logits (anything else is rounded to bf16 first, as
     log_probs_from_logits does); k <= 256."""
-    batch_dim, vocab = logits.shape[:-1], logits.shape[-1]
-    z = logits.to(torch.bfloat16).reshape(-1, vocab)
+    from spatialthinker_amd import ops
+    z = logits if logits.dtype == torch.bfloat16 else logits.to(torch.bfloat16)
+    if z.dim() != 2:
+        z = z.reshape(-1, z.shape[-1])
     if z.stride(-1) != 1:
         z = z.contiguous()
-    from spatialthinker_amd import ops
     ids, logp, lse = ops.topk_logprob(z, int(k), float(temperature))
+    if logits.dim() == 2:
+        return ids, logp, lse
+    batch_dim = logits.shape[:-1]
     return ids.view(*batch_dim, k), logp.view(*batch_dim, k), lse.view(batch_dim)
 
 
