@@ -174,7 +174,7 @@ __global__ __launch_bounds__(256) void head_tile_kernel(const uint16_t* __restri
 // The same logit tile for few rows (T <= 128): the launch is a stream of the head's weights, so the tile is small and several workgroups share a CU
 // to keep copies in flight: BT = 16 MT rows x 128 vocabulary columns, four waves of 32 columns each, K-steps of 64 through SLOTS LDS slots filled
 // by LDS-DMA (16-byte chunk c of a row at position c ^ (row & 7): conflict-free fragment reads), SLOTS - 1 steps in flight behind one barrier per
-// step.  Epilogues as head_tile_kernel; part[n0 / 128][m].  DLOGITS also leaves d transposed, dt[n][T64], for head_dw_few_kernel.
+// step.  Epilogues as head_tile_kernel; part[n0 / 128][m].  DLOGITS also leaves d transposed, dt[n][TP], for head_dw_few_kernel.
 // ------------------------------------------------------------------------------------------------------------------------------------
 template <int N> __device__ __forceinline__ void vh_wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
@@ -182,7 +182,7 @@ template <int MT, int SLOTS, bool DLOGITS>
 __global__ __launch_bounds__(256, 2) void head_few_kernel(const uint16_t* __restrict__ h, int64_t ldh, const uint16_t* __restrict__ w, int64_t ldw, int T, int V,
                                                          int H, float sc, const int64_t* __restrict__ labels, float2* __restrict__ part,
                                                          float* __restrict__ zlab, VhTargets tg, const VhRow* __restrict__ rows, int v0,
-                                                         uint16_t* __restrict__ d, int64_t ldd, uint16_t* __restrict__ dt, int T64) {
+                                                         uint16_t* __restrict__ d, int64_t ldd, uint16_t* __restrict__ dt, int TP) {
     constexpr int BT = 16 * MT, SLOT = (128 + BT) * 128, HC = MT / 2;    // HC: 1-KiB copies of h per wave and step
     static_assert(MT % 2 == 0, "every wave copies the same number of rows");
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -328,15 +328,14 @@ __global__ __launch_bounds__(256, 2) void head_few_kernel(const uint16_t* __rest
         }
         __syncthreads();
         const int cols = min(128, (int)ldd - n0);                    // ldd % 64 == 0
-        for (int i = threadIdx.x; i < T64 * 16; i += 256) {
+        for (int i = threadIdx.x; i < T * 16; i += 256) {
             const int row = i >> 4, c = (i & 15) * 8;
-            if (c < cols)
-                *reinterpret_cast<uint4*>(d + (int64_t)row * ldd + n0 + c) = row < BT ? *reinterpret_cast<const uint4*>(smem + row * RB + c * 2) : make_uint4(0, 0, 0, 0);
+            if (c < cols) *reinterpret_cast<uint4*>(d + (int64_t)row * ldd + n0 + c) = *reinterpret_cast<const uint4*>(smem + row * RB + c * 2);
         }
-        const int per = T64 >> 3;                                    // 16-byte chunks of a row of dt
+        const int per = TP >> 3;                                     // 16-byte chunks of a row of dt: TP is BT, or more (zeros)
         for (int i = threadIdx.x; i < cols * per; i += 256) {
             const int col = i / per, c = (i - col * per) * 8;
-            *reinterpret_cast<uint4*>(dt + (int64_t)(n0 + col) * T64 + c) = c < BT ? *reinterpret_cast<const uint4*>(img_t + col * CB + c * 2) : make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(dt + (int64_t)(n0 + col) * TP + c) = c < BT ? *reinterpret_cast<const uint4*>(img_t + col * CB + c * 2) : make_uint4(0, 0, 0, 0);
         }
     }
 }
@@ -351,6 +350,7 @@ __global__ __launch_bounds__(1024) void head_lse_kernel(const float2* __restrict
     const int row = blockIdx.x * 16 + r;
     float m = -INFINITY, s = 0.f;
     if (row < T)
+#pragma unroll 4
         for (int p = sl; p < n_parts; p += 64) {
             const float2 v = part[(int64_t)p * T + row];
             const float mn = fmaxf(m, v.x);
@@ -455,7 +455,8 @@ __global__ __launch_bounds__(256) void head_dh_kernel(const uint16_t* __restrict
     }
 }
 
-// The same for few rows (T64 <= 128): a stream of w, [32 vocabulary rows][256 columns] per step through SLOTS LDS slots, next to a [T64][32] tile of d.
+// The same for few rows (T <= 128): a stream of w, [32 vocabulary rows][256 columns] per step through SLOTS LDS slots, next to a [16 MT][32] tile of d
+// (rows beyond T: the last one, never stored).
 // w is contraction-major: its fragments are LDS transpose reads (image and swizzle as the contraction-major operands of gemm_asm4.hip).  Four
 // waves of 64 columns, all rows each; the vocabulary is cut into slices so that every CU has two workgroups.
 template <int MT, int SLOTS, bool ACCUM>
@@ -478,7 +479,7 @@ __global__ __launch_bounds__(256, 2) void head_dh_few_kernel(const uint16_t* __r
 #pragma unroll
     for (int j = 0; j < DC; ++j) {                                   // copies of d: 16 rows of 64 bytes, 16-byte chunk (lane & 3) ^ (row >> 2)
         const int row = (wave * DC + j) * 16 + (lane >> 2);
-        dsrc[j] = d + (int64_t)row * ldd + (((lane & 3) ^ ((row >> 2) & 3)) << 3);
+        dsrc[j] = d + (int64_t)min(row, T - 1) * ldd + (((lane & 3) ^ ((row >> 2) & 3)) << 3);
     }
     auto stage = [&](int kt) {
         char* dst = smem + (kt % SLOTS) * SLOT;
@@ -608,14 +609,14 @@ __global__ __launch_bounds__(256) void head_dw_kernel(const uint16_t* __restrict
     }
 }
 
-// dw for few rows (T64 <= 128): the launch is the write of dw, V H elements, next to 2 KS products of 32 rows each.  Operands stand contraction-
-// contiguous (dt[v][T64], hzt[n][T64]), so fragments come straight from memory: dt once per workgroup, hzt from the caches, a step ahead.  A
+// dw for few rows (TP = 32 KS, T rounded up to 32, 64 or 128): the launch is the write of dw, V H elements, next to 2 KS products of 32 rows each.  Operands stand contraction-
+// contiguous (dt[v][TP], hzt[n][TP]), so fragments come straight from memory: dt once per workgroup, hzt from the caches, a step ahead.  A
 // workgroup owns 128 vocabulary rows and walks the columns 256 at a time, 64 per wave; the bf16 tile goes through LDS, because a row has to leave in
 // long runs: 64-byte pieces of 16 rows at a pitch of H elements meet in a few cache channels (V = 152 064, H = 3584: 292 us against 160 for a fill).
 template <int KS, bool OUT_BF16, bool ACCUM>
 __global__ __launch_bounds__(256) void head_dw_few_kernel(const uint16_t* __restrict__ dt, const uint16_t* __restrict__ hzt, int kv, int H,
                                                          uint16_t* __restrict__ dwb, float* __restrict__ dwf, int64_t lddw) {
-    constexpr int T64 = KS * 32, MI = 8;                             // 16 MI vocabulary rows per workgroup
+    constexpr int TP = KS * 32, MI = 8;                             // 16 MI vocabulary rows per workgroup
     __shared__ __attribute__((aligned(16))) char img[OUT_BF16 ? 16 * MI * VH_ROWB : 16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fk = lane >> 4;
     const int r0 = blockIdx.x * (16 * MI);
@@ -623,14 +624,14 @@ __global__ __launch_bounds__(256) void head_dw_few_kernel(const uint16_t* __rest
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
-        for (int s = 0; s < KS; ++s) df[mi][s] = *reinterpret_cast<const bf16x8*>(dt + (int64_t)min(r0 + mi * 16 + fr, kv - 1) * T64 + s * 32 + fk * 8);
+        for (int s = 0; s < KS; ++s) df[mi][s] = *reinterpret_cast<const bf16x8*>(dt + (int64_t)min(r0 + mi * 16 + fr, kv - 1) * TP + s * 32 + fk * 8);
     auto fetch = [&](int c) {                                        // (columns beyond H: the last ones, never stored)
 #pragma unroll
         for (int ni = 0; ni < 4; ++ni)
 #pragma unroll
-            for (int s = 0; s < KS; ++s) ahead[ni][s] = *reinterpret_cast<const bf16x8*>(hzt + (int64_t)min(c + ni * 16 + fr, H - 1) * T64 + s * 32 + fk * 8);
+            for (int s = 0; s < KS; ++s) ahead[ni][s] = *reinterpret_cast<const bf16x8*>(hzt + (int64_t)min(c + ni * 16 + fr, H - 1) * TP + s * 32 + fk * 8);
     };
-    if constexpr (KS == 2) fetch(wave * 64);
+    if constexpr (KS <= 2) fetch(wave * 64);
     for (int c0 = 0; c0 < H; c0 += 256) {
         const int c = c0 + wave * 64;
         if constexpr (KS > 2) fetch(c);                              // (no registers left to be a step ahead)
@@ -638,7 +639,7 @@ __global__ __launch_bounds__(256) void head_dw_few_kernel(const uint16_t* __rest
         for (int ni = 0; ni < 4; ++ni)
 #pragma unroll
             for (int s = 0; s < KS; ++s) hf[ni][s] = ahead[ni][s];
-        if constexpr (KS == 2) fetch(c + 256);
+        if constexpr (KS <= 2) fetch(c + 256);
 #pragma unroll
         for (int mi = 0; mi < MI; ++mi) {
 #pragma unroll
@@ -674,8 +675,8 @@ __global__ __launch_bounds__(256) void head_dw_few_kernel(const uint16_t* __rest
     }
 }
 
-// hzt[n][t] = hz[t][n]: 64 x 64 elements per workgroup
-__global__ __launch_bounds__(256) void head_hzt_kernel(const uint16_t* __restrict__ hz, uint16_t* __restrict__ hzt, int T64, int H) {
+// hzt[n][t] = hz[t][n], t < TP <= 64 ceil(T / 64): 64 x 64 elements per workgroup
+__global__ __launch_bounds__(256) void head_hzt_kernel(const uint16_t* __restrict__ hz, uint16_t* __restrict__ hzt, int TP, int H) {
     __shared__ uint16_t tile[64][72];
     const int n0 = blockIdx.x * 64, t0 = blockIdx.y * 64;
     for (int i = threadIdx.x; i < 64 * 8; i += 256)
@@ -683,10 +684,11 @@ __global__ __launch_bounds__(256) void head_hzt_kernel(const uint16_t* __restric
     __syncthreads();
     for (int i = threadIdx.x; i < 64 * 8; i += 256) {
         const int n = i >> 3, c = (i & 7) * 8;
+        if (t0 + c >= TP) continue;
         uint4 o;
         o.x = tile[c][n] | (uint32_t)tile[c + 1][n] << 16; o.y = tile[c + 2][n] | (uint32_t)tile[c + 3][n] << 16;
         o.z = tile[c + 4][n] | (uint32_t)tile[c + 5][n] << 16; o.w = tile[c + 6][n] | (uint32_t)tile[c + 7][n] << 16;
-        *reinterpret_cast<uint4*>(hzt + (int64_t)(n0 + n) * T64 + t0 + c) = o;
+        *reinterpret_cast<uint4*>(hzt + (int64_t)(n0 + n) * TP + t0 + c) = o;
     }
 }
 
@@ -815,7 +817,7 @@ __global__ __launch_bounds__(128) void head_rows_kl_kernel(const uint16_t* __res
 // log q of the forward pass.  An id that a row holds twice gets the sum of its probabilities from both entries: the same value twice.
 __global__ __launch_bounds__(256) void head_sparse_kernel(const int32_t* __restrict__ ids, const float* __restrict__ a, int K, int renorm,
                                                          const float* __restrict__ logq, const VhRow* __restrict__ rows, int v0, int kv,
-                                                         uint16_t* __restrict__ d, int64_t ldd, uint16_t* __restrict__ dt, int T64, int T, int V) {
+                                                         uint16_t* __restrict__ d, int64_t ldd, uint16_t* __restrict__ dt, int TP, int T, int V) {
     const int lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (t >= T) return;
     ids += (int64_t)t * K; a += (int64_t)t * K; logq += (int64_t)t * K;
@@ -830,7 +832,7 @@ __global__ __launch_bounds__(256) void head_sparse_kernel(const int32_t* __restr
         for (int j = 0; j < K; ++j) if (ids[j] == id) p += vh_exp2((a[j] - th.shift) * VH_LOG2E);
         const uint16_t x = f2bf(r * (th.total * vh_exp2(logq[k] * VH_LOG2E) - p));
         d[(int64_t)t * ldd + id - v0] = x;
-        if (dt) dt[(int64_t)(id - v0) * T64 + t] = x;
+        if (dt) dt[(int64_t)(id - v0) * TP + t] = x;
     }
 }
 
@@ -843,7 +845,7 @@ __global__ __launch_bounds__(256) void head_zero_kernel(char* __restrict__ p, in
 // ------------------------------------------------------------------------------------------------------------------------------------
 namespace {
 struct Plan {                                                        // workspace layout (byte offsets) and piece / slice counts of one call
-    int T64, pieces, piece, split;
+    int T64, TP, pieces, piece, split;                               // TP: row pitch of the transposed operands of head_dw_few_kernel
     int64_t part, zlab, stat, start, list, fwd_bytes;
     int64_t rows, scale, hz, hzt, d, dt, slab, bwd_bytes;
     bool few;                                                        // the weight-streaming kernels
@@ -854,6 +856,7 @@ Plan head_plan(int T, int V, int H, int K) {                         // K: targe
     Plan p;
     p.T64 = (int)up(T, 64);
     p.few = T <= VH_FEW;
+    p.TP = T <= 32 ? 32 : p.T64;
     const int64_t n_parts = 2 * (int64_t)st_cdiv(V, 256);
     p.part = 0;
     p.zlab = up(n_parts * T * 8, 256);
@@ -974,7 +977,7 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
     allow_lds<head_dh_kernel<false>>(); allow_lds<head_dh_kernel<true>>();
     allow_lds<head_dw_kernel<true, false>>(); allow_lds<head_dw_kernel<false, false>>(); allow_lds<head_dw_kernel<false, true>>();
     if (p.few && (dwb || dwf)) {
-        hipLaunchKernelGGL(head_hzt_kernel, dim3(H / 64, p.T64 / 64), dim3(256), 0, s, hz, hzt, p.T64, H);
+        hipLaunchKernelGGL(head_hzt_kernel, dim3(H / 64, p.T64 / 64), dim3(256), 0, s, hz, hzt, p.TP, H);
         ST_CHECK_LAUNCH();
     }
     for (int i = 0; i < p.pieces; ++i) {
@@ -983,7 +986,7 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
         const uint16_t* wp = w + (int64_t)v0 * ldw;
         if (p.few) {
             const int rc = launch_few<true>(T, kv, s, h, ldh, wp, ldw, T, kv, H, sc, (const int64_t*)nullptr, (float2*)nullptr, (float*)nullptr,
-                                            VhTargets{}, rows, v0, d, ldd, dt, p.T64);
+                                            VhTargets{}, rows, v0, d, ldd, dt, p.TP);
             if (rc) return rc;
         } else {
         hipLaunchKernelGGL((head_tile_kernel<true>), dim3(tm * tn), dim3(256), VH_SMEM, s, h, ldh, wp, ldw, T, kv, H, tm, tn, sc, (const int64_t*)nullptr,
@@ -1010,7 +1013,8 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
             if (p.few) {
                 const dim3 few_grid(st_cdiv(kv, 128));
 #define VH_DW_FEW(KS, OB, AC) hipLaunchKernelGGL((head_dw_few_kernel<KS, OB, AC>), few_grid, dim3(256), 0, s, dt, hzt, kv, H, ob, of, lddw)
-                if (p.T64 == 64) { if (dwb) VH_DW_FEW(2, true, false); else if (accumulate) VH_DW_FEW(2, false, true); else VH_DW_FEW(2, false, false); }
+                if (p.TP == 32) { if (dwb) VH_DW_FEW(1, true, false); else if (accumulate) VH_DW_FEW(1, false, true); else VH_DW_FEW(1, false, false); }
+                else if (p.TP == 64) { if (dwb) VH_DW_FEW(2, true, false); else if (accumulate) VH_DW_FEW(2, false, true); else VH_DW_FEW(2, false, false); }
                 else { if (dwb) VH_DW_FEW(4, true, false); else if (accumulate) VH_DW_FEW(4, false, true); else VH_DW_FEW(4, false, false); }
 #undef VH_DW_FEW
             }
@@ -1124,7 +1128,7 @@ int st_linear_topk_kl_bwd(const st_bf16* hidden, int64_t ldh, const st_bf16* wei
     return head_backward(hidden, ldh, weight, ldw, inv_temperature * VH_LOG2E, dhidden, lddh, dweight_bf16, dweight_f32, lddw, accumulate, ws, p, T, V, H, s,
                          [&](int v0, int kv, uint16_t* d, int64_t ldd, uint16_t* dt) -> int {
                              hipLaunchKernelGGL(head_sparse_kernel, dim3(st_cdiv(T, 4)), dim3(256), 0, s, ids, teacher_logp, K, renormalize, logq,
-                                                (const VhRow*)(ws + p.rows), v0, kv, d, ldd, dt, p.T64, T, V);
+                                                (const VhRow*)(ws + p.rows), v0, kv, d, ldd, dt, p.TP, T, V);
                              ST_CHECK_LAUNCH();
                              return 0;
                          });
