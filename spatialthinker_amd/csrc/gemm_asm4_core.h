@@ -41,6 +41,13 @@ template <int OFF> __device__ __forceinline__ void a4_read_tr(s16x4_t& f, uint32
 __device__ __forceinline__ void a4_dma0(uint32_t voff, i32x4 srd) {        // the K-tile offset sits in the resource's base address
     asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(srd) : "memory");
 }
+// the same two with the non-temporal policy: an operand that ONE workgroup reads, once
+__device__ __forceinline__ void a4_dma_nt(uint32_t voff, i32x4 srd, uint32_t soff) {
+    asm volatile("buffer_load_dwordx4 %0, %1, %2 offen nt lds" : : "v"(voff), "s"(srd), "s"(soff) : "memory");
+}
+__device__ __forceinline__ void a4_dma0_nt(uint32_t voff, i32x4 srd) {
+    asm volatile("buffer_load_dwordx4 %0, %1, 0 offen nt lds" : : "v"(voff), "s"(srd) : "memory");
+}
 __device__ __forceinline__ void a4_flip(uint32_t& addr) { asm volatile("v_xor_b32 %0, 0x10000, %0" : "+v"(addr)); }
 __device__ __forceinline__ void a4_m0_set(uint32_t v) { asm volatile("s_mov_b32 m0, %0" : : "s"(v) : "memory"); }
 __device__ __forceinline__ void a4_m0_next() { asm volatile("s_add_u32 m0, m0, 0x400" : : : "memory", "scc"); }
@@ -74,7 +81,8 @@ template <int N> __device__ __forceinline__ void a4_wait_vm() {
 // before the wait that stands there (an fp32 epilogue got the old value of the last accumulator in half of its lanes).  With GUARD the last MFMA
 // of every K-tile waits in its own statement: 1 % of the loop.  check_mfma_waits.py looks through the built code of every kernel and fails the
 // build where a result is touched too early; kernels that it names are built with GUARD, the others need not pay for it.
-template <bool AS, bool BS, bool SWIGLU, int DBG = 0, bool KCLAMP = false, bool GUARD = false>
+// BNT: B streams with the non-temporal policy (one row tile: no other workgroup reads its rows).
+template <bool AS, bool BS, bool SWIGLU, int DBG = 0, bool KCLAMP = false, bool GUARD = false, bool BNT = false>
 __device__ __forceinline__ void a4_mainloop(char* smem, const uint16_t* __restrict__ A, int64_t lda, const uint16_t* __restrict__ B, int64_t ldb, int m0,
                                             int n0, int M, int N, int kt0, int nk, int k_rows, f32x4 (&acc)[8][8]) {
     const int lane = threadIdx.x & 63;
@@ -208,7 +216,9 @@ __device__ __forceinline__ void a4_mainloop(char* smem, const uint16_t* __restri
     auto dma_tile = [&](auto jc) {                                   // copy j of the NEXT issue (voff already points at its K-tile)
         constexpr int j = decltype(jc)::value;
         if constexpr (j < 8) { if constexpr (AS) a4_dma0(voffA[j], srdA); else a4_dma(voffA[j], srdA, koff); }
+        else if constexpr (BS && BNT) a4_dma0_nt(voffB[j - 8], srdB);
         else if constexpr (BS) a4_dma0(voffB[j - 8], srdB);
+        else if constexpr (BNT) a4_dma_nt(voffB[j - 8], srdB, koff);
         else if (SWIGLU && (((wave * 64 + (j - 8) * 8) >> 4) & 1)) a4_dma(voffB[j - 8], srdB2, koff);
         else a4_dma(voffB[j - 8], srdB, koff);
     };

@@ -66,7 +66,7 @@ __device__ __forceinline__ void vh_store_image(const char* smem, uint16_t* __res
 // has exactly the maximum's value.
 // DLOGITS: d[m][n] (bf16, pitch ldd, zero in columns [V, ldd) and rows [T, T64)).
 // ------------------------------------------------------------------------------------------------------------------------------------
-template <bool DLOGITS>
+template <bool DLOGITS, bool ONE_ROW_TILE>
 __global__ __launch_bounds__(256) void head_tile_kernel(const uint16_t* __restrict__ h, int64_t ldh, const uint16_t* __restrict__ w, int64_t ldw, int T,
                                                        int V, int H, int tiles_m, int tiles_n, float sc, const int64_t* __restrict__ labels,
                                                        float2* __restrict__ part, float* __restrict__ zlab, VhTargets tg, const VhRow* __restrict__ rows, int v0,
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256) void head_tile_kernel(const uint16_t* __restri
     vh_tile(blockIdx.x, tiles_m, tiles_n, tm, tn);
     const int m0 = tm * A4_BM, n0 = tn * A4_BN;
     f32x4 acc[8][8];
-    a4_mainloop<false, false, false>(smem, h, ldh, w, ldw, m0, n0, T, V, 0, H / 64, H, acc);
+    a4_mainloop<false, false, false, 0, false, false, ONE_ROW_TILE>(smem, h, ldh, w, ldw, m0, n0, T, V, 0, H / 64, H, acc);
     const int col0 = n0 + wn * 128 + (lane >> 4) * 4;                // column of (ni, r): col0 + ni*16 + r
     const bool inside = n0 + A4_BN <= V;
     if constexpr (!DLOGITS) {
@@ -423,7 +423,7 @@ __global__ __launch_bounds__(128) void head_rows_label_kernel(const uint16_t* __
 }
 
 // slab[s][m][n] (+)= sum over the K-slice s of d[m][:] w[:][n]: w is contraction-major as stored; `kv` of the ldd columns of d are vocabulary
-template <bool ACCUM>
+template <bool ACCUM, bool ONE_ROW_TILE>
 __global__ __launch_bounds__(256) void head_dh_kernel(const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ w, int64_t ldw, int T,
                                                      int kv, int H, int tiles_m, int tiles_n, int split, float* __restrict__ slab) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -437,7 +437,7 @@ __global__ __launch_bounds__(256) void head_dh_kernel(const uint16_t* __restrict
     const int nkt = (kv + 63) / 64, per = (nkt + split - 1) / split, kt0 = slice * per;
     const int nk = min(nkt - kt0, per);                              // >= 1: the host gives no slice without K-tiles
     f32x4 acc[8][8];
-    a4_mainloop<false, true, false, 0, true>(smem, d, ldd, w, ldw, m0, n0, T, H, kt0, nk, kv, acc);
+    a4_mainloop<false, true, false, 0, true, false, ONE_ROW_TILE>(smem, d, ldd, w, ldw, m0, n0, T, H, kt0, nk, kv, acc);
     float* out = slab + (int64_t)slice * T * H;
 #pragma unroll
     for (int mi = 0; mi < 8; ++mi) {
@@ -671,6 +671,112 @@ __global__ __launch_bounds__(256) void head_dw_few_kernel(const uint16_t* __rest
                     __builtin_nontemporal_store(*reinterpret_cast<const f32x4*>(img + row * VH_ROWB + col * 2), reinterpret_cast<f32x4*>(dwb + (int64_t)(r0 + row) * lddw + c0 + col));
             }
             __syncthreads();
+        }
+    }
+}
+
+// dw for 129 .. 256 rows (T64 = 32 KS): as above the write of dw next to few products per value, but the operands are too long to come straight from
+// the caches for every wave.  A workgroup owns 256 vocabulary rows, 64 per wave, whose d stays in registers for the whole walk; the hidden states
+// come 64 columns at a time, [T64][64], through LDS for all four waves.  Both are contraction-major as they lie in memory, so fragments are LDS
+// transpose reads: image of 128-byte rows, 32-byte chunk c of row r at position c ^ f(r), f(r) = ((r >> 1) & 1) | ((r >> 3) & 1) << 1, which
+// gives the eight rows that a half wave touches eight places of the 256-byte bank row.  Two workgroups per CU: one stores while the other multiplies.
+__device__ __forceinline__ void vh_tr_frag4(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, bf16x8 (&f)[4]) {
+    union Frag { bf16x8 v; s16x4_t h[2]; } x[4];
+    // reads and their wait in one statement; rows +4 .. +7 of a fragment lie 512 bytes on
+    asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:512\n\tds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:512\n\t"
+                 "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:512\n\tds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:512\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0].h[0]), "=&v"(x[0].h[1]), "=&v"(x[1].h[0]), "=&v"(x[1].h[1]), "=&v"(x[2].h[0]), "=&v"(x[2].h[1]), "=&v"(x[3].h[0]), "=&v"(x[3].h[1])
+                 : "v"(a0), "v"(a1), "v"(a2), "v"(a3)
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = x[i].v;
+}
+
+template <int KS, bool OUT_BF16, bool ACCUM>
+__global__ __launch_bounds__(256, OUT_BF16 ? 2 : 1) void head_dw_mid_kernel(const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ hz, int kv, int H,
+                                                            uint16_t* __restrict__ dwb, float* __restrict__ dwf, int64_t lddw) {
+    constexpr int T64 = KS * 32, TB = T64 * 128, RB = 64 * 2 + 16;       // TB: bytes of a [T64][64] image; RB: row of the output image
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63, fr = lane & 15, fk = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r0 = blockIdx.x * 256;
+    // copy of 8 image rows: lane -> row (lane >> 3), 16-byte piece lane & 7: half (lane & 1) of the chunk at position (lane & 7) >> 1
+    const int cr = lane >> 3;
+    auto col_of = [&](int row) { return (((((lane & 7) >> 1) ^ (((row >> 1) & 1) | (((row >> 3) & 1) << 1))) << 4) | ((lane & 1) << 3)); };
+    uint32_t tr[4];                                                  // fragment address of 16-column chunk i, k-rows fk*8 ..
+    {
+        const int row = fk * 8 + (fr >> 2), f = ((row >> 1) & 1) | (((row >> 3) & 1) << 1);
+        // rows +4 .. +7 keep f: bits 1 and 3 of the row do not change below a multiple of 8 but for bit 2
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tr[i] = (uint32_t)(uintptr_t)smem + row * 128 + ((i ^ f) << 5) + (lane & 3) * 8;
+    }
+    bf16x8 df[KS][4];
+    for (int wv = 0; wv < 4; ++wv) {                                 // d of each wave's 64 vocabulary rows in turn through the image
+        if (wv) __syncthreads();
+        for (int j = wave; j < T64 / 8; j += 4) {
+            const int row = j * 8 + cr;
+            st_glds16(d + (int64_t)row * ldd + min(r0 + wv * 64 + col_of(row), (int)ldd - 8), smem + j * 1024);
+        }
+        vh_wait_vm<0>();
+        __syncthreads();
+        if (wv == wave)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) vh_tr_frag4(tr[0] + s * 4096, tr[1] + s * 4096, tr[2] + s * 4096, tr[3] + s * 4096, df[s]);
+    }
+    char* img = smem + TB;
+    for (int c0 = 0; c0 < H; c0 += 64) {
+        __syncthreads();                                             // every wave has read the image (and stored its part of the output)
+        for (int j = wave; j < T64 / 8; j += 4) {
+            const int row = j * 8 + cr;
+            st_glds16(hz + (int64_t)row * H + c0 + col_of(row), smem + j * 1024);
+        }
+        vh_wait_vm<0>();
+        __syncthreads();
+        f32x4 acc[4][4];                                             // [vocabulary tile][column tile]
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            bf16x8 hf[4];
+            vh_tr_frag4(tr[0] + s * 4096, tr[1] + s * 4096, tr[2] + s * 4096, tr[3] + s * 4096, hf);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hf[j], df[s][i], acc[i][j], 0, 0, 0);
+        }
+        if constexpr (OUT_BF16) {                                    // a wave's 64 x 64 tile through its own part of the output image
+            char* my = img + wave * 64 * RB;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint2 pk;
+                    pk.x = f2bf2(acc[i][j][0], acc[i][j][1]); pk.y = f2bf2(acc[i][j][2], acc[i][j][3]);
+                    *reinterpret_cast<uint2*>(my + (i * 16 + fr) * RB + (j * 16 + fk * 4) * 2) = pk;
+                }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int row = k * 8 + cr, v = r0 + wave * 64 + row;
+                const f32x4 o = *reinterpret_cast<const f32x4*>(my + row * RB + (lane & 7) * 16);
+                if (v < kv) __builtin_nontemporal_store(o, reinterpret_cast<f32x4*>(dwb + (int64_t)v * lddw + c0 + (lane & 7) * 8));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int v = r0 + wave * 64 + i * 16 + fr;
+                if (v >= kv) continue;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float4* q = reinterpret_cast<float4*>(dwf + (int64_t)v * lddw + c0 + j * 16 + fk * 4);
+                    float4 o = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+                    if constexpr (ACCUM) { const float4 b = *q; o.x += b.x; o.y += b.y; o.z += b.z; o.w += b.w; }
+                    *q = o;
+                }
+            }
         }
     }
 }
@@ -934,10 +1040,13 @@ int head_stats(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, c
                                          (int64_t)0, (uint16_t*)nullptr, 0);
         if (rc) return rc;
     } else {
-    allow_lds<head_tile_kernel<false>>();
-    hipLaunchKernelGGL((head_tile_kernel<false>), dim3(tm * tn), dim3(256), VH_SMEM, s, h, ldh, w, ldw, T, V, H, tm, tn, sc, labels, part, zlab, tg,
-                       (const VhRow*)nullptr, 0, (uint16_t*)nullptr, (int64_t)0, 0);
-    ST_CHECK_LAUNCH();
+        auto go = [&](auto kern) {
+            hipLaunchKernelGGL(kern, dim3(tm * tn), dim3(256), VH_SMEM, s, h, ldh, w, ldw, T, V, H, tm, tn, sc, labels, part, zlab, tg,
+                               (const VhRow*)nullptr, 0, (uint16_t*)nullptr, (int64_t)0, 0);
+        };
+        allow_lds<head_tile_kernel<false, true>>(); allow_lds<head_tile_kernel<false, false>>();
+        if (tm == 1) go(head_tile_kernel<false, true>); else go(head_tile_kernel<false, false>);
+        ST_CHECK_LAUNCH();
     }
     hipLaunchKernelGGL(head_lse_kernel, dim3(st_cdiv(T, 16)), dim3(1024), 0, s, part, n_parts, zlab, labels, logp, lse, (float2*)(ws + p.stat), T, V);
     ST_CHECK_LAUNCH();
@@ -973,8 +1082,8 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
     uint16_t* hzt = (uint16_t*)(ws + p.hzt);
     float* slab = (float*)(ws + p.slab);
     const int tm = st_cdiv(T, 256), th = st_cdiv(H, 256);
-    allow_lds<head_tile_kernel<true>>();
-    allow_lds<head_dh_kernel<false>>(); allow_lds<head_dh_kernel<true>>();
+    allow_lds<head_tile_kernel<true, true>>(); allow_lds<head_tile_kernel<true, false>>();
+    allow_lds<head_dh_kernel<false, true>>(); allow_lds<head_dh_kernel<true, true>>(); allow_lds<head_dh_kernel<false, false>>(); allow_lds<head_dh_kernel<true, false>>();
     allow_lds<head_dw_kernel<true, false>>(); allow_lds<head_dw_kernel<false, false>>(); allow_lds<head_dw_kernel<false, true>>();
     if (p.few && (dwb || dwf)) {
         hipLaunchKernelGGL(head_hzt_kernel, dim3(H / 64, p.T64 / 64), dim3(256), 0, s, hz, hzt, p.TP, H);
@@ -989,9 +1098,12 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
                                             VhTargets{}, rows, v0, d, ldd, dt, p.TP);
             if (rc) return rc;
         } else {
-        hipLaunchKernelGGL((head_tile_kernel<true>), dim3(tm * tn), dim3(256), VH_SMEM, s, h, ldh, wp, ldw, T, kv, H, tm, tn, sc, (const int64_t*)nullptr,
-                           (float2*)nullptr, (float*)nullptr, VhTargets{}, rows, v0, d, ldd, p.T64);
-        ST_CHECK_LAUNCH();
+            auto go = [&](auto kern) {
+                hipLaunchKernelGGL(kern, dim3(tm * tn), dim3(256), VH_SMEM, s, h, ldh, wp, ldw, T, kv, H, tm, tn, sc, (const int64_t*)nullptr,
+                                   (float2*)nullptr, (float*)nullptr, VhTargets{}, rows, v0, d, ldd, p.T64);
+            };
+            if (tm == 1) go(head_tile_kernel<true, true>); else go(head_tile_kernel<true, false>);
+            ST_CHECK_LAUNCH();
         }
         const int rc = sparse(v0, kv, d, ldd, dt);
         if (rc) return rc;
@@ -1001,8 +1113,9 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
         } else if (dh) {
             const int nkt = st_cdiv(kv, 64), per = st_cdiv(nkt, p.split), slices = st_cdiv(nkt, per);      // (a short last piece may fill fewer slices)
             const dim3 grid(tm * th * slices);
-            if (i == 0) hipLaunchKernelGGL((head_dh_kernel<false>), grid, dim3(256), VH_SMEM, s, d, ldd, wp, ldw, T, kv, H, tm, th, p.split, slab);
-            else hipLaunchKernelGGL((head_dh_kernel<true>), grid, dim3(256), VH_SMEM, s, d, ldd, wp, ldw, T, kv, H, tm, th, p.split, slab);
+            auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), VH_SMEM, s, d, ldd, wp, ldw, T, kv, H, tm, th, p.split, slab); };
+            if (tm == 1) { if (i == 0) go(head_dh_kernel<false, true>); else go(head_dh_kernel<true, true>); }
+            else { if (i == 0) go(head_dh_kernel<false, false>); else go(head_dh_kernel<true, false>); }
             ST_CHECK_LAUNCH();
         }
         if (dwb || dwf) {
@@ -1017,6 +1130,14 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
                 else if (p.TP == 64) { if (dwb) VH_DW_FEW(2, true, false); else if (accumulate) VH_DW_FEW(2, false, true); else VH_DW_FEW(2, false, false); }
                 else { if (dwb) VH_DW_FEW(4, true, false); else if (accumulate) VH_DW_FEW(4, false, true); else VH_DW_FEW(4, false, false); }
 #undef VH_DW_FEW
+            }
+            else if (p.T64 <= 256 && 2 * tv >= st_num_cus()) {           // (fewer row blocks than half the CUs: the square tile spreads better)
+                const int smem = p.T64 * 128 + 4 * 64 * 144;
+#define VH_DW_MID(KS, OB, AC) do { allow_lds<head_dw_mid_kernel<KS, OB, AC>>(smem); \
+        hipLaunchKernelGGL((head_dw_mid_kernel<KS, OB, AC>), dim3(tv), dim3(256), smem, s, d, ldd, hz, kv, H, ob, of, lddw); } while (0)
+                if (p.T64 == 192) { if (dwb) VH_DW_MID(6, true, false); else if (accumulate) VH_DW_MID(6, false, true); else VH_DW_MID(6, false, false); }
+                else { if (dwb) VH_DW_MID(8, true, false); else if (accumulate) VH_DW_MID(8, false, true); else VH_DW_MID(8, false, false); }
+#undef VH_DW_MID
             }
             else if (dwb) hipLaunchKernelGGL((head_dw_kernel<true, false>), grid, dim3(256), VH_SMEM, s, d, ldd, hz, p.T64, kv, H, tv, th, ob, of, lddw);
             else if (accumulate) hipLaunchKernelGGL((head_dw_kernel<false, true>), grid, dim3(256), VH_SMEM, s, d, ldd, hz, p.T64, kv, H, tv, th, ob, of, lddw);

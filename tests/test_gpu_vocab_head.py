@@ -109,7 +109,7 @@ def test_more_than_one_piece_of_the_vocabulary():
     check_grads(h, w, d, derr, dh, dw, UB)
 
 
-@pytest.mark.parametrize("T", [20, 100, 190])
+@pytest.mark.parametrize("T", [20, 100, 190, 250, 300])
 @pytest.mark.parametrize("accumulate", [False, True])
 def test_fp32_weight_gradient_and_single_gradients(T, accumulate):
     from spatialthinker_amd import ops
