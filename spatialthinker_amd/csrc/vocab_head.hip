@@ -380,6 +380,38 @@ __global__ __launch_bounds__(1024) void head_lse_kernel(const float2* __restrict
     }
 }
 
+// the same for few rows, where reading the partials one behind the other is what takes the time: a workgroup per row
+__global__ __launch_bounds__(1024) void head_lse_few_kernel(const float2* __restrict__ part, int n_parts, const float* __restrict__ zlab,
+                                                           const int64_t* __restrict__ labels, float* __restrict__ logp, float* __restrict__ lse,
+                                                           float2* __restrict__ stat, int T, int V) {
+    __shared__ float2 red[16];
+    const int row = blockIdx.x, lane = threadIdx.x & 63;
+    float2 a = make_float2(-INFINITY, 0.f);
+    auto join = [](float2 x, float2 y) {
+        const float m = fmaxf(x.x, y.x);
+        return make_float2(m, m != -INFINITY ? x.y * vh_exp2(x.x - m) + y.y * vh_exp2(y.x - m) : x.y + y.y);
+    };
+    for (int p = threadIdx.x; p < n_parts; p += 1024) a = join(a, part[(int64_t)p * T + row]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) a = join(a, make_float2(__shfl_xor(a.x, o, 64), __shfl_xor(a.y, o, 64)));
+    if (lane == 0) red[threadIdx.x >> 6] = a;
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        a = red[lane & 15];
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) a = join(a, make_float2(__shfl_xor(a.x, o, 64), __shfl_xor(a.y, o, 64)));
+        if (lane == 0) {
+            const float ls = log2f(a.y);
+            lse[row] = (a.x + ls) * VH_LN2;
+            if (stat) stat[row] = make_float2(a.x, ls);
+            if (labels) {
+                const int64_t lab = labels[row];
+                logp[row] = lab >= 0 && lab < V ? ((zlab[row] - a.x) - ls) * VH_LN2 : 0.f;
+            }
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------------------------------------
 // Backward: row coefficients and the packed hidden states.  A row of d is held as scale_t * d', with d' in the workspace and the scale in
 // hz[t][:] = bf16(scale_t h[t][:]) (for dW) and in the finish of dh.  Where one target dominates a row the scale is that target's gradient: its d' is
@@ -424,15 +456,14 @@ __global__ __launch_bounds__(128) void head_rows_label_kernel(const uint16_t* __
 
 // slab[s][m][n] (+)= sum over the K-slice s of d[m][:] w[:][n]: w is contraction-major as stored; `kv` of the ldd columns of d are vocabulary
 template <bool ACCUM, bool ONE_ROW_TILE>
-__global__ __launch_bounds__(256) void head_dh_kernel(const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ w, int64_t ldw, int T,
-                                                     int kv, int H, int tiles_m, int tiles_n, int split, float* __restrict__ slab) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+__device__ __forceinline__ void head_dh_tile(char* smem, int block, const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ w, int64_t ldw,
+                                             int T, int kv, int H, int tiles_m, int tiles_n, int split, float* __restrict__ slab) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1;
-    const int nb = tiles_m * tiles_n, slice = blockIdx.x / nb;
+    const int nb = tiles_m * tiles_n, slice = block / nb;
     int tm, tn;
-    vh_tile(blockIdx.x % nb, tiles_m, tiles_n, tm, tn);
+    vh_tile(block % nb, tiles_m, tiles_n, tm, tn);
     const int m0 = tm * A4_BM, n0 = tn * A4_BN;
     const int nkt = (kv + 63) / 64, per = (nkt + split - 1) / split, kt0 = slice * per;
     const int nk = min(nkt - kt0, per);                              // >= 1: the host gives no slice without K-tiles
@@ -453,6 +484,13 @@ __global__ __launch_bounds__(256) void head_dh_kernel(const uint16_t* __restrict
             *p = o;
         }
     }
+}
+
+template <bool ACCUM, bool ONE_ROW_TILE>
+__global__ __launch_bounds__(256) void head_dh_kernel(const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ w, int64_t ldw, int T,
+                                                     int kv, int H, int tiles_m, int tiles_n, int split, float* __restrict__ slab) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    head_dh_tile<ACCUM, ONE_ROW_TILE>(smem, blockIdx.x, d, ldd, w, ldw, T, kv, H, tiles_m, tiles_n, split, slab);
 }
 
 // The same for few rows (T <= 128): a stream of w, [32 vocabulary rows][256 columns] per step through SLOTS LDS slots, next to a [16 MT][32] tile of d
@@ -566,14 +604,13 @@ __global__ __launch_bounds__(256) void head_dh_finish_kernel(const float* __rest
 
 // dw[v][n] = sum_t d[t][v] hz[t][n]: both operands contraction-major as they lie in memory.  bf16 result, or fp32 (+=).
 template <bool OUT_BF16, bool ACCUM>
-__global__ __launch_bounds__(256) void head_dw_kernel(const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ hz, int T64, int kv, int H,
-                                                     int tiles_m, int tiles_n, uint16_t* __restrict__ dwb, float* __restrict__ dwf, int64_t lddw) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+__device__ __forceinline__ void head_dw_tile(char* smem, int block, const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ hz, int T64,
+                                             int kv, int H, int tiles_m, int tiles_n, uint16_t* __restrict__ dwb, float* __restrict__ dwf, int64_t lddw) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1;
     int tm, tn;
-    vh_tile(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    vh_tile(block, tiles_m, tiles_n, tm, tn);
     const int m0 = tm * A4_BM, n0 = tn * A4_BN;
     f32x4 acc[8][8];
     a4_mainloop<true, true, false, 0, false, !OUT_BF16>(smem, d, ldd, hz, H, m0, n0, (int)ldd, H, 0, T64 / 64, T64, acc);
@@ -607,6 +644,25 @@ __global__ __launch_bounds__(256) void head_dw_kernel(const uint16_t* __restrict
             }
         }
     }
+}
+
+template <bool OUT_BF16, bool ACCUM>
+__global__ __launch_bounds__(256) void head_dw_kernel(const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ hz, int T64, int kv, int H,
+                                                     int tiles_m, int tiles_n, uint16_t* __restrict__ dwb, float* __restrict__ dwf, int64_t lddw) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    head_dw_tile<OUT_BF16, ACCUM>(smem, blockIdx.x, d, ldd, hz, T64, kv, H, tiles_m, tiles_n, dwb, dwf, lddw);
+}
+
+// Both gradients of a piece in one launch: the few long tiles of dh first, the many short ones of dw behind them fill the CUs up, where two launches
+// would each leave part of their last round idle (8192 x 3584, a piece of 30 464 columns: 448 and 1666 tiles on 256 CUs).
+template <bool DW_BF16, bool DW_ACCUM, bool DH_ACCUM>
+__global__ __launch_bounds__(256) void head_grads_kernel(const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ w, int64_t ldw,
+                                                        const uint16_t* __restrict__ hz, int T, int T64, int kv, int H, int tiles_t, int tiles_v, int tiles_h,
+                                                        int split, int dh_blocks, float* __restrict__ slab, uint16_t* __restrict__ dwb,
+                                                        float* __restrict__ dwf, int64_t lddw) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    if ((int)blockIdx.x < dh_blocks) head_dh_tile<DH_ACCUM, false>(smem, blockIdx.x, d, ldd, w, ldw, T, kv, H, tiles_t, tiles_h, split, slab);
+    else head_dw_tile<DW_BF16, DW_ACCUM>(smem, blockIdx.x - dh_blocks, d, ldd, hz, T64, kv, H, tiles_v, tiles_h, dwb, dwf, lddw);
 }
 
 // dw for few rows (TP = 32 KS, T rounded up to 32, 64 or 128): the launch is the write of dw, V H elements, next to 2 KS products of 32 rows each.  Operands stand contraction-
@@ -951,7 +1007,7 @@ __global__ __launch_bounds__(256) void head_zero_kernel(char* __restrict__ p, in
 // ------------------------------------------------------------------------------------------------------------------------------------
 namespace {
 struct Plan {                                                        // workspace layout (byte offsets) and piece / slice counts of one call
-    int T64, TP, pieces, piece, split;                               // TP: row pitch of the transposed operands of head_dw_few_kernel
+    int T64, TP, pieces, piece, split, split_both;                               // TP: row pitch of the transposed operands of head_dw_few_kernel
     int64_t part, zlab, stat, start, list, fwd_bytes;
     int64_t rows, scale, hz, hzt, d, dt, slab, bwd_bytes;
     bool few;                                                        // the weight-streaming kernels
@@ -985,6 +1041,14 @@ Plan head_plan(int T, int V, int H, int K) {                         // K: targe
         const int64_t cost = (int64_t)st_cdiv((int64_t)tiles * s, ncu) * (st_cdiv(nkt, s) + 14) + 2 * s;
         if (cost < best) { best = cost; p.split = s; }
     }
+    // beside dw in one launch: no slice longer than half of what a CU has to do (~8 and ~14 K-steps for the rest of a dw and a dh tile)
+    p.split_both = 1;
+    if (!p.few) {
+        const int64_t dw_steps = (int64_t)st_cdiv(std::min(V, p.piece), 256) * st_cdiv(H, 256) * (p.T64 / 64 + 8);
+        while (p.split_both < 32 && nkt / (p.split_both + 1) >= 8 &&
+               2 * (int64_t)(st_cdiv(nkt, p.split_both) + 14) * ncu > (int64_t)tiles * (nkt + 14 * p.split_both) + dw_steps)
+            ++p.split_both;
+    }
     p.rows = 0;
     p.scale = up((int64_t)T * (int64_t)sizeof(VhRow), 256);
     p.hz = p.scale + up((int64_t)T * 4, 256);
@@ -992,7 +1056,7 @@ Plan head_plan(int T, int V, int H, int K) {                         // K: targe
     p.d = p.hzt + (p.few ? up((int64_t)p.T64 * H * 2, 256) : 0);
     p.dt = p.d + up((int64_t)p.T64 * p.piece * 2, 256);
     p.slab = p.dt + (p.few ? up((int64_t)p.T64 * p.piece * 2, 256) : 0);
-    p.bwd_bytes = p.slab + up((int64_t)p.split * T * H * 4, 256);
+    p.bwd_bytes = p.slab + up((int64_t)std::max(p.split, p.split_both) * T * H * 4, 256);
     return p;
 }
 
@@ -1048,7 +1112,8 @@ int head_stats(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, c
         if (tm == 1) go(head_tile_kernel<false, true>); else go(head_tile_kernel<false, false>);
         ST_CHECK_LAUNCH();
     }
-    hipLaunchKernelGGL(head_lse_kernel, dim3(st_cdiv(T, 16)), dim3(1024), 0, s, part, n_parts, zlab, labels, logp, lse, (float2*)(ws + p.stat), T, V);
+    if (T <= 512) hipLaunchKernelGGL(head_lse_few_kernel, dim3(T), dim3(1024), 0, s, part, n_parts, zlab, labels, logp, lse, (float2*)(ws + p.stat), T, V);
+    else hipLaunchKernelGGL(head_lse_kernel, dim3(st_cdiv(T, 16)), dim3(1024), 0, s, part, n_parts, zlab, labels, logp, lse, (float2*)(ws + p.stat), T, V);
     ST_CHECK_LAUNCH();
     return 0;
 }
@@ -1082,6 +1147,12 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
     uint16_t* hzt = (uint16_t*)(ws + p.hzt);
     float* slab = (float*)(ws + p.slab);
     const int tm = st_cdiv(T, 256), th = st_cdiv(H, 256);
+    const bool mid = !p.few && p.T64 <= 256 && 2 * st_cdiv(p.piece, 256) >= st_num_cus();        // (fewer row blocks: the square tile spreads better)
+    const bool both = dh && (dwb || dwf) && !p.few && !mid;
+    const int split = both ? p.split_both : p.split;
+    allow_lds<head_grads_kernel<true, false, false>>(); allow_lds<head_grads_kernel<true, false, true>>();
+    allow_lds<head_grads_kernel<false, false, false>>(); allow_lds<head_grads_kernel<false, false, true>>();
+    allow_lds<head_grads_kernel<false, true, false>>(); allow_lds<head_grads_kernel<false, true, true>>();
     allow_lds<head_tile_kernel<true, true>>(); allow_lds<head_tile_kernel<true, false>>();
     allow_lds<head_dh_kernel<false, true>>(); allow_lds<head_dh_kernel<true, true>>(); allow_lds<head_dh_kernel<false, false>>(); allow_lds<head_dh_kernel<true, false>>();
     allow_lds<head_dw_kernel<true, false>>(); allow_lds<head_dw_kernel<false, false>>(); allow_lds<head_dw_kernel<false, true>>();
@@ -1107,22 +1178,33 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
         }
         const int rc = sparse(v0, kv, d, ldd, dt);
         if (rc) return rc;
+        const int tv = st_cdiv(kv, 256), nkt = st_cdiv(kv, 64), slices = st_cdiv(nkt, st_cdiv(nkt, split));      // (a short last piece may fill fewer slices)
+        uint16_t* ob = dwb ? dwb + (int64_t)v0 * lddw : nullptr;
+        float* of = dwf ? dwf + (int64_t)v0 * lddw : nullptr;
+        if (both) {
+            const int dh_blocks = tm * th * slices;
+            const dim3 grid(dh_blocks + tv * th);
+            auto go = [&](auto kern) {
+                hipLaunchKernelGGL(kern, grid, dim3(256), VH_SMEM, s, d, ldd, wp, ldw, hz, T, p.T64, kv, H, tm, tv, th, split, dh_blocks, slab, ob, of, lddw);
+            };
+            if (dwb) { if (i == 0) go(head_grads_kernel<true, false, false>); else go(head_grads_kernel<true, false, true>); }
+            else if (accumulate) { if (i == 0) go(head_grads_kernel<false, true, false>); else go(head_grads_kernel<false, true, true>); }
+            else { if (i == 0) go(head_grads_kernel<false, false, false>); else go(head_grads_kernel<false, false, true>); }
+            ST_CHECK_LAUNCH();
+            continue;
+        }
         if (dh && p.few) {
             const int rc = launch_dh_few(d, ldd, wp, ldw, T, kv, H, th, p, i > 0, slab, s);
             if (rc) return rc;
         } else if (dh) {
-            const int nkt = st_cdiv(kv, 64), per = st_cdiv(nkt, p.split), slices = st_cdiv(nkt, per);      // (a short last piece may fill fewer slices)
             const dim3 grid(tm * th * slices);
-            auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), VH_SMEM, s, d, ldd, wp, ldw, T, kv, H, tm, th, p.split, slab); };
+            auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), VH_SMEM, s, d, ldd, wp, ldw, T, kv, H, tm, th, split, slab); };
             if (tm == 1) { if (i == 0) go(head_dh_kernel<false, true>); else go(head_dh_kernel<true, true>); }
             else { if (i == 0) go(head_dh_kernel<false, false>); else go(head_dh_kernel<true, false>); }
             ST_CHECK_LAUNCH();
         }
         if (dwb || dwf) {
-            const int tv = st_cdiv(kv, 256);
             const dim3 grid(tv * th);
-            uint16_t* ob = dwb ? dwb + (int64_t)v0 * lddw : nullptr;
-            float* of = dwf ? dwf + (int64_t)v0 * lddw : nullptr;
             if (p.few) {
                 const dim3 few_grid(st_cdiv(kv, 128));
 #define VH_DW_FEW(KS, OB, AC) hipLaunchKernelGGL((head_dw_few_kernel<KS, OB, AC>), few_grid, dim3(256), 0, s, dt, hzt, kv, H, ob, of, lddw)
@@ -1131,7 +1213,7 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
                 else { if (dwb) VH_DW_FEW(4, true, false); else if (accumulate) VH_DW_FEW(4, false, true); else VH_DW_FEW(4, false, false); }
 #undef VH_DW_FEW
             }
-            else if (p.T64 <= 256 && 2 * tv >= st_num_cus()) {           // (fewer row blocks than half the CUs: the square tile spreads better)
+            else if (mid) {
                 const int smem = p.T64 * 128 + 4 * 64 * 144;
 #define VH_DW_MID(KS, OB, AC) do { allow_lds<head_dw_mid_kernel<KS, OB, AC>>(smem); \
         hipLaunchKernelGGL((head_dw_mid_kernel<KS, OB, AC>), dim3(tv), dim3(256), smem, s, d, ldd, hz, kv, H, ob, of, lddw); } while (0)
@@ -1146,7 +1228,7 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
         }
     }
     if (dh) {
-        const int nkt = st_cdiv(std::min(V, p.piece), p.few ? 32 : 64), slices = st_cdiv(nkt, st_cdiv(nkt, p.split));
+        const int nkt = st_cdiv(std::min(V, p.piece), p.few ? 32 : 64), slices = st_cdiv(nkt, st_cdiv(nkt, split));
         hipLaunchKernelGGL(head_dh_finish_kernel, dim3(st_cdiv((int64_t)T * H, 1024)), dim3(256), 0, s, slab, slices, (const float*)(ws + p.scale), dh, lddh, T, H);
         ST_CHECK_LAUNCH();
     }
