@@ -387,13 +387,14 @@ __global__ __launch_bounds__(NT) void topk_join_kernel(const uint64_t* __restric
 }
 
 // Threads per workgroup: one maximum per thread bounds the k-th largest value from below, so k is at most about half of them (with k = NT the
-// bound is the least of the maxima); otherwise the smaller workgroup, of which more run side by side.
-static int topk_threads(int k) { return k <= 96 ? 256 : 512; }
+// bound is the least of the maxima); otherwise the smaller workgroup, of which more run side by side (MI355X, V = 152 064, 256 / 512 threads:
+// 2048 rows, k = 128 174 / 192 us; 256 rows, k = 128 56 / 46 us).
+static int topk_threads(int T, int k) { return k <= 96 || (k <= 128 && T >= 4 * st_num_cus()) ? 256 : 512; }
 
 // Slices of a row: whole rounds of the workgroups that fit (1024 threads per CU), each costing its slice plus about 32 K values' time of threshold,
 // ranking and launch; a slice keeps at least a load per thread, the slices' keys fit the join's list.
 static int topk_slices(int T, int V, int k) {
-    const int nt = topk_threads(k), slots = 1024 / nt * st_num_cus(), most = std::max(1, std::min({TK_CAP(512) / k, st_cdiv(V, TK_CHUNK(nt)), 64}));
+    const int nt = topk_threads(T, k), slots = 1024 / nt * st_num_cus(), most = std::max(1, std::min({TK_CAP(512) / k, st_cdiv(V, TK_CHUNK(nt)), 64}));
     int best = 1;
     int64_t cost = INT64_MAX;
     for (int s = 1; s <= most; ++s) {
@@ -433,7 +434,7 @@ int st_topk_logprob(const st_bf16* logits, int64_t ldl, int k, float inv_tempera
                                logp + (int64_t)t0 * k, lse + t0, slices > 1 ? keys + (int64_t)t0 * used * k : nullptr,
                                slices > 1 ? stats + (int64_t)t0 * used : nullptr);
         };
-        if (topk_threads(k) == 256) go(topk_row_kernel<256>, 256); else go(topk_row_kernel<512>, 512);
+        if (topk_threads(T, k) == 256) go(topk_row_kernel<256>, 256); else go(topk_row_kernel<512>, 512);
         ST_CHECK_LAUNCH();
     }
     if (used > 1) {

@@ -419,24 +419,31 @@ __global__ __launch_bounds__(1024) void head_lse_few_kernel(const float2* __rest
 // hz is 0 for rows without a gradient and for the padding rows [T, T64): what such rows of h hold (also infinities and NaN) cannot reach dW
 // through 0 * x.
 // ------------------------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void vh_pack_row(const uint16_t* __restrict__ h, int64_t ldh, uint16_t* __restrict__ hz, int t, bool live, float scale, int H) {
+// Either of hz and hzt (transposed, row pitch TP: the few-row kernels) is written.
+__device__ __forceinline__ void vh_pack_row(const uint16_t* __restrict__ h, int64_t ldh, uint16_t* __restrict__ hz, uint16_t* __restrict__ hzt, int TP, int t,
+                                            bool live, float scale, int H) {
     for (int i = threadIdx.x * 8; i < H; i += blockDim.x * 8) {
-        uint4 o = make_uint4(0, 0, 0, 0);
+        union { uint4 v; uint16_t e[8]; } o;
+        o.v = make_uint4(0, 0, 0, 0);
         if (live) {
             float f[8];
             unpack8(*reinterpret_cast<const uint4*>(h + (int64_t)t * ldh + i), f);
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] *= scale;
-            o = pack8(f);
+            o.v = pack8(f);
         }
-        *reinterpret_cast<uint4*>(hz + (int64_t)t * H + i) = o;
+        if (hz) *reinterpret_cast<uint4*>(hz + (int64_t)t * H + i) = o.v;
+        else
+#pragma unroll
+            for (int j = 0; j < 8; ++j) hzt[(int64_t)(i + j) * TP + t] = o.e[j];
     }
 }
 
 __global__ __launch_bounds__(128) void head_rows_label_kernel(const uint16_t* __restrict__ h, int64_t ldh, const int64_t* __restrict__ labels,
                                                              const float* __restrict__ logp, const float* __restrict__ lse,
                                                              const float* __restrict__ g, float inv_temp, VhRow* __restrict__ rows,
-                                                             float* __restrict__ scale, uint16_t* __restrict__ hz, int T, int V, int H) {
+                                                             float* __restrict__ scale, uint16_t* __restrict__ hz, uint16_t* __restrict__ hzt, int TP,
+                                                          int T, int V, int H) {
     const int t = blockIdx.x;
     VhRow ri = {0.f, 0.f, 0.f, -1};
     float sc = 1.f;
@@ -451,7 +458,7 @@ __global__ __launch_bounds__(128) void head_rows_label_kernel(const uint16_t* __
         }
         if (threadIdx.x == 0) { rows[t] = ri; scale[t] = sc; }
     }
-    vh_pack_row(h, ldh, hz, t, ri.hot != 0.f, sc, H);
+    vh_pack_row(h, ldh, hz, hzt, TP, t, ri.hot != 0.f, sc, H);
 }
 
 // slab[s][m][n] (+)= sum over the K-slice s of d[m][:] w[:][n]: w is contraction-major as stored; `kv` of the ldd columns of d are vocabulary
@@ -837,23 +844,6 @@ __global__ __launch_bounds__(256, OUT_BF16 ? 2 : 1) void head_dw_mid_kernel(cons
     }
 }
 
-// hzt[n][t] = hz[t][n], t < TP <= 64 ceil(T / 64): 64 x 64 elements per workgroup
-__global__ __launch_bounds__(256) void head_hzt_kernel(const uint16_t* __restrict__ hz, uint16_t* __restrict__ hzt, int TP, int H) {
-    __shared__ uint16_t tile[64][72];
-    const int n0 = blockIdx.x * 64, t0 = blockIdx.y * 64;
-    for (int i = threadIdx.x; i < 64 * 8; i += 256)
-        *reinterpret_cast<uint4*>(&tile[i >> 3][(i & 7) * 8]) = *reinterpret_cast<const uint4*>(hz + (int64_t)(t0 + (i >> 3)) * H + n0 + (i & 7) * 8);
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 8; i += 256) {
-        const int n = i >> 3, c = (i & 7) * 8;
-        if (t0 + c >= TP) continue;
-        uint4 o;
-        o.x = tile[c][n] | (uint32_t)tile[c + 1][n] << 16; o.y = tile[c + 2][n] | (uint32_t)tile[c + 3][n] << 16;
-        o.z = tile[c + 4][n] | (uint32_t)tile[c + 5][n] << 16; o.w = tile[c + 6][n] | (uint32_t)tile[c + 7][n] << 16;
-        *reinterpret_cast<uint4*>(hzt + (int64_t)(n0 + n) * TP + t0 + c) = o;
-    }
-}
-
 // ------------------------------------------------------------------------------------------------------------------------------------
 // Distillation from k teacher log-probs per row.
 // ------------------------------------------------------------------------------------------------------------------------------------
@@ -946,7 +936,8 @@ __global__ __launch_bounds__(256) void head_kl_kernel(const int32_t* __restrict_
 __global__ __launch_bounds__(128) void head_rows_kl_kernel(const uint16_t* __restrict__ h, int64_t ldh, const int32_t* __restrict__ ids,
                                                           const float* __restrict__ a, int K, int renorm, const float* __restrict__ lse,
                                                           const float* __restrict__ logq, const float* __restrict__ g, float inv_temp,
-                                                          VhRow* __restrict__ rows, float* __restrict__ scale, uint16_t* __restrict__ hz, int T, int V, int H) {
+                                                          VhRow* __restrict__ rows, float* __restrict__ scale, uint16_t* __restrict__ hz, uint16_t* __restrict__ hzt, int TP,
+                                                          int T, int V, int H) {
     const int t = blockIdx.x, lane = threadIdx.x & 63;
     VhRow ri = {0.f, 0.f, 0.f, -1};
     float sc = 1.f;
@@ -972,7 +963,7 @@ __global__ __launch_bounds__(128) void head_rows_kl_kernel(const uint16_t* __res
         }
         if (threadIdx.x == 0) { rows[t] = ri; scale[t] = sc; }
     }
-    vh_pack_row(h, ldh, hz, t, ri.c != 0.f, sc, H);
+    vh_pack_row(h, ldh, hz, hzt, TP, t, ri.c != 0.f, sc, H);
 }
 
 // d' at the targets of a piece [v0, v0 + kv): overwritten with the whole value (c / P) (P q - sum of the p of this id), from the fp32
@@ -1052,8 +1043,8 @@ Plan head_plan(int T, int V, int H, int K) {                         // K: targe
     p.rows = 0;
     p.scale = up((int64_t)T * (int64_t)sizeof(VhRow), 256);
     p.hz = p.scale + up((int64_t)T * 4, 256);
-    p.hzt = p.hz + up((int64_t)p.T64 * H * 2, 256);
-    p.d = p.hzt + (p.few ? up((int64_t)p.T64 * H * 2, 256) : 0);
+    p.hzt = p.hz;                                                    // one of the two
+    p.d = p.hz + up((int64_t)p.T64 * H * 2, 256);
     p.dt = p.d + up((int64_t)p.T64 * p.piece * 2, 256);
     p.slab = p.dt + (p.few ? up((int64_t)p.T64 * p.piece * 2, 256) : 0);
     p.bwd_bytes = p.slab + up((int64_t)std::max(p.split, p.split_both) * T * H * 4, 256);
@@ -1156,10 +1147,6 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
     allow_lds<head_tile_kernel<true, true>>(); allow_lds<head_tile_kernel<true, false>>();
     allow_lds<head_dh_kernel<false, true>>(); allow_lds<head_dh_kernel<true, true>>(); allow_lds<head_dh_kernel<false, false>>(); allow_lds<head_dh_kernel<true, false>>();
     allow_lds<head_dw_kernel<true, false>>(); allow_lds<head_dw_kernel<false, false>>(); allow_lds<head_dw_kernel<false, true>>();
-    if (p.few && (dwb || dwf)) {
-        hipLaunchKernelGGL(head_hzt_kernel, dim3(H / 64, p.T64 / 64), dim3(256), 0, s, hz, hzt, p.TP, H);
-        ST_CHECK_LAUNCH();
-    }
     for (int i = 0; i < p.pieces; ++i) {
         const int v0 = i * p.piece, kv = std::min(p.piece, V - v0), tn = st_cdiv(kv, 256);
         const int64_t ldd = up(kv, 64);
@@ -1282,8 +1269,8 @@ int st_linear_logprob_bwd(const st_bf16* hidden, int64_t ldh, const st_bf16* wei
     const Plan p = head_plan(T, V, H, 0);
     if (!workspace || workspace_bytes < p.bwd_bytes) return ST_EINVAL;
     char* ws = (char*)workspace;
-    hipLaunchKernelGGL(head_rows_label_kernel, dim3(p.T64), dim3(128), 0, s, hidden, ldh, labels, logp, lse, g, inv_temperature, (VhRow*)(ws + p.rows),
-                       (float*)(ws + p.scale), (uint16_t*)(ws + p.hz), T, V, H);
+    hipLaunchKernelGGL(head_rows_label_kernel, dim3(p.few ? p.TP : p.T64), dim3(128), 0, s, hidden, ldh, labels, logp, lse, g, inv_temperature, (VhRow*)(ws + p.rows),
+                       (float*)(ws + p.scale), p.few ? nullptr : (uint16_t*)(ws + p.hz), (uint16_t*)(ws + p.hzt), p.TP, T, V, H);
     ST_CHECK_LAUNCH();
     return head_backward(hidden, ldh, weight, ldw, inv_temperature * VH_LOG2E, dhidden, lddh, dweight_bf16, dweight_f32, lddw, accumulate, ws, p, T, V, H, s,
                          [](int, int, uint16_t*, int64_t, uint16_t*) { return 0; });
@@ -1325,8 +1312,8 @@ int st_linear_topk_kl_bwd(const st_bf16* hidden, int64_t ldh, const st_bf16* wei
     const Plan p = head_plan(T, V, H, 0);
     if (!workspace || workspace_bytes < p.bwd_bytes) return ST_EINVAL;
     char* ws = (char*)workspace;
-    hipLaunchKernelGGL(head_rows_kl_kernel, dim3(p.T64), dim3(128), 0, s, hidden, ldh, ids, teacher_logp, K, renormalize, lse, logq, g, inv_temperature,
-                       (VhRow*)(ws + p.rows), (float*)(ws + p.scale), (uint16_t*)(ws + p.hz), T, V, H);
+    hipLaunchKernelGGL(head_rows_kl_kernel, dim3(p.few ? p.TP : p.T64), dim3(128), 0, s, hidden, ldh, ids, teacher_logp, K, renormalize, lse, logq, g, inv_temperature,
+                       (VhRow*)(ws + p.rows), (float*)(ws + p.scale), p.few ? nullptr : (uint16_t*)(ws + p.hz), (uint16_t*)(ws + p.hzt), p.TP, T, V, H);
     ST_CHECK_LAUNCH();
     return head_backward(hidden, ldh, weight, ldw, inv_temperature * VH_LOG2E, dhidden, lddh, dweight_bf16, dweight_f32, lddw, accumulate, ws, p, T, V, H, s,
                          [&](int v0, int kv, uint16_t* d, int64_t ldd, uint16_t* dt) -> int {
