@@ -758,7 +758,7 @@ __device__ __forceinline__ void vh_tr_frag4(uint32_t a0, uint32_t a1, uint32_t a
 
 template <int KS, bool OUT_BF16, bool ACCUM>
 __global__ __launch_bounds__(256, OUT_BF16 ? 2 : 1) void head_dw_mid_kernel(const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ hz, int kv, int H,
-                                                            uint16_t* __restrict__ dwb, float* __restrict__ dwf, int64_t lddw) {
+                                                            int cols_per, uint16_t* __restrict__ dwb, float* __restrict__ dwf, int64_t lddw) {
     constexpr int T64 = KS * 32, TB = T64 * 128, RB = 64 * 2 + 16;       // TB: bytes of a [T64][64] image; RB: row of the output image
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, fr = lane & 15, fk = lane >> 4;
@@ -788,7 +788,7 @@ __global__ __launch_bounds__(256, OUT_BF16 ? 2 : 1) void head_dw_mid_kernel(cons
             for (int s = 0; s < KS; ++s) vh_tr_frag4(tr[0] + s * 4096, tr[1] + s * 4096, tr[2] + s * 4096, tr[3] + s * 4096, df[s]);
     }
     char* img = smem + TB;
-    for (int c0 = 0; c0 < H; c0 += 64) {
+    for (int c0 = blockIdx.y * cols_per; c0 < min(H, (int)(blockIdx.y + 1) * cols_per); c0 += 64) {
         __syncthreads();                                             // every wave has read the image (and stored its part of the output)
         for (int j = wave; j < T64 / 8; j += 4) {
             const int row = j * 8 + cr;
@@ -848,6 +848,8 @@ __global__ __launch_bounds__(256, OUT_BF16 ? 2 : 1) void head_dw_mid_kernel(cons
 // Distillation from k teacher log-probs per row.
 // ------------------------------------------------------------------------------------------------------------------------------------
 #define VH_MAX_K 1024
+#define VH_MID_SPLIT 3                                               // column ranges of head_dw_mid_kernel: 594 row blocks alone are 1.2 rounds of two per CU
+
 #define VH_FEW 128                                                   // rows up to which the weight stream bounds the products
 #define VH_MAX_V (1 << 22)                                           // column tiles fit the counters of head_bucket_kernel
 
@@ -1201,9 +1203,9 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
 #undef VH_DW_FEW
             }
             else if (mid) {
-                const int smem = p.T64 * 128 + 4 * 64 * 144;
+                const int smem = p.T64 * 128 + 4 * 64 * 144, mid_cols = (int)up(st_cdiv(H, VH_MID_SPLIT), 64);
 #define VH_DW_MID(KS, OB, AC) do { allow_lds<head_dw_mid_kernel<KS, OB, AC>>(smem); \
-        hipLaunchKernelGGL((head_dw_mid_kernel<KS, OB, AC>), dim3(tv), dim3(256), smem, s, d, ldd, hz, kv, H, ob, of, lddw); } while (0)
+        hipLaunchKernelGGL((head_dw_mid_kernel<KS, OB, AC>), dim3(tv, st_cdiv(H, mid_cols)), dim3(256), smem, s, d, ldd, hz, kv, H, mid_cols, ob, of, lddw); } while (0)
                 if (p.T64 == 192) { if (dwb) VH_DW_MID(6, true, false); else if (accumulate) VH_DW_MID(6, false, true); else VH_DW_MID(6, false, false); }
                 else { if (dwb) VH_DW_MID(8, true, false); else if (accumulate) VH_DW_MID(8, false, true); else VH_DW_MID(8, false, false); }
 #undef VH_DW_MID
