@@ -387,6 +387,10 @@ class Qwen25VL:
         self.fp8 = False                 # config #5: the LM's four projection GEMMs run forward in MX-fp8 (enable_fp8)
         self.fp8_dgrad = False           # ... and their input-gradient GEMMs too
         self.fp8_wgrad = False           # ... and their weight-gradient GEMMs
+        # True: the lm_head writes its bf16 logits, (response rows x vocabulary).  False: log-probs and their gradients straight from the hidden
+        # states (ops.linear_logprob_*): no logits buffer (2.5 GB at 8192 rows of the 7B head, the workspace stays near 0.5 GiB + the
+        # fp32 dhidden), fp32 logits, and one more product in the backward, which forms the logits again
+        self.store_logits = os.environ.get("ST_STORE_LOGITS", "1") != "0"
 
     # ---------------------------------------------------------------- Ulysses sequence parallelism
     def set_sequence_parallel(self, group) -> None:
@@ -816,6 +820,9 @@ class Qwen25VL:
         xr = ops.rows_gather(x, b.logit_rows)                       # only rows that predict a response token
         hn, rn = ops.rmsnorm_fwd(xr, w["final_norm"], c.rms_eps)
         head = w["embed"] if c.tie_word_embeddings else w["lm_head"]
+        if not self.store_logits:
+            logp, lse = ops.linear_logprob_fwd(hn, head, b.labels, temperature)
+            return xr, hn, rn, None, logp, lse
         logits = ops.gemm_nt(hn, head)
         logp, lse = ops.logprob_fwd(logits, b.labels, temperature)
         return xr, hn, rn, logits, logp, lse
@@ -854,8 +861,10 @@ class Qwen25VL:
             ops.rows_gather(x, b.logit_rows, out=xr[n_first:n_first + n_rest])
         hn, _ = ops.rmsnorm_fwd(xr, w["final_norm"], c.rms_eps)
         head = w["embed"] if c.tie_word_embeddings else w["lm_head"]
-        logits = ops.gemm_nt(hn, head)
-        logp, _ = ops.logprob_fwd(logits, b.labels, temperature)
+        if self.store_logits:
+            logp, _ = ops.logprob_fwd(ops.gemm_nt(hn, head), b.labels, temperature)
+        else:
+            logp, _ = ops.linear_logprob_fwd(hn, head, b.labels, temperature)
         out = torch.zeros(b.pk.B * b.pk.R, dtype=F32, device=x.device)
         out.index_copy_(0, b.out_index, logp[:len(b.out_index)])
         return out.view(b.pk.B, b.pk.R)
@@ -1005,10 +1014,13 @@ class Qwen25VL:
             # so every weight gradient below is a partial sum over the rank's tokens (the sp ranks' gradients add up to the full one)
             mine = (b.logit_rows[:Tr] >= sp_lo) & (b.logit_rows[:Tr] < sp_lo + sp_Tl)
             grow[:Tr] *= mine.to(grow.dtype)
-        ops.logprob_bwd_(logits, b.labels, lse, grow, temperature)                       # logits buffer now holds dlogits
         head_name = "embed" if c.tie_word_embeddings else "lm_head"
-        self._dw(g[head_name], logits, hn, None)
-        dhn = ops.gemm_nn(logits, w[head_name])
+        if logits is None:
+            dhn = ops.linear_logprob_bwd(hn, w[head_name], b.labels, logp, lse, grow, temperature, dweight_f32=g[head_name], accumulate=True)
+        else:
+            ops.logprob_bwd_(logits, b.labels, lse, grow, temperature)                   # logits buffer now holds dlogits
+            self._dw(g[head_name], logits, hn, None)
+            dhn = ops.gemm_nn(logits, w[head_name])
         dxr = ops.rmsnorm_bwd(xr, self.p.w["final_norm"], rn, dhn, dw_accum=g["final_norm"])
         if on_final is not None and not c.tie_word_embeddings:      # final_norm + lm_head close the buffer (param_layout)
             on_final(off["final_norm"], self.p.numel)

@@ -68,6 +68,9 @@ ActorConfig = _build("ActorConfig", {
     "optim": (OptimConfig, OptimConfig), "fsdp": (FSDPConfig, FSDPConfig), "offload": (OffloadConfig, OffloadConfig),
     "global_batch_size_per_device": (int, -1), "disable_kl": (bool, False), "use_kl_loss": (bool, False), "kl_penalty": (str, "kl"),
     "kl_coef": (float, 0.0),
+    # extension (not a reference key; default = the reference's behaviour): false computes log-probs and their gradients without writing the
+    # (rows x vocabulary) logits, in the actor's and the reference policy's passes (spatialthinker_amd.model Qwen25VL.store_logits)
+    "store_logits": (bool, True),
 })
 
 RefConfig = _build("RefConfig", {

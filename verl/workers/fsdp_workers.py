@@ -169,6 +169,7 @@ class FSDPWorker(Worker):
                                grad_exchange_dtype="bf16" if str(a.fsdp.mp_reduce_dtype).lower() in ("bf16", "bfloat16") else "fp32")
             self.model_config, self.special = cfg, special
             self.actor = PolicyEngine(cfg, store, hyper, sp_group=self.sp_group)
+            self.actor.model.store_logits &= bool(a.store_logits)
             self.flops_counter = FlopsCounter(cfg)
             if self.world_size > 1:                          # sync_module_states: rank 0's weights everywhere (fsdp_workers.py:261-263)
                 dist.broadcast(store.flat, src=0)
@@ -185,6 +186,7 @@ class FSDPWorker(Worker):
                 dist.broadcast(store.flat, src=0)
             self.model_config, self.special = cfg, special
             self.ref_policy = PolicyEngine(cfg, store, None, sp_group=self.sp_group)
+            self.ref_policy.model.store_logits &= bool(self.config.actor.store_logits)
 
     # ------------------------------------------------------------------------------------------------
     @staticmethod
