@@ -64,7 +64,7 @@ int st_logprob_bwd(st_bf16* logits, int64_t ldl, const int64_t* labels, const fl
  * weight^T * inv_temperature is formed tile by tile in fp32 and never stored; the logits of st_gemm_nt + st_logprob_fwd are rounded to bf16 and
  * take 2 T V bytes.  Call sites they stand next to: verl/workers/actor/dp_actor.py:125-128 (logits / temperature, log_probs_from_logits) and
  * its backward :266-279.
- *   - H % 64 == 0; V <= 2^22; T * K < 2^31; ldh, ldw multiples of 8 below 2^22; hidden, weight, dweight_bf16, dweight_f32 16-byte, dhidden 8-byte aligned; T == 0 is
+ *   - H % 64 == 0; V <= 2^21; T * K < 2^31; ldh, ldw multiples of 8 below 2^22; hidden, weight, dweight_bf16, dweight_f32 16-byte, dhidden 8-byte aligned; T == 0 is
  *     allowed (dweight: zeros, or left as it is with accumulate).
  *   - workspace: st_linear_head_workspace_bytes(T, V, H, K (0 for labels), backward) bytes, 16-byte aligned, contents irrelevant.  Nothing is kept in it between
  *     calls: calls on several streams and captured graphs need one each.  backward != 0 covers any subset of the gradients.

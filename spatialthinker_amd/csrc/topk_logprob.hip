@@ -416,7 +416,7 @@ int st_topk_logprob_workspace_bytes(int T, int V, int k, int64_t* bytes_host, st
 
 int st_topk_logprob(const st_bf16* logits, int64_t ldl, int k, float inv_temperature, int32_t* ids, float* logp, float* lse, void* workspace,
                     int64_t workspace_bytes, int T, int V, st_stream_t stream) {
-    if (T < 0 || V <= 0 || k <= 0 || k > V || k > TK_MAX_K || !(inv_temperature > 0.f && inv_temperature < INFINITY)) return ST_EINVAL;
+    if (T < 0 || V <= 0 || k <= 0 || k > V || k > TK_MAX_K || !(inv_temperature > 0.f && inv_temperature * TK_LOG2E < INFINITY)) return ST_EINVAL;
     if (T == 0) return 0;
     if (!logits || ldl < V || !ids || !logp || !lse || T > 0x7fffffff / TK_MAX_K || (((uintptr_t)logits) & 1)) return ST_EINVAL;
     hipStream_t s = (hipStream_t)stream;

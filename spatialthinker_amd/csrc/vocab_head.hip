@@ -851,7 +851,7 @@ __global__ __launch_bounds__(256, OUT_BF16 ? 2 : 1) void head_dw_mid_kernel(cons
 #define VH_MID_SPLIT 3                                               // column ranges of head_dw_mid_kernel: 594 row blocks alone are 1.2 rounds of two per CU
 
 #define VH_FEW 128                                                   // rows up to which the weight stream bounds the products
-#define VH_MAX_V (1 << 22)                                           // column tiles fit the counters of head_bucket_kernel
+#define VH_MAX_V (1 << 21)                                           // column tiles fit the counters of head_bucket_kernel
 
 // teacher probabilities of one row, by one wave: p_k of present entries (0 <= id < V), 0 for the others; log p_k = a_k - shift
 struct VhTeacher { float shift, total; };
@@ -1055,7 +1055,7 @@ Plan head_plan(int T, int V, int H, int K) {                         // K: targe
 
 bool operands_ok(const void* h, int64_t ldh, const void* w, int64_t ldw, int T, int V, int H, float inv_temp) {
     return h && w && T >= 0 && V > 0 && V <= VH_MAX_V && H > 0 && H % 64 == 0 && !(ldh & 7) && !(ldw & 7) && ldh >= H && ldw >= H && ldh < (1 << 22) && ldw < (1 << 22) &&
-           !(((uintptr_t)h) & 15) && !(((uintptr_t)w) & 15) && inv_temp > 0.f && inv_temp < INFINITY && (int64_t)st_cdiv(T, 256) * st_cdiv(V, 256) < (1 << 30);
+           !(((uintptr_t)h) & 15) && !(((uintptr_t)w) & 15) && inv_temp > 0.f && inv_temp * VH_LOG2E < INFINITY && (int64_t)st_cdiv(T, 256) * st_cdiv(V, 256) < (1 << 30);
 }
 
 // one attribute per kernel and device, set before its first launch there

@@ -118,7 +118,7 @@ def grpo_advantage(rewards, mask, group, n_groups: int, eps: float = 1e-6):
 
 # ------------------------------------------------------------------ vocabulary head without stored logits
 HEAD_MAX_TARGETS = 1024         # VH_MAX_K of the library
-HEAD_MAX_VOCAB = 1 << 22        # VH_MAX_V of the library
+HEAD_MAX_VOCAB = 1 << 21        # VH_MAX_V of the library
 TOPK_MAX = 256                  # TK_MAX_K of the library
 
 
@@ -143,8 +143,8 @@ def _vec(t, dtype, shape, device, what):
 
 
 def _positive(temperature):
-    if not (temperature > 0.0 and math.isfinite(temperature) and math.isfinite(1.0 / temperature)):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not (temperature > 0.0 and 1e-30 < 1.0 / temperature < 1e30):
+        raise ValueError(f"temperature must be positive, finite and its inverse within 1e-30 .. 1e30, got {temperature}")
 
 
 def _head_operands(hidden, weight, temperature):
