@@ -4,6 +4,9 @@ Host bookkeeping on (batch, length) tensors — masked_mean, get_response_mask, 
 torch.  The heavy entries are the HIP library behind the reference's own signatures, so code written against the reference imports
 and runs unchanged:
   log_probs_from_logits(logits, labels)   :34-66    -> autograd.Function over st_logprob_fwd / st_logprob_bwd
+  linear_log_probs(hidden, weight, labels)          -> the same log-probs from the head's inputs, no logits kept (st_linear_logprob_fwd / _bwd)
+  top_log_probs(logits, k)                          -> a teacher's k largest log-probs of every row (st_topk_logprob)
+  linear_topk_kl(hidden, weight, ids, log_probs)    -> distillation from them, no logits kept (st_linear_topk_kl_fwd / _bwd)
   AnyPrecisionAdamW(params, lr, ...)      :201-329  -> torch.optim.Optimizer whose step() is st_adamw_kahan_step per parameter
   get_constant_schedule_with_warmup(...)  :187-197  -> LambdaLR with the same multiplier
 The training engine (spatialthinker_amd/actor.py) calls the same kernels on its flat buffers directly."""
@@ -188,8 +191,8 @@ def _flat(t: torch.Tensor, dtype: torch.dtype, device: torch.device) -> torch.Te
 
 def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
     """log_probs_from_logits(hidden @ weight^T / temperature, labels) without the logits: hidden (..., H), weight (V, H) (the head), labels (...)
-    -> (...) fp32, differentiable in hidden and weight.  At V = 152 064 the logits of 8192 rows are 2.5 GB; here the backward's workspace stays
-    within 0.5 GiB for one piece of the vocabulary and the logits stay in fp32.  A label outside [0, V) (padding, -100) marks a row that is not
+    -> (...) fp32, differentiable in hidden and weight.  At V = 152 064 the logits of 8192 rows are 2.5 GB; here the backward keeps
+    one piece of the vocabulary's gradient at a time (0.5 GiB at most) next to fp32 partial sums of hidden's, and the logits stay in fp32.  A label outside [0, V) (padding, -100) marks a row that is not
     scored: 0, and no gradient from it.  H must be a multiple of 64; GPU tensors only."""
     if labels.shape != hidden.shape[:-1]:
         raise ValueError(f"labels {tuple(labels.shape)} do not match hidden {tuple(hidden.shape)}")
