@@ -171,24 +171,27 @@ __global__ __launch_bounds__(256) void head_tile_kernel(const uint16_t* __restri
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
-// The same logit tile for few rows (T <= 128): the launch is a stream of the head's weights, so the tile is small and several workgroups share a CU
-// to keep copies in flight: BT = 16 MT rows x 128 vocabulary columns, four waves of 32 columns each, K-steps of 64 through SLOTS LDS slots filled
-// by LDS-DMA (16-byte chunk c of a row at position c ^ (row & 7): conflict-free fragment reads), SLOTS - 1 steps in flight behind one barrier per
-// step.  Epilogues as head_tile_kernel; part[n0 / 128][m].  DLOGITS also leaves d transposed, dt[n][TP], for head_dw_few_kernel.
+// The same logit tile for few rows (T <= 160): the launch is a stream of the head's weights.  BT = 16 MT rows x 32 vocabulary columns per wave, K-steps
+// of 64 through SLOTS LDS slots filled by LDS-DMA (16-byte chunk c of a row at position c ^ (row & 7): conflict-free fragment reads), SLOTS - 1 steps
+// in flight behind one barrier per step.  Up to 64 rows four waves, so that several workgroups share a CU and one's epilogue hides behind another's
+// copies; beyond, eight waves with the whole LDS, because the hidden states are copied again for every workgroup: 128 rows beside 128 columns fill as
+// many bytes with them as with weights.  Epilogues as head_tile_kernel; part[block][m].  DLOGITS also leaves d transposed, dt[n][TP], up to 128 rows.
+// MI355X, V = 152 064, forward with its join (of 6.8 TB/s that a read alone reaches): H = 3584, 1 row 162 us = 6.7 TB/s, 64 rows 176 = 6.2, 96 rows
+// 207 = 5.3 (128 columns: 226), 128 rows 217 = 5.0 (245), 160 rows 247 = 4.4 (256-row tile 275); H = 2048, 1 row 104 us = 6.0 TB/s, 160 rows 149.
 // ------------------------------------------------------------------------------------------------------------------------------------
 template <int N> __device__ __forceinline__ void vh_wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-template <int MT, int SLOTS, bool DLOGITS>
-__global__ __launch_bounds__(256, 2) void head_few_kernel(const uint16_t* __restrict__ h, int64_t ldh, const uint16_t* __restrict__ w, int64_t ldw, int T, int V,
+template <int MT, int SLOTS, int WAVES, bool DLOGITS>
+__global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t* __restrict__ h, int64_t ldh, const uint16_t* __restrict__ w, int64_t ldw, int T, int V,
                                                          int H, float sc, const int64_t* __restrict__ labels, float2* __restrict__ part,
                                                          float* __restrict__ zlab, VhTargets tg, const VhRow* __restrict__ rows, int v0,
                                                          uint16_t* __restrict__ d, int64_t ldd, uint16_t* __restrict__ dt, int TP) {
-    constexpr int BT = 16 * MT, SLOT = (128 + BT) * 128, HC = MT / 2;    // HC: 1-KiB copies of h per wave and step
-    static_assert(MT % 2 == 0, "every wave copies the same number of rows");
+    constexpr int BT = 16 * MT, BN = 32 * WAVES, SLOT = (BN + BT) * 128, NT = 64 * WAVES;
+    constexpr int HC = (2 * MT + WAVES - 1) / WAVES;                 // 1-KiB copies of h per wave and step (the last waves may copy some rows again)
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n0 = blockIdx.x * 128;
+    const int n0 = blockIdx.x * BN;
     // copy j of a wave: 8 rows, lane -> row (lane >> 3), 16-byte chunk (lane & 7) ^ row
     const int cr = lane >> 3, ch = ((lane & 7) ^ cr) * 8;
     const uint16_t* wsrc[4];
@@ -196,20 +199,24 @@ __global__ __launch_bounds__(256, 2) void head_few_kernel(const uint16_t* __rest
 #pragma unroll
     for (int j = 0; j < 4; ++j) wsrc[j] = w + (int64_t)min(n0 + wave * 32 + j * 8 + cr, V - 1) * ldw + ch;
 #pragma unroll
-    for (int j = 0; j < HC; ++j) hsrc[j] = h + (int64_t)min(wave * 8 * HC + j * 8 + cr, T - 1) * ldh + ch;
+    for (int j = 0; j < HC; ++j) hsrc[j] = h + (int64_t)min((wave * HC + j) % (2 * MT) * 8 + cr, T - 1) * ldh + ch;
+    const int nk = H / 64, fr = lane & 15, fk = lane >> 4;
+    // K-step kt reads k = (kt + turn) % nk: rows at a pitch of whole 4 KiB meet in a few memory channels where all workgroups stand at the same k
+    // (V = 100 000, H = 2048: 8 rows 89 -> 79 us, 100 rows 107 -> 90; H = 4096: 168 -> 141, 200 -> 157; at other pitches 0 to 3 % slower, so not there)
+    const int turn = (ldw & 2047) == 0 ? (int)blockIdx.x % nk : 0;
     auto stage = [&](int kt) {
         char* dst = smem + (kt % SLOTS) * SLOT;
+        const int k = (kt + turn < nk ? kt + turn : kt + turn - nk) * 64;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) st_glds16_nt(wsrc[j] + kt * 64, dst + (wave * 32 + j * 8) * 128);       // one workgroup reads a weight, once
+        for (int j = 0; j < 4; ++j) st_glds16_nt(wsrc[j] + k, dst + (wave * 32 + j * 8) * 128);       // one workgroup reads a weight, once
 #pragma unroll
-        for (int j = 0; j < HC; ++j) st_glds16(hsrc[j] + kt * 64, dst + (128 + wave * 8 * HC + j * 8) * 128);
+        for (int j = 0; j < HC; ++j) st_glds16(hsrc[j] + k, dst + (BN + (wave * HC + j) % (2 * MT) * 8) * 128);
     };
     f32x4 acc[2][MT];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < MT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    const int nk = H / 64, fr = lane & 15, fk = lane >> 4;
 #pragma unroll
     for (int s = 0; s < SLOTS - 1; ++s) if (s < nk) stage(s);
     for (int kt = 0; kt < nk; ++kt) {
@@ -219,7 +226,7 @@ __global__ __launch_bounds__(256, 2) void head_few_kernel(const uint16_t* __rest
         asm volatile("" ::: "memory");
         if (kt + SLOTS - 1 < nk) stage(kt + SLOTS - 1);
         const char* lw = smem + (kt % SLOTS) * SLOT + wave * 32 * 128;
-        const char* lh = smem + (kt % SLOTS) * SLOT + 128 * 128;
+        const char* lh = smem + (kt % SLOTS) * SLOT + BN * 128;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const int c = ((s * 4 + fk) ^ (fr & 7)) << 4;
@@ -239,16 +246,18 @@ __global__ __launch_bounds__(256, 2) void head_few_kernel(const uint16_t* __rest
     if constexpr (!DLOGITS) {
         constexpr int ROWB = 128 * 4 + 16;
         const int e0 = tg.start ? tg.start[n0 >> 8] : 0, e1 = tg.start ? tg.start[(n0 >> 8) + 1] : 0;
-        if (e1 > e0) {
+        for (int p = 0; p < BN / 128 && e1 > e0; ++p) {              // the tile through LDS, 128 columns at a time
+            if (wave >> 2 == p) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(smem + (j * 16 + fr) * ROWB + (wave * 32 + i * 16 + fk * 4) * 4) = acc[i][j];
+                    for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(smem + (j * 16 + fr) * ROWB + ((wave & 3) * 32 + i * 16 + fk * 4) * 4) = acc[i][j];
+            }
             __syncthreads();
-            for (int e = e0 + threadIdx.x; e < e1; e += 256) {
+            for (int e = e0 + threadIdx.x; e < e1; e += NT) {
                 const uint32_t it = tg.list[e];
                 const int row = it & 255, col = (it >> 8) & 255;
-                if ((col >> 7) == ((n0 >> 7) & 1))
+                if ((col >> 7) == (((n0 >> 7) + p) & 1))
                     tg.z2[(int64_t)row * tg.K + (it >> 16)] = sc * *reinterpret_cast<const float*>(smem + row * ROWB + (col & 127) * 4);
             }
             __syncthreads();
@@ -286,10 +295,10 @@ __global__ __launch_bounds__(256, 2) void head_few_kernel(const uint16_t* __rest
             }
         }
         __syncthreads();
-        for (int m = threadIdx.x; m < min(BT, T); m += 256) {
+        for (int m = threadIdx.x; m < min(BT, T); m += NT) {
             float2 a = red[m];
 #pragma unroll
-            for (int wv = 1; wv < 4; ++wv) {
+            for (int wv = 1; wv < WAVES; ++wv) {
                 const float2 b = red[wv * BT + m];
                 const float mn = fmaxf(a.x, b.x);
                 a = make_float2(mn, mn != -INFINITY ? a.y * vh_exp2(a.x - mn) + b.y * vh_exp2(b.x - mn) : a.y + b.y);
@@ -297,8 +306,8 @@ __global__ __launch_bounds__(256, 2) void head_few_kernel(const uint16_t* __rest
             part[(int64_t)blockIdx.x * T + m] = a;
         }
     } else {
-        // two bf16 images: [BT rows][128 columns] and [128 columns][BT rows]
-        constexpr int RB = 128 * 2 + 16, CB = BT * 2 + 16;
+        // two bf16 images: [BT rows][BN columns] and (up to 128 rows) [BN columns][BT rows]
+        constexpr int RB = BN * 2 + 16, CB = BT * 2 + 16;
         char* img_t = smem + BT * RB;
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
@@ -320,22 +329,30 @@ __global__ __launch_bounds__(256, 2) void head_few_kernel(const uint16_t* __rest
                 pk.x = f2bf2(o[0], o[1]); pk.y = f2bf2(o[2], o[3]);
                 const int col = wave * 32 + i * 16 + fk * 4;
                 *reinterpret_cast<uint2*>(smem + m * RB + col * 2) = pk;
-                *reinterpret_cast<uint16_t*>(img_t + (col + 0) * CB + m * 2) = (uint16_t)pk.x;
-                *reinterpret_cast<uint16_t*>(img_t + (col + 1) * CB + m * 2) = (uint16_t)(pk.x >> 16);
-                *reinterpret_cast<uint16_t*>(img_t + (col + 2) * CB + m * 2) = (uint16_t)pk.y;
-                *reinterpret_cast<uint16_t*>(img_t + (col + 3) * CB + m * 2) = (uint16_t)(pk.y >> 16);
+                if constexpr (MT <= 8) {
+                    *reinterpret_cast<uint16_t*>(img_t + (col + 0) * CB + m * 2) = (uint16_t)pk.x;
+                    *reinterpret_cast<uint16_t*>(img_t + (col + 1) * CB + m * 2) = (uint16_t)(pk.x >> 16);
+                    *reinterpret_cast<uint16_t*>(img_t + (col + 2) * CB + m * 2) = (uint16_t)pk.y;
+                    *reinterpret_cast<uint16_t*>(img_t + (col + 3) * CB + m * 2) = (uint16_t)(pk.y >> 16);
+                }
             }
         }
         __syncthreads();
-        const int cols = min(128, (int)ldd - n0);                    // ldd % 64 == 0
-        for (int i = threadIdx.x; i < T * 16; i += 256) {
-            const int row = i >> 4, c = (i & 15) * 8;
-            if (c < cols) *reinterpret_cast<uint4*>(d + (int64_t)row * ldd + n0 + c) = *reinterpret_cast<const uint4*>(smem + row * RB + c * 2);
+        const int cols = min(BN, (int)ldd - n0);                     // ldd % 64 == 0
+        constexpr int CH = BN / 8;                                   // 16-byte chunks of a row of d
+        const int rows_out = MT <= 8 ? T : TP;                       // rows [T, TP) are zero for head_dw_mid_kernel
+        for (int i = threadIdx.x; i < rows_out * CH; i += NT) {
+            const int row = i / CH, c = (i % CH) * 8;
+            if (c < cols)
+                *reinterpret_cast<uint4*>(d + (int64_t)row * ldd + n0 + c) =
+                    MT <= 8 || row < BT ? *reinterpret_cast<const uint4*>(smem + row * RB + c * 2) : make_uint4(0, 0, 0, 0);
         }
-        const int per = TP >> 3;                                     // 16-byte chunks of a row of dt: TP is BT, or more (zeros)
-        for (int i = threadIdx.x; i < cols * per; i += 256) {
-            const int col = i / per, c = (i - col * per) * 8;
-            *reinterpret_cast<uint4*>(dt + (int64_t)(n0 + col) * TP + c) = c < BT ? *reinterpret_cast<const uint4*>(img_t + col * CB + c * 2) : make_uint4(0, 0, 0, 0);
+        if constexpr (MT <= 8) {
+            const int per = TP >> 3;                                 // 16-byte chunks of a row of dt: TP is BT, or more (zeros)
+            for (int i = threadIdx.x; i < cols * per; i += NT) {
+                const int col = i / per, c = (i - col * per) * 8;
+                *reinterpret_cast<uint4*>(dt + (int64_t)(n0 + col) * TP + c) = c < BT ? *reinterpret_cast<const uint4*>(img_t + col * CB + c * 2) : make_uint4(0, 0, 0, 0);
+            }
         }
     }
 }
@@ -694,15 +711,14 @@ __global__ __launch_bounds__(256) void head_dw_few_kernel(const uint16_t* __rest
 #pragma unroll
             for (int s = 0; s < KS; ++s) ahead[ni][s] = *reinterpret_cast<const bf16x8*>(hzt + (int64_t)min(c + ni * 16 + fr, H - 1) * TP + s * 32 + fk * 8);
     };
-    if constexpr (KS <= 2) fetch(wave * 64);
-    for (int c0 = 0; c0 < H; c0 += 256) {
+    auto block = [&](int c0, int next) {
         const int c = c0 + wave * 64;
         if constexpr (KS > 2) fetch(c);                              // (no registers left to be a step ahead)
 #pragma unroll
         for (int ni = 0; ni < 4; ++ni)
 #pragma unroll
             for (int s = 0; s < KS; ++s) hf[ni][s] = ahead[ni][s];
-        if constexpr (KS <= 2) fetch(c + 256);
+        if constexpr (KS <= 2) fetch(next + wave * 64);
 #pragma unroll
         for (int mi = 0; mi < MI; ++mi) {
 #pragma unroll
@@ -735,6 +751,18 @@ __global__ __launch_bounds__(256) void head_dw_few_kernel(const uint16_t* __rest
             }
             __syncthreads();
         }
+    };
+    if constexpr (KS <= 2) {                                         // each workgroup starts at another column block
+        const int nc = (H + 255) >> 8;
+        int c0 = (blockIdx.x % nc) << 8;
+        fetch(c0 + wave * 64);
+        for (int i = 0; i < nc; ++i) {
+            const int next = c0 + 256 < H ? c0 + 256 : 0;
+            block(c0, next);
+            c0 = next;
+        }
+    } else {
+        for (int c0 = 0; c0 < H; c0 += 256) block(c0, 0);
     }
 }
 
@@ -1069,20 +1097,27 @@ template <auto KERN> void allow_lds(int bytes = VH_SMEM) {
     }
 }
 
-// one launch of the few-row tile: T <= 32, 64 or 128 rows
+// one launch of the few-row tile: T <= 32, 64, 96, 128 or 160 rows
+constexpr int VH_STREAM = 160;
+int few_cols(int T) { return T <= 64 ? 128 : 256; }                  // vocabulary columns of a workgroup
+template <bool DLOGITS, int MT, int SLOTS, int WAVES, class... A>
+int launch_few_as(int V, hipStream_t s, A... args) {
+    constexpr int BT = 16 * MT, BN = 32 * WAVES, RING = SLOTS * (BN + BT) * 128;
+    constexpr int IMAGES = DLOGITS ? BT * (BN * 2 + 16) + (MT <= 8 ? BN * (BT * 2 + 16) : 0) : std::max(BT * (128 * 4 + 16), WAVES * BT * 8);
+    constexpr int SMEM = std::max(RING, IMAGES);
+    static_assert(SMEM <= 160 * 1024, "the ring and the epilogue's images share the LDS of a CU");
+    allow_lds<head_few_kernel<MT, SLOTS, WAVES, DLOGITS>>(SMEM);
+    hipLaunchKernelGGL((head_few_kernel<MT, SLOTS, WAVES, DLOGITS>), dim3(st_cdiv(V, BN)), dim3(64 * WAVES), SMEM, s, args...);
+    ST_CHECK_LAUNCH();
+    return 0;
+}
 template <bool DLOGITS, class... A>
 int launch_few(int T, int V, hipStream_t s, A... args) {
-    const dim3 grid(st_cdiv(V, 128));
-    auto go = [&](auto kern, int smem) {
-        hipLaunchKernelGGL(kern, grid, dim3(256), smem, s, args...);
-        ST_CHECK_LAUNCH();
-        return 0;
-    };
-    constexpr int S32 = 4 * 160 * 128, S64 = 3 * 192 * 128, S128 = 2 * 256 * 128;
-    if (T <= 32) { allow_lds<head_few_kernel<2, 4, DLOGITS>>(S32); return go(head_few_kernel<2, 4, DLOGITS>, S32); }
-    if (T <= 64) { allow_lds<head_few_kernel<4, 3, DLOGITS>>(S64); return go(head_few_kernel<4, 3, DLOGITS>, S64); }
-    allow_lds<head_few_kernel<8, 2, DLOGITS>>(S128 + 8192);
-    return go(head_few_kernel<8, 2, DLOGITS>, S128 + 8192);          // (the two images of the d epilogue: 128 x 272 bytes each)
+    if (T <= 32) return launch_few_as<DLOGITS, 2, 4, 4>(V, s, args...);
+    if (T <= 64) return launch_few_as<DLOGITS, 4, 3, 4>(V, s, args...);
+    if (T <= 96) return launch_few_as<DLOGITS, 6, 3, 8>(V, s, args...);
+    if (T <= 128) return launch_few_as<DLOGITS, 8, 3, 8>(V, s, args...);
+    return launch_few_as<DLOGITS, 10, 3, 8>(V, s, args...);
 }
 
 int head_stats(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, const int64_t* labels, float sc, float* logp, float* lse, VhTargets tg,
@@ -1091,8 +1126,8 @@ int head_stats(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, c
     float2* part = (float2*)(ws + p.part);
     float* zlab = (float*)(ws + p.zlab);
     int n_parts = 2 * tn;
-    if (p.few) {
-        n_parts = st_cdiv(V, 128);
+    if (T <= VH_STREAM) {
+        n_parts = st_cdiv(V, few_cols(T));
         const int rc = launch_few<false>(T, V, s, h, ldh, w, ldw, T, V, H, sc, labels, part, zlab, tg, (const VhRow*)nullptr, 0, (uint16_t*)nullptr,
                                          (int64_t)0, (uint16_t*)nullptr, 0);
         if (rc) return rc;
@@ -1153,9 +1188,9 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
         const int v0 = i * p.piece, kv = std::min(p.piece, V - v0), tn = st_cdiv(kv, 256);
         const int64_t ldd = up(kv, 64);
         const uint16_t* wp = w + (int64_t)v0 * ldw;
-        if (p.few) {
+        if (T <= VH_STREAM) {
             const int rc = launch_few<true>(T, kv, s, h, ldh, wp, ldw, T, kv, H, sc, (const int64_t*)nullptr, (float2*)nullptr, (float*)nullptr,
-                                            VhTargets{}, rows, v0, d, ldd, dt, p.TP);
+                                            VhTargets{}, rows, v0, d, ldd, dt, p.few ? p.TP : p.T64);
             if (rc) return rc;
         } else {
             auto go = [&](auto kern) {

@@ -214,6 +214,14 @@ def test_linear_topk_kl_forward_and_gradients(T, H, V, K, temperature, renorm):
     assert torch.isfinite(dh).all() and torch.isfinite(dw).all()
 
 
+@pytest.mark.parametrize("T", [32, 33, 77, 96, 97, 128, 130, 160, 161])
+@pytest.mark.parametrize("H", [64, 192, 2048])
+def test_row_tiles_of_the_weight_stream(T, H):
+    """The last and first row counts of each tile, with fewer, as many and more steps of 64 than copies in flight; H = 2048: rows at a pitch of 4 KiB."""
+    test_linear_log_probs_forward_and_gradients(T, H, 701, 1.0)
+    test_linear_topk_kl_forward_and_gradients(T, H, 519, 40, 1.0, True)
+
+
 def test_gradients_against_differences():
     """Central differences along random directions: <dh, h+ - h-> against the change of sum(g out), for steps that bf16 holds exactly.  The third-order
     rest of a difference of width e |h| (logits move by < 0.03) is below 1e-4 of the change's scale; 2 % covers it, the bf16 gradients (2^-8 per
@@ -268,6 +276,20 @@ def test_top_log_probs(T, V, k):
     z = (3 * torch.randn(T, V, device="cuda", generator=g)).to(BF16)               # 16-bit values over 150 000 places: many ties
     check_top(z, k, 1.0)
     check_top(z, k, 0.6)
+
+
+def test_top_log_probs_beyond_2_31_elements():
+    V, k = 152064, 20
+    T = 2 ** 31 // V + 40
+    g = torch.Generator(device="cuda").manual_seed(8)
+    z = torch.empty(T, V, device="cuda", dtype=BF16).normal_(generator=g)
+    from spatialthinker_amd import ops
+    ids, logp, lse = ops.topk_logprob(z, k)
+    rows = torch.tensor([0, 1, T // 2, T - 41, T - 40, T - 39, T - 1], device="cuda")
+    wi, wl, we = top64(z[rows], k, 1.0)
+    assert torch.equal(ids[rows], wi)
+    assert ((lse[rows].to(F64) - we).abs() <= 8 * U32 * (8 + we.abs()) + 2.0 ** -20).all()
+    assert ((logp[rows].to(F64) - wl).abs() <= 8 * U32 * (8 + we.abs()[:, None]) + 2.0 ** -20).all()
 
 
 @pytest.mark.parametrize("T", [1, 600])
