@@ -212,11 +212,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t*
 #pragma unroll
         for (int j = 0; j < HC; ++j) st_glds16(hsrc[j] + k, dst + (BN + (wave * HC + j) % (2 * MT) * 8) * 128);
     };
-    f32x4 acc[2][MT];
+    f32x4 acc[2][MT], sum[2][MT];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < MT; ++j) sum[i][j] = acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < SLOTS - 1; ++s) if (s < nk) stage(s);
     for (int kt = 0; kt < nk; ++kt) {
@@ -240,7 +240,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t*
 #pragma unroll
                 for (int j = 0; j < MT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[i], hf[j], acc[i][j], 0, 0, 0);
         }
+        if constexpr (MT <= 4) {                                     // sums of sums: fewer roundings, where registers and time are free
+            if ((kt & 7) == 7)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) { sum[i][j] += acc[i][j]; acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f}; }
+        }
     }
+    if constexpr (MT <= 4)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) acc[i][j] += sum[i][j];
     __syncthreads();                                                 // the slots are free
     const int col0 = n0 + wave * 32 + fk * 4;                        // column of (i, r): col0 + i*16 + r
     if constexpr (!DLOGITS) {
@@ -816,7 +828,9 @@ __global__ __launch_bounds__(256, OUT_BF16 ? 2 : 1) void head_dw_mid_kernel(cons
             for (int s = 0; s < KS; ++s) vh_tr_frag4(tr[0] + s * 4096, tr[1] + s * 4096, tr[2] + s * 4096, tr[3] + s * 4096, df[s]);
     }
     char* img = smem + TB;
-    for (int c0 = blockIdx.y * cols_per; c0 < min(H, (int)(blockIdx.y + 1) * cols_per); c0 += 64) {
+    const int first = blockIdx.y * cols_per, nc = (min(H, first + cols_per) - first) >> 6;
+    for (int i = 0, b = (int)blockIdx.x % nc; i < nc; ++i, b = b + 1 < nc ? b + 1 : 0) {   // each workgroup starts at another column block
+        const int c0 = first + b * 64;
         __syncthreads();                                             // every wave has read the image (and stored its part of the output)
         for (int j = wave; j < T64 / 8; j += 4) {
             const int row = j * 8 + cr;
