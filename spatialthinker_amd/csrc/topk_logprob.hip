@@ -2,7 +2,8 @@
 //
 //   ids = the k largest logits of a row in falling order (equal logits: the lower id first), logp = logit / temperature - lse,
 //   lse = log sum_v exp(logit_v / temperature)
-// Bound: HBM, 2 V bytes per row read once.
+// Bound: HBM, 2 V bytes per row read once (MI355X, 2048 rows of V = 152 064, k = 64: 134 us = 4.65 TB/s of the 6.8 that a read alone reaches, the rest
+// being the vector instructions of comparing, raising and summing 16-bit values; one row, k = 20: 8 us and 6 us more to join its slices).
 //
 // One workgroup walks a row (or a slice of it) in segments.  Every thread keeps the largest value it has met; the k-th largest of these
 // per-thread maxima is reached by at least k values, so whatever lies below it can be dropped: this threshold rises as the maxima grow and

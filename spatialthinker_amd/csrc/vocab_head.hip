@@ -65,6 +65,9 @@ __device__ __forceinline__ void vh_store_image(const char* smem, uint16_t* __res
 // from the tile's list of targets (head_bucket_kernel): from the same accumulators as the statistics, so that a target that is its row's maximum
 // has exactly the maximum's value.
 // DLOGITS: d[m][n] (bf16, pitch ldd, zero in columns [V, ldd) and rows [T, T64)).
+// Bound by the matrix pipe: the main loop is the four-wave tile of the framework's GEMM, and the epilogue has to cost little beside it.  MI355X,
+// V = 152 064, H = 3584: 4096 rows 3.05 ms = 1.46 PF/s with the join (the GEMM alone, writing logits, 3.15); 161 .. 256 rows, one row tile: 260 us
+// whatever their number, 4.2 TB/s of weights (2.3 rounds of 256 tiles: a last part round in narrower tiles was 0 to 8 % slower).
 // ------------------------------------------------------------------------------------------------------------------------------------
 template <bool DLOGITS, bool ONE_ROW_TILE>
 __global__ __launch_bounds__(256) void head_tile_kernel(const uint16_t* __restrict__ h, int64_t ldh, const uint16_t* __restrict__ w, int64_t ldw, int T,
@@ -370,7 +373,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t*
 }
 
 // (max, sum) partials -> lse (natural log), stat = (max, log2 sum); logp = label logit - lse for rows with a label inside the vocabulary, 0 for the others.
-// 16 rows x 64 slices per workgroup: 16 consecutive lanes read 128 contiguous bytes of one partial row.
+// 16 rows x 64 slices per workgroup: 16 consecutive lanes read 128 contiguous bytes of one partial row.  Bound: reading the partials, 8 B per row and
+// 128 columns (4096 rows, V = 152 064: 39 MB in 15 us).
 __global__ __launch_bounds__(1024) void head_lse_kernel(const float2* __restrict__ part, int n_parts, const float* __restrict__ zlab,
                                                        const int64_t* __restrict__ labels, float* __restrict__ logp, float* __restrict__ lse, float2* __restrict__ stat,
                                                        int T, int V) {
@@ -409,7 +413,7 @@ __global__ __launch_bounds__(1024) void head_lse_kernel(const float2* __restrict
     }
 }
 
-// the same for few rows, where reading the partials one behind the other is what takes the time: a workgroup per row
+// the same for few rows, where reading the partials one behind the other is what takes the time: a workgroup per row (up to 200 rows 4 to 6 us)
 __global__ __launch_bounds__(1024) void head_lse_few_kernel(const float2* __restrict__ part, int n_parts, const float* __restrict__ zlab,
                                                            const int64_t* __restrict__ labels, float* __restrict__ logp, float* __restrict__ lse,
                                                            float2* __restrict__ stat, int T, int V) {
@@ -490,7 +494,10 @@ __global__ __launch_bounds__(128) void head_rows_label_kernel(const uint16_t* __
     vh_pack_row(h, ldh, hz, hzt, TP, t, ri.hot != 0.f, sc, H);
 }
 
-// slab[s][m][n] (+)= sum over the K-slice s of d[m][:] w[:][n]: w is contraction-major as stored; `kv` of the ldd columns of d are vocabulary
+// slab[s][m][n] (+)= sum over the K-slice s of d[m][:] w[:][n]: w is contraction-major as stored; `kv` of the ldd columns of d are vocabulary.
+// On its own where there is one row tile (129 .. 256 rows) or no dW is asked for: the vocabulary is the long axis, so it is cut into slices that
+// fill the CUs in whole rounds, joined in slice order by head_dh_finish_kernel.  Bound: the weight stream through 256-row tiles (200 x 3584 x 152 064:
+// 259 us = 4.2 TB/s; 150 x 2048 x 151 936: 155 us = 4.0).
 template <bool ACCUM, bool ONE_ROW_TILE>
 __device__ __forceinline__ void head_dh_tile(char* smem, int block, const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ w, int64_t ldw,
                                              int T, int kv, int H, int tiles_m, int tiles_n, int split, float* __restrict__ slab) {
@@ -532,7 +539,8 @@ __global__ __launch_bounds__(256) void head_dh_kernel(const uint16_t* __restrict
 // The same for few rows (T <= 128): a stream of w, [32 vocabulary rows][256 columns] per step through SLOTS LDS slots, next to a [16 MT][32] tile of d
 // (rows beyond T: the last one, never stored).
 // w is contraction-major: its fragments are LDS transpose reads (image and swizzle as the contraction-major operands of gemm_asm4.hip).  Four
-// waves of 64 columns, all rows each; the vocabulary is cut into slices so that every CU has two workgroups.
+// waves of 64 columns, all rows each; the vocabulary is cut into slices so that every CU has two workgroups.  Bound: the weight stream (3584 x 152 064:
+// 16 rows 186 us = 5.9 TB/s, 128 rows 244 us = 4.5).
 template <int MT, int SLOTS, bool ACCUM>
 __global__ __launch_bounds__(256, 2) void head_dh_few_kernel(const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ w, int64_t ldw, int T,
                                                             int kv, int H, int tiles_n, int per, float* __restrict__ slab) {
@@ -622,7 +630,7 @@ __global__ __launch_bounds__(256, 2) void head_dh_few_kernel(const uint16_t* __r
     }
 }
 
-// dh = bf16(row scale * sum of the slabs, in slice order)
+// dh = bf16(row scale * sum of the slabs, in slice order).  Bound: the slabs (8192 x 3584, two of them: 235 MB read in 30 us, part of it from the caches)
 __global__ __launch_bounds__(256) void head_dh_finish_kernel(const float* __restrict__ slab, int split, const float* __restrict__ scale, uint16_t* __restrict__ dh, int64_t lddh, int T, int H) {
     const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= (int64_t)T * H) return;
@@ -638,7 +646,8 @@ __global__ __launch_bounds__(256) void head_dh_finish_kernel(const float* __rest
     *reinterpret_cast<uint2*>(dh + (i / H) * lddh + i % H) = o;
 }
 
-// dw[v][n] = sum_t d[t][v] hz[t][n]: both operands contraction-major as they lie in memory.  bf16 result, or fp32 (+=).
+// dw[v][n] = sum_t d[t][v] hz[t][n]: both operands contraction-major as they lie in memory.  bf16 result, or fp32 (+=).  Bound: the matrix pipe
+// (alone, where no dh is asked for: 4096 x 3584 x 152 064 3.6 ms = 1.24 PF/s).
 template <bool OUT_BF16, bool ACCUM>
 __device__ __forceinline__ void head_dw_tile(char* smem, int block, const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ hz, int T64,
                                              int kv, int H, int tiles_m, int tiles_n, uint16_t* __restrict__ dwb, float* __restrict__ dwf, int64_t lddw) {
@@ -690,7 +699,8 @@ __global__ __launch_bounds__(256) void head_dw_kernel(const uint16_t* __restrict
 }
 
 // Both gradients of a piece in one launch: the few long tiles of dh first, the many short ones of dw behind them fill the CUs up, where two launches
-// would each leave part of their last round idle (8192 x 3584, a piece of 30 464 columns: 448 and 1666 tiles on 256 CUs).
+// would each leave part of their last round idle (8192 x 3584, a piece of 30 464 columns: 448 and 1666 tiles on 256 CUs).  Bound: the matrix pipe (that
+// piece 2.55 ms = 1.40 PF/s; 1000 x 2048 x 151 936 1.05 ms = 1.19 PF/s).
 template <bool DW_BF16, bool DW_ACCUM, bool DH_ACCUM>
 __global__ __launch_bounds__(256) void head_grads_kernel(const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ w, int64_t ldw,
                                                         const uint16_t* __restrict__ hz, int T, int T64, int kv, int H, int tiles_t, int tiles_v, int tiles_h,
@@ -705,6 +715,7 @@ __global__ __launch_bounds__(256) void head_grads_kernel(const uint16_t* __restr
 // contiguous (dt[v][TP], hzt[n][TP]), so fragments come straight from memory: dt once per workgroup, hzt from the caches, a step ahead.  A
 // workgroup owns 128 vocabulary rows and walks the columns 256 at a time, 64 per wave; the bf16 tile goes through LDS, because a row has to leave in
 // long runs: 64-byte pieces of 16 rows at a pitch of H elements meet in a few cache channels (V = 152 064, H = 3584: 292 us against 160 for a fill).
+// With it 221 us at 16 rows = 4.9 TB/s written, 230 at 48, 265 at 128.
 template <int KS, bool OUT_BF16, bool ACCUM>
 __global__ __launch_bounds__(256) void head_dw_few_kernel(const uint16_t* __restrict__ dt, const uint16_t* __restrict__ hzt, int kv, int H,
                                                          uint16_t* __restrict__ dwb, float* __restrict__ dwf, int64_t lddw) {
@@ -783,6 +794,8 @@ __global__ __launch_bounds__(256) void head_dw_few_kernel(const uint16_t* __rest
 // come 64 columns at a time, [T64][64], through LDS for all four waves.  Both are contraction-major as they lie in memory, so fragments are LDS
 // transpose reads: image of 128-byte rows, 32-byte chunk c of row r at position c ^ f(r), f(r) = ((r >> 1) & 1) | ((r >> 3) & 1) << 1, which
 // gives the eight rows that a half wave touches eight places of the 256-byte bank row.  Two workgroups per CU: one stores while the other multiplies.
+// Bound: the write of dw and, next to it, the copies of hz that every workgroup repeats (200 x 3584 x 152 064 270 us = 4.0 TB/s written; 150 x 2048 x
+// 151 936 180 us = 3.5, 215 before each workgroup started at another column block).
 __device__ __forceinline__ void vh_tr_frag4(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, bf16x8 (&f)[4]) {
     union Frag { bf16x8 v; s16x4_t h[2]; } x[4];
     // reads and their wait in one statement; rows +4 .. +7 of a fragment lie 512 bytes on
@@ -957,6 +970,7 @@ __global__ __launch_bounds__(1024) void head_bucket_kernel(const int32_t* __rest
     }
 }
 
+// (The kernels of targets only, from here to head_sparse_kernel, take 4 to 15 us each up to 4096 x 64 targets: launches and latency.)
 // kl and log q of every row, one wave per row: logq[t][k] (in: z2 of the target, out: natural log q; 0 for absent entries)
 __global__ __launch_bounds__(256) void head_kl_kernel(const int32_t* __restrict__ ids, const float* __restrict__ a, int K, int renorm,
                                                      const float2* __restrict__ stat, float* __restrict__ logq, float* __restrict__ kl, int T, int V) {
