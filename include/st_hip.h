@@ -61,37 +61,41 @@ int st_logprob_bwd(st_bf16* logits, int64_t ldl, const int64_t* labels, const fl
 
 /* ---- vocabulary head without stored logits ----------------------------------------------------
  * The same log-probs (and a distillation loss) straight from the head's operands: hidden (T, H) bf16, weight (V, H) bf16, z = hidden .
- * weight^T * inv_temperature is formed tile by tile in fp32 and never stored; the logits of st_gemm_nt + st_logprob_fwd are rounded to bf16 and
+ * weight^T * inv_temperature is formed tile by tile in fp32 and not stored (or kept in fp32, see logits); the logits of st_gemm_nt + st_logprob_fwd are rounded to bf16 and
  * take 2 T V bytes.  Call sites they stand next to: verl/workers/actor/dp_actor.py:125-128 (logits / temperature, log_probs_from_logits) and
  * its backward :266-279.
  *   - H % 64 == 0; V <= 2^21; T * K < 2^31; ldh, ldw multiples of 8 below 2^22; hidden, weight, dweight_bf16, dweight_f32 16-byte, dhidden 8-byte aligned; T == 0 is
  *     allowed (dweight: zeros, or left as it is with accumulate).
  *   - workspace: st_linear_head_workspace_bytes(T, V, H, K (0 for labels), backward) bytes, 16-byte aligned, contents irrelevant.  Nothing is kept in it between
  *     calls: calls on several streams and captured graphs need one each.  backward != 0 covers any subset of the gradients.
+ *   - logits: NULL, or a (T, ldz >= V rounded up to 64) fp32 buffer, 16-byte aligned, ldz % 4 == 0, in which the forward leaves h . w (before the
+ *     temperature) for the backward of the same call; without it the backward forms them again, a piece of the vocabulary at a time.  Both ways
+ *     give the same bits.
  *   - the same inputs give the same bits. */
 int st_linear_head_workspace_bytes(int T, int V, int H, int K, int backward, int64_t* bytes_host, st_stream_t stream);
 /* logp[t] = z[t][labels[t]] - lse[t], lse[t] = log sum_v exp z[t][v].  A label outside [0, V) marks a row that is not scored: logp 0 (lse is
  * still written) and no gradient, whatever its hidden state and g hold. */
 int st_linear_logprob_fwd(const st_bf16* hidden, int64_t ldh, const st_bf16* weight, int64_t ldw, const int64_t* labels, float inv_temperature,
-                          float* logp, float* lse, void* workspace, int64_t workspace_bytes, int T, int V, int H, st_stream_t stream);
+                          float* logp, float* lse, float* logits, int64_t ldz, void* workspace, int64_t workspace_bytes, int T, int V, int H,
+                          st_stream_t stream);
 /* Gradients of sum_t g[t] logp[t] (logp, lse: what the forward wrote): dhidden (T, H) bf16 and / or dweight as bf16 (overwritten) or fp32 (accumulate: added to); NULL = not wanted.
  * The logit gradients pass through bf16, as operands of the two products; sums are fp32.  A row's scale may move into its hidden state, which then
  * passes through bf16 once more on the way to dweight. */
 int st_linear_logprob_bwd(const st_bf16* hidden, int64_t ldh, const st_bf16* weight, int64_t ldw, const int64_t* labels, const float* logp, const float* lse,
-                          const float* g, float inv_temperature, st_bf16* dhidden, int64_t lddh, st_bf16* dweight_bf16, float* dweight_f32, int64_t lddw, int accumulate,
-                          void* workspace, int64_t workspace_bytes, int T, int V, int H, st_stream_t stream);
+                          const float* g, float inv_temperature, const float* logits, int64_t ldz, st_bf16* dhidden, int64_t lddh, st_bf16* dweight_bf16,
+                          float* dweight_f32, int64_t lddw, int accumulate, void* workspace, int64_t workspace_bytes, int T, int V, int H, st_stream_t stream);
 /* Distillation from a teacher's K <= 1024 log-probs per row: ids (T, K) int32, teacher_logp (T, K) fp32, contiguous.
  *   kl[t] = sum_k p_k (log p_k - log q[ids_k]),  log q = z - lse,  p_k = exp(teacher_logp_k), or softmax over the row's entries if renormalize.
  * Entries with an id outside [0, V) are absent (their teacher_logp is not read as a number); a row without entries has kl 0 and no gradient.
  * An id may stand in a row more than once: its probabilities add up.  logq (T, K) fp32 is what the backward needs (0 at absent entries). */
 int st_linear_topk_kl_fwd(const st_bf16* hidden, int64_t ldh, const st_bf16* weight, int64_t ldw, const int32_t* ids, const float* teacher_logp, int K,
-                          int renormalize, float inv_temperature, float* kl, float* lse, float* logq, void* workspace, int64_t workspace_bytes, int T,
-                          int V, int H, st_stream_t stream);
+                          int renormalize, float inv_temperature, float* kl, float* lse, float* logq, float* logits, int64_t ldz, void* workspace,
+                          int64_t workspace_bytes, int T, int V, int H, st_stream_t stream);
 /* Gradients of sum_t g[t] kl[t] (none for the teacher): as st_linear_logprob_bwd. */
 int st_linear_topk_kl_bwd(const st_bf16* hidden, int64_t ldh, const st_bf16* weight, int64_t ldw, const int32_t* ids, const float* teacher_logp, int K,
-                          int renormalize, float inv_temperature, const float* lse, const float* logq, const float* g, st_bf16* dhidden, int64_t lddh,
-                          st_bf16* dweight_bf16, float* dweight_f32, int64_t lddw, int accumulate, void* workspace, int64_t workspace_bytes, int T, int V,
-                          int H, st_stream_t stream);
+                          int renormalize, float inv_temperature, const float* lse, const float* logq, const float* g, const float* logits, int64_t ldz,
+                          st_bf16* dhidden, int64_t lddh, st_bf16* dweight_bf16, float* dweight_f32, int64_t lddw, int accumulate, void* workspace,
+                          int64_t workspace_bytes, int T, int V, int H, st_stream_t stream);
 /* The k <= 256 largest log-probs of each row of logits (T, V) bf16 (any row pitch >= V, no alignment beyond 2 bytes): ids (T, k) int32 in falling
  * order, equal logits by rising id (-0 equals 0); logp (T, k) = logit * inv_temperature - lse; lse (T,) = log sum_v exp(logit_v * inv_temperature).
  * -inf logits are allowed (logp -inf); a row with NaN or +inf, or of -inf alone, has NaN log-probs and distinct ids inside [0, V).

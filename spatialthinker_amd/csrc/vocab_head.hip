@@ -1,15 +1,17 @@
-// vocab_head.hip — losses of the vocabulary head straight from the hidden states, for gfx950: no (rows x vocabulary) logits in memory.
+// vocab_head.hip — losses of the vocabulary head straight from the hidden states, for gfx950: (rows x vocabulary) logits only in fp32 and on request.
 //
 //   z[t][v] = (h_t . w_v) / temperature,   lse_t = log sum_v exp z[t][v]
 //   log-prob of given tokens:          logp_t = z[t][label_t] - lse_t
 //   distillation from top log-probs:   kl_t = sum_k p_tk (log p_tk - (z[t][id_tk] - lse_t)),  p from the teacher's k log-probs of the row
 // Both gradients have one form: d[t][v] = c_t exp(z[t][v] - lse_t) + (sparse targets), dh = d W, dW = d^T h, so both share every product:
 //   forward   head_tile_kernel<STATS>   z tile in registers -> per row (max, sum 2^(z - max)) of 128 columns; then head_lse_kernel
-//   backward  per piece of the vocabulary: head_tile_kernel<DLOGITS> recomputes the tile and writes d (bf16) into a bounded workspace,
-//             head_dh_kernel adds d W into fp32 slabs, head_dw_kernel writes d^T h
+//   backward  per piece of the vocabulary: head_tile_kernel<DLOGITS> forms the tile again and writes d (bf16) into a bounded workspace, or
+//             head_d_kernel writes it from kept logits; head_dh_kernel adds d W into fp32 slabs, head_dw_kernel writes d^T h
+// Kept logits cost the forward their write and save the backward one of its three products (forward + backward, 152 064 x 3584: 16 rows 745 -> 621 us,
+// 203 rows 1114 -> 883, 1501 rows 4893 -> 4113, 8192 rows 25 580 -> 21 100; 50 257 x 1024, 256 rows 188 -> 181) for 4 T V bytes: the caller chooses.
 // d is rounded to bf16 because it is the operand of two bf16 matrix products: half a bf16 step (2^-8 relative) per element, the size of the
 // rounding of the bf16 gradients themselves.  Logits, softmax statistics and every sum stay in fp32.
-// What bounds them: the matrix pipe (2 T V H flop forward, 6 T V H backward) from a few hundred rows on, the weight stream (2 V H bytes) below.
+// What bounds them: the matrix pipe (2 T V H flop forward, 4 or 6 T V H backward) from a few hundred rows on, the weight stream (2 V H bytes) below.
 #include "gemm_asm4_core.h"
 #include <algorithm>
 
@@ -64,16 +66,17 @@ __device__ __forceinline__ void vh_store_image(const char* smem, uint16_t* __res
 // STATS: part[tn*2 + wn][m] = (max, sum) in base 2 of the 128 columns of a wave; zlab[m] = the label's logit, or z2[m][k] = the logit of target k
 // from the tile's list of targets (head_bucket_kernel): from the same accumulators as the statistics, so that a target that is its row's maximum
 // has exactly the maximum's value.
+// KEEP: z[m][n] = h_m . w_n in fp32 as well, straight from the accumulators (64-byte runs; V = 152 064, H = 3584, 4096 rows: 416 us for 2.5 GB).
 // DLOGITS: d[m][n] (bf16, pitch ldd, zero in columns [V, ldd) and rows [T, T64)).
 // Bound by the matrix pipe: the main loop is the four-wave tile of the framework's GEMM, and the epilogue has to cost little beside it.  MI355X,
 // V = 152 064, H = 3584: 4096 rows 3.05 ms = 1.46 PF/s with the join (the GEMM alone, writing logits, 3.15); 161 .. 256 rows, one row tile: 260 us
 // whatever their number, 4.2 TB/s of weights (2.3 rounds of 256 tiles: a last part round in narrower tiles was 0 to 8 % slower).
 // ------------------------------------------------------------------------------------------------------------------------------------
-template <bool DLOGITS, bool ONE_ROW_TILE>
+template <bool DLOGITS, bool ONE_ROW_TILE, bool KEEP = false>
 __global__ __launch_bounds__(256) void head_tile_kernel(const uint16_t* __restrict__ h, int64_t ldh, const uint16_t* __restrict__ w, int64_t ldw, int T,
                                                        int V, int H, int tiles_m, int tiles_n, float sc, const int64_t* __restrict__ labels,
                                                        float2* __restrict__ part, float* __restrict__ zlab, VhTargets tg, const VhRow* __restrict__ rows, int v0,
-                                                       uint16_t* __restrict__ d, int64_t ldd, int T64) {
+                                                       uint16_t* __restrict__ d, int64_t ldd, int T64, float* __restrict__ z, int64_t ldz) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -82,10 +85,20 @@ __global__ __launch_bounds__(256) void head_tile_kernel(const uint16_t* __restri
     vh_tile(blockIdx.x, tiles_m, tiles_n, tm, tn);
     const int m0 = tm * A4_BM, n0 = tn * A4_BN;
     f32x4 acc[8][8];
-    a4_mainloop<false, false, false, 0, false, false, ONE_ROW_TILE>(smem, h, ldh, w, ldw, m0, n0, T, V, 0, H / 64, H, acc);
+    a4_mainloop<false, false, false, 0, false, KEEP, ONE_ROW_TILE>(smem, h, ldh, w, ldw, m0, n0, T, V, 0, H / 64, H, acc);
     const int col0 = n0 + wn * 128 + (lane >> 4) * 4;                // column of (ni, r): col0 + ni*16 + r
     const bool inside = n0 + A4_BN <= V;
     if constexpr (!DLOGITS) {
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int mi = 0; mi < 8; ++mi) {
+                const int m = m0 + wm * 128 + mi * 16 + (lane & 15);
+                if (m >= T) continue;
+#pragma unroll
+                for (int ni = 0; ni < 8; ++ni)
+                    if (col0 + ni * 16 < ldz) *reinterpret_cast<f32x4*>(z + (int64_t)m * ldz + col0 + ni * 16) = acc[ni][mi];
+            }
+        }
         const int e0 = tg.start ? tg.start[tm * (tiles_n + 1) + tn] : 0, e1 = tg.start ? tg.start[tm * (tiles_n + 1) + tn + 1] : 0;
         if (e1 > e0) {                                               // the tile through LDS, 128 columns (64 of each wave pair) at a time
 #pragma unroll
@@ -188,7 +201,7 @@ template <int MT, int SLOTS, int WAVES, bool DLOGITS>
 __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t* __restrict__ h, int64_t ldh, const uint16_t* __restrict__ w, int64_t ldw, int T, int V,
                                                          int H, float sc, const int64_t* __restrict__ labels, float2* __restrict__ part,
                                                          float* __restrict__ zlab, VhTargets tg, const VhRow* __restrict__ rows, int v0,
-                                                         uint16_t* __restrict__ d, int64_t ldd, uint16_t* __restrict__ dt, int TP) {
+                                                         uint16_t* __restrict__ d, int64_t ldd, uint16_t* __restrict__ dt, int TP, float* __restrict__ z, int64_t ldz) {
     constexpr int BT = 16 * MT, BN = 32 * WAVES, SLOT = (BN + BT) * 128, NT = 64 * WAVES;
     constexpr int HC = (2 * MT + WAVES - 1) / WAVES;                 // 1-KiB copies of h per wave and step (the last waves may copy some rows again)
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -260,6 +273,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t*
     const int col0 = n0 + wave * 32 + fk * 4;                        // column of (i, r): col0 + i*16 + r
     if constexpr (!DLOGITS) {
         constexpr int ROWB = 128 * 4 + 16;
+        if (z) {
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                if (j * 16 + fr >= T) continue;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (col0 + i * 16 < ldz) *reinterpret_cast<f32x4*>(z + (int64_t)(j * 16 + fr) * ldz + col0 + i * 16) = acc[i][j];
+            }
+        }
         const int e0 = tg.start ? tg.start[n0 >> 8] : 0, e1 = tg.start ? tg.start[(n0 >> 8) + 1] : 0;
         for (int p = 0; p < BN / 128 && e1 > e0; ++p) {              // the tile through LDS, 128 columns at a time
             if (wave >> 2 == p) {
@@ -368,6 +390,58 @@ __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t*
                 const int col = i / per, c = (i - col * per) * 8;
                 *reinterpret_cast<uint4*>(dt + (int64_t)(n0 + col) * TP + c) = c < BT ? *reinterpret_cast<const uint4*>(img_t + col * CB + c * 2) : make_uint4(0, 0, 0, 0);
             }
+        }
+    }
+}
+
+// d of a piece from the logits that the forward has kept: the epilogue of the tiles above, element by element with the same roundings.  64 rows x 128
+// columns per workgroup, eight columns per thread; FEW: also dt.  Bound: 4 B read and 2 B (FEW: 4 B) written per value
+// (4096 x 152 064: 690 us = 5.4 TB/s; 48 rows 19 us).
+template <bool FEW>
+__global__ __launch_bounds__(256) void head_d_kernel(const float* __restrict__ z, int64_t ldz, const VhRow* __restrict__ rows, int T, int V, float sc, int v0,
+                                                     uint16_t* __restrict__ d, int64_t ldd, int T64, uint16_t* __restrict__ dt, int TP) {
+    constexpr int CB = 64 * 2 + 16;
+    __shared__ __attribute__((aligned(16))) char img[FEW ? 128 * CB : 16];
+    const int n0 = blockIdx.x * 128, r0 = blockIdx.y * 64, c = (threadIdx.x & 15) * 8, rr = threadIdx.x >> 4;
+    const bool in = n0 + c < ldd;
+    f32x4 v[4][2];
+    VhRow ri[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int m = r0 + i * 16 + rr;
+        ri[i] = {0.f, 0.f, 0.f, -1};
+        v[i][0] = v[i][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        if (m < T && in) {
+            ri[i] = rows[m];
+            v[i][0] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(z + (int64_t)m * ldz + n0 + c));
+            v[i][1] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(z + (int64_t)m * ldz + n0 + c + 4));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int m = r0 + i * 16 + rr, lab = ri[i].label - v0 - n0 - c;
+        const bool live = ri[i].c != 0.f || ri[i].hot != 0.f;
+        float o[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            float x = ri[i].c * vh_exp2(fmaf(v[i][k >> 2][k & 3], sc, -ri[i].lse2));
+            if (lab == k) x = ri[i].hot;
+            o[k] = live && n0 + c + k < V ? x : 0.f;
+        }
+        uint4 pk;
+        pk.x = f2bf2(o[0], o[1]); pk.y = f2bf2(o[2], o[3]); pk.z = f2bf2(o[4], o[5]); pk.w = f2bf2(o[6], o[7]);
+        if (in && m < (FEW ? T : T64)) *reinterpret_cast<uint4*>(d + (int64_t)m * ldd + n0 + c) = pk;
+        if constexpr (FEW) {
+            const uint32_t u[4] = {pk.x, pk.y, pk.z, pk.w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) *reinterpret_cast<uint16_t*>(img + (c + k) * CB + (i * 16 + rr) * 2) = (uint16_t)(u[k >> 1] >> ((k & 1) * 16));
+        }
+    }
+    if constexpr (FEW) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < 128 * 8; i += 256) {
+            const int col = i >> 3, r = (i & 7) * 8;
+            if (n0 + col < ldd && r0 + r < TP) *reinterpret_cast<uint4*>(dt + (int64_t)(n0 + col) * TP + r0 + r) = *reinterpret_cast<const uint4*>(img + col * CB + r * 2);
         }
     }
 }
@@ -1149,7 +1223,7 @@ int launch_few(int T, int V, hipStream_t s, A... args) {
 }
 
 int head_stats(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, const int64_t* labels, float sc, float* logp, float* lse, VhTargets tg,
-               char* ws, const Plan& p, int T, int V, int H, hipStream_t s) {
+               float* z, int64_t ldz, char* ws, const Plan& p, int T, int V, int H, hipStream_t s) {
     const int tm = st_cdiv(T, 256), tn = st_cdiv(V, 256);
     float2* part = (float2*)(ws + p.part);
     float* zlab = (float*)(ws + p.zlab);
@@ -1157,15 +1231,17 @@ int head_stats(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, c
     if (T <= VH_STREAM) {
         n_parts = st_cdiv(V, few_cols(T));
         const int rc = launch_few<false>(T, V, s, h, ldh, w, ldw, T, V, H, sc, labels, part, zlab, tg, (const VhRow*)nullptr, 0, (uint16_t*)nullptr,
-                                         (int64_t)0, (uint16_t*)nullptr, 0);
+                                         (int64_t)0, (uint16_t*)nullptr, 0, z, ldz);
         if (rc) return rc;
     } else {
         auto go = [&](auto kern) {
             hipLaunchKernelGGL(kern, dim3(tm * tn), dim3(256), VH_SMEM, s, h, ldh, w, ldw, T, V, H, tm, tn, sc, labels, part, zlab, tg,
-                               (const VhRow*)nullptr, 0, (uint16_t*)nullptr, (int64_t)0, 0);
+                               (const VhRow*)nullptr, 0, (uint16_t*)nullptr, (int64_t)0, 0, z, ldz);
         };
         allow_lds<head_tile_kernel<false, true>>(); allow_lds<head_tile_kernel<false, false>>();
-        if (tm == 1) go(head_tile_kernel<false, true>); else go(head_tile_kernel<false, false>);
+        allow_lds<head_tile_kernel<false, true, true>>(); allow_lds<head_tile_kernel<false, false, true>>();
+        if (z) { if (tm == 1) go(head_tile_kernel<false, true, true>); else go(head_tile_kernel<false, false, true>); }
+        else if (tm == 1) go(head_tile_kernel<false, true>); else go(head_tile_kernel<false, false>);
         ST_CHECK_LAUNCH();
     }
     if (T <= 512) hipLaunchKernelGGL(head_lse_few_kernel, dim3(T), dim3(1024), 0, s, part, n_parts, zlab, labels, logp, lse, (float2*)(ws + p.stat), T, V);
@@ -1194,7 +1270,7 @@ int launch_dh_few(const uint16_t* d, int64_t ldd, const uint16_t* w, int64_t ldw
 
 // the pieces of a backward pass behind the row coefficients; `sparse` finishes d at the targets of a piece
 template <class F>
-int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, float sc, uint16_t* dh, int64_t lddh, uint16_t* dwb, float* dwf,
+int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, float sc, const float* z, int64_t ldz, uint16_t* dh, int64_t lddh, uint16_t* dwb, float* dwf,
                   int64_t lddw, int accumulate, char* ws, const Plan& p, int T, int V, int H, hipStream_t s, F&& sparse) {
     const VhRow* rows = (const VhRow*)(ws + p.rows);
     const uint16_t* hz = (const uint16_t*)(ws + p.hz);
@@ -1216,14 +1292,19 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
         const int v0 = i * p.piece, kv = std::min(p.piece, V - v0), tn = st_cdiv(kv, 256);
         const int64_t ldd = up(kv, 64);
         const uint16_t* wp = w + (int64_t)v0 * ldw;
-        if (T <= VH_STREAM) {
+        if (z) {
+            const dim3 grid(st_cdiv(ldd, 128), p.T64 / 64);
+            if (p.few) hipLaunchKernelGGL(head_d_kernel<true>, grid, dim3(256), 0, s, z + v0, ldz, rows, T, kv, sc, v0, d, ldd, p.T64, dt, p.TP);
+            else hipLaunchKernelGGL(head_d_kernel<false>, grid, dim3(256), 0, s, z + v0, ldz, rows, T, kv, sc, v0, d, ldd, p.T64, dt, p.TP);
+            ST_CHECK_LAUNCH();
+        } else if (T <= VH_STREAM) {
             const int rc = launch_few<true>(T, kv, s, h, ldh, wp, ldw, T, kv, H, sc, (const int64_t*)nullptr, (float2*)nullptr, (float*)nullptr,
-                                            VhTargets{}, rows, v0, d, ldd, dt, p.few ? p.TP : p.T64);
+                                            VhTargets{}, rows, v0, d, ldd, dt, p.few ? p.TP : p.T64, (float*)nullptr, (int64_t)0);
             if (rc) return rc;
         } else {
             auto go = [&](auto kern) {
                 hipLaunchKernelGGL(kern, dim3(tm * tn), dim3(256), VH_SMEM, s, h, ldh, wp, ldw, T, kv, H, tm, tn, sc, (const int64_t*)nullptr,
-                                   (float2*)nullptr, (float*)nullptr, VhTargets{}, rows, v0, d, ldd, p.T64);
+                                   (float2*)nullptr, (float*)nullptr, VhTargets{}, rows, v0, d, ldd, p.T64, (float*)nullptr, (int64_t)0);
             };
             if (tm == 1) go(head_tile_kernel<true, true>); else go(head_tile_kernel<true, false>);
             ST_CHECK_LAUNCH();
@@ -1294,6 +1375,8 @@ bool grads_ok(const void* dh, int64_t lddh, const void* dwb, const void* dwf, in
     return true;
 }
 
+bool logits_ok(const float* z, int64_t ldz, int V) { return !z || (!(((uintptr_t)z) & 15) && !(ldz & 3) && ldz >= up(V, 64)); }
+
 // no rows: dW is a sum over nothing
 int empty_dw(uint16_t* dwb, float* dwf, int64_t lddw, int accumulate, int V, int H, hipStream_t s) {
     if (accumulate || (!dwb && !dwf)) return 0;
@@ -1315,38 +1398,39 @@ int st_linear_head_workspace_bytes(int T, int V, int H, int K, int backward, int
 }
 
 int st_linear_logprob_fwd(const st_bf16* hidden, int64_t ldh, const st_bf16* weight, int64_t ldw, const int64_t* labels, float inv_temperature,
-                          float* logp, float* lse, void* workspace, int64_t workspace_bytes, int T, int V, int H, st_stream_t stream) {
+                          float* logp, float* lse, float* logits, int64_t ldz, void* workspace, int64_t workspace_bytes, int T, int V, int H,
+                          st_stream_t stream) {
     if (T == 0) return V > 0 && H > 0 && H % 64 == 0 ? 0 : ST_EINVAL;
-    if (!operands_ok(hidden, ldh, weight, ldw, T, V, H, inv_temperature) || !labels || !logp || !lse) return ST_EINVAL;
+    if (!operands_ok(hidden, ldh, weight, ldw, T, V, H, inv_temperature) || !labels || !logp || !lse || !logits_ok(logits, ldz, V)) return ST_EINVAL;
     const Plan p = head_plan(T, V, H, 0);
     if (!workspace || workspace_bytes < p.fwd_bytes) return ST_EINVAL;
-    return head_stats(hidden, ldh, weight, ldw, labels, inv_temperature * VH_LOG2E, logp, lse, VhTargets{}, (char*)workspace, p, T, V, H,
+    return head_stats(hidden, ldh, weight, ldw, labels, inv_temperature * VH_LOG2E, logp, lse, VhTargets{}, logits, ldz, (char*)workspace, p, T, V, H,
                       (hipStream_t)stream);
 }
 
 int st_linear_logprob_bwd(const st_bf16* hidden, int64_t ldh, const st_bf16* weight, int64_t ldw, const int64_t* labels, const float* logp, const float* lse,
-                          const float* g, float inv_temperature, st_bf16* dhidden, int64_t lddh, st_bf16* dweight_bf16, float* dweight_f32, int64_t lddw, int accumulate,
-                          void* workspace, int64_t workspace_bytes, int T, int V, int H, st_stream_t stream) {
+                          const float* g, float inv_temperature, const float* logits, int64_t ldz, st_bf16* dhidden, int64_t lddh, st_bf16* dweight_bf16,
+                          float* dweight_f32, int64_t lddw, int accumulate, void* workspace, int64_t workspace_bytes, int T, int V, int H, st_stream_t stream) {
     hipStream_t s = (hipStream_t)stream;
     if (V <= 0 || H <= 0 || H % 64 || T < 0 || !grads_ok(dhidden, lddh, dweight_bf16, dweight_f32, lddw, accumulate, H)) return ST_EINVAL;
     if (T == 0) return empty_dw(dweight_bf16, dweight_f32, lddw, accumulate, V, H, s);
-    if (!operands_ok(hidden, ldh, weight, ldw, T, V, H, inv_temperature) || !labels || !logp || !lse || !g) return ST_EINVAL;
+    if (!operands_ok(hidden, ldh, weight, ldw, T, V, H, inv_temperature) || !labels || !logp || !lse || !g || !logits_ok(logits, ldz, V)) return ST_EINVAL;
     const Plan p = head_plan(T, V, H, 0);
     if (!workspace || workspace_bytes < p.bwd_bytes) return ST_EINVAL;
     char* ws = (char*)workspace;
     hipLaunchKernelGGL(head_rows_label_kernel, dim3(p.few ? p.TP : p.T64), dim3(128), 0, s, hidden, ldh, labels, logp, lse, g, inv_temperature, (VhRow*)(ws + p.rows),
                        (float*)(ws + p.scale), p.few ? nullptr : (uint16_t*)(ws + p.hz), (uint16_t*)(ws + p.hzt), p.TP, T, V, H);
     ST_CHECK_LAUNCH();
-    return head_backward(hidden, ldh, weight, ldw, inv_temperature * VH_LOG2E, dhidden, lddh, dweight_bf16, dweight_f32, lddw, accumulate, ws, p, T, V, H, s,
+    return head_backward(hidden, ldh, weight, ldw, inv_temperature * VH_LOG2E, logits, ldz, dhidden, lddh, dweight_bf16, dweight_f32, lddw, accumulate, ws, p, T, V, H, s,
                          [](int, int, uint16_t*, int64_t, uint16_t*) { return 0; });
 }
 
 int st_linear_topk_kl_fwd(const st_bf16* hidden, int64_t ldh, const st_bf16* weight, int64_t ldw, const int32_t* ids, const float* teacher_logp, int K,
-                          int renormalize, float inv_temperature, float* kl, float* lse, float* logq, void* workspace, int64_t workspace_bytes, int T,
-                          int V, int H, st_stream_t stream) {
+                          int renormalize, float inv_temperature, float* kl, float* lse, float* logq, float* logits, int64_t ldz, void* workspace,
+                          int64_t workspace_bytes, int T, int V, int H, st_stream_t stream) {
     if (K <= 0 || K > VH_MAX_K || (int64_t)T * K > INT32_MAX) return ST_EINVAL;
     if (T == 0) return V > 0 && H > 0 && H % 64 == 0 ? 0 : ST_EINVAL;
-    if (!operands_ok(hidden, ldh, weight, ldw, T, V, H, inv_temperature) || !ids || !teacher_logp || !kl || !lse || !logq) return ST_EINVAL;
+    if (!operands_ok(hidden, ldh, weight, ldw, T, V, H, inv_temperature) || !ids || !teacher_logp || !kl || !lse || !logq || !logits_ok(logits, ldz, V)) return ST_EINVAL;
     const Plan p = head_plan(T, V, H, K);
     if (!workspace || workspace_bytes < p.fwd_bytes) return ST_EINVAL;
     hipStream_t s = (hipStream_t)stream;
@@ -1357,7 +1441,7 @@ int st_linear_topk_kl_fwd(const st_bf16* hidden, int64_t ldh, const st_bf16* wei
     const int tn = st_cdiv(V, 256);
     hipLaunchKernelGGL(head_bucket_kernel, dim3(st_cdiv(T, 256)), dim3(1024), (tn + 16) * 4, s, ids, K, start, list, logq, T, V, tn);
     ST_CHECK_LAUNCH();
-    const int rc = head_stats(hidden, ldh, weight, ldw, nullptr, sc, nullptr, lse, VhTargets{start, list, logq, K}, ws, p, T, V, H, s);
+    const int rc = head_stats(hidden, ldh, weight, ldw, nullptr, sc, nullptr, lse, VhTargets{start, list, logq, K}, logits, ldz, ws, p, T, V, H, s);
     if (rc) return rc;
     hipLaunchKernelGGL(head_kl_kernel, dim3(st_cdiv(T, 4)), dim3(256), 0, s, ids, teacher_logp, K, renormalize,
                        (const float2*)(ws + p.stat), logq, kl, T, V);
@@ -1366,21 +1450,21 @@ int st_linear_topk_kl_fwd(const st_bf16* hidden, int64_t ldh, const st_bf16* wei
 }
 
 int st_linear_topk_kl_bwd(const st_bf16* hidden, int64_t ldh, const st_bf16* weight, int64_t ldw, const int32_t* ids, const float* teacher_logp, int K,
-                          int renormalize, float inv_temperature, const float* lse, const float* logq, const float* g, st_bf16* dhidden, int64_t lddh,
-                          st_bf16* dweight_bf16, float* dweight_f32, int64_t lddw, int accumulate, void* workspace, int64_t workspace_bytes, int T, int V,
-                          int H, st_stream_t stream) {
+                          int renormalize, float inv_temperature, const float* lse, const float* logq, const float* g, const float* logits, int64_t ldz,
+                          st_bf16* dhidden, int64_t lddh, st_bf16* dweight_bf16, float* dweight_f32, int64_t lddw, int accumulate, void* workspace,
+                          int64_t workspace_bytes, int T, int V, int H, st_stream_t stream) {
     hipStream_t s = (hipStream_t)stream;
     if (K <= 0 || K > VH_MAX_K || V <= 0 || H <= 0 || H % 64 || T < 0 || !grads_ok(dhidden, lddh, dweight_bf16, dweight_f32, lddw, accumulate, H))
         return ST_EINVAL;
     if (T == 0) return empty_dw(dweight_bf16, dweight_f32, lddw, accumulate, V, H, s);
-    if (!operands_ok(hidden, ldh, weight, ldw, T, V, H, inv_temperature) || !ids || !teacher_logp || !lse || !logq || !g) return ST_EINVAL;
+    if (!operands_ok(hidden, ldh, weight, ldw, T, V, H, inv_temperature) || !ids || !teacher_logp || !lse || !logq || !g || !logits_ok(logits, ldz, V)) return ST_EINVAL;
     const Plan p = head_plan(T, V, H, 0);
     if (!workspace || workspace_bytes < p.bwd_bytes) return ST_EINVAL;
     char* ws = (char*)workspace;
     hipLaunchKernelGGL(head_rows_kl_kernel, dim3(p.few ? p.TP : p.T64), dim3(128), 0, s, hidden, ldh, ids, teacher_logp, K, renormalize, lse, logq, g, inv_temperature,
                        (VhRow*)(ws + p.rows), (float*)(ws + p.scale), p.few ? nullptr : (uint16_t*)(ws + p.hz), (uint16_t*)(ws + p.hzt), p.TP, T, V, H);
     ST_CHECK_LAUNCH();
-    return head_backward(hidden, ldh, weight, ldw, inv_temperature * VH_LOG2E, dhidden, lddh, dweight_bf16, dweight_f32, lddw, accumulate, ws, p, T, V, H, s,
+    return head_backward(hidden, ldh, weight, ldw, inv_temperature * VH_LOG2E, logits, ldz, dhidden, lddh, dweight_bf16, dweight_f32, lddw, accumulate, ws, p, T, V, H, s,
                          [&](int v0, int kv, uint16_t* d, int64_t ldd, uint16_t* dt) -> int {
                              hipLaunchKernelGGL(head_sparse_kernel, dim3(st_cdiv(T, 4)), dim3(256), 0, s, ids, teacher_logp, K, renormalize, logq,
                                                 (const VhRow*)(ws + p.rows), v0, kv, d, ldd, dt, p.TP, T, V);

@@ -201,33 +201,54 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def linear_logprob_fwd(hidden, weight, labels, temperature: float = 1.0):
+def head_logits_buffer(T, V, device):
+    """The fp32 buffer in which linear_logprob_fwd / linear_topk_kl_fwd keep a call's logits for its backward."""
+    return torch.empty(T, (V + 63) // 64 * 64, dtype=F32, device=device)
+
+
+def _kept_logits(logits, T, V, device):
+    """-> (pointer, row pitch) of an optional kept-logits buffer."""
+    if logits is None or T == 0:
+        return None, 0
+    _chk(logits, F32, "logits")
+    if logits.device != device or logits.dim() != 2 or logits.shape[0] != T or logits.shape[1] < (V + 63) // 64 * 64:
+        raise ValueError(f"logits: expected ({T}, >= {(V + 63) // 64 * 64}) on {device}, got {tuple(logits.shape)} on {logits.device}")
+    ldz = logits.stride(0) if T > 1 else logits.shape[1]
+    if ldz < logits.shape[1] or ldz % 4 or logits.data_ptr() % 16:
+        raise ValueError("logits: rows must not overlap and start at 16-byte boundaries")
+    return logits.data_ptr(), ldz
+
+
+def linear_logprob_fwd(hidden, weight, labels, temperature: float = 1.0, logits=None):
     """hidden (T,H) bf16, weight (V,H) bf16, labels (T,) int64 -> (logp (T,) f32, lse (T,) f32) of z = hidden @ weight^T / temperature, whose
-    logits are never stored.  Labels outside [0, V): rows that are not scored (logp 0)."""
+    logits are not stored, or kept in `logits` (head_logits_buffer) for the backward.  Labels outside [0, V): rows that are not scored (logp 0)."""
     T, V, H, ldh, ldw = _head_operands(hidden, weight, temperature)
     dev = hidden.device
     _vec(labels, I64, (T,), dev, "labels")
     with _current(dev):
         logp = torch.empty(T, dtype=F32, device=dev)
         lse = torch.empty(T, dtype=F32, device=dev)
+        z, ldz = _kept_logits(logits, T, V, dev)
         if T:
             ws = _head_workspace(T, V, H, 0, 0, dev)
             lib().st_linear_logprob_fwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, labels.data_ptr(), 1.0 / temperature, logp.data_ptr(), lse.data_ptr(),
-                                        ws.data_ptr(), ws.numel(), T, V, H, torch._C._cuda_getCurrentRawStream(dev.index))
+                                        z, ldz, ws.data_ptr(), ws.numel(), T, V, H, torch._C._cuda_getCurrentRawStream(dev.index))
     return logp, lse
 
 
-def linear_logprob_bwd(hidden, weight, labels, logp, lse, g, temperature: float = 1.0, *, want_dhidden=True, dweight=None, dweight_f32=None, accumulate=False):
+def linear_logprob_bwd(hidden, weight, labels, logp, lse, g, temperature: float = 1.0, *, want_dhidden=True, dweight=None, dweight_f32=None, accumulate=False,
+                       logits=None):
     """Gradients of sum(g * logp): returns dhidden (T,H) bf16 (None unless wanted); dweight (bf16, overwritten) or dweight_f32 (fp32, accumulate:
-    added to) is filled in place."""
+    added to) is filled in place.  logits: what the forward kept, or None: formed again."""
     T, V, H, ldh, ldw = _head_operands(hidden, weight, temperature)
     dev = hidden.device
     _vec(labels, I64, (T,), dev, "labels"); _vec(logp, F32, (T,), dev, "logp"); _vec(lse, F32, (T,), dev, "lse"); _vec(g, F32, (T,), dev, "g")
     with _current(dev):
         dh, lddw = _head_grads(hidden, weight, want_dhidden, dweight, dweight_f32, accumulate)
+        z, ldz = _kept_logits(logits, T, V, dev)
         ws = _head_workspace(T, V, H, 0, 1, dev)
         lib().st_linear_logprob_bwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, labels.data_ptr(), logp.data_ptr(), lse.data_ptr(), g.data_ptr(),
-                                    1.0 / temperature, _ptr(dh), H, _ptr(dweight), _ptr(dweight_f32), lddw, int(accumulate), ws.data_ptr(), ws.numel(),
+                                    1.0 / temperature, z, ldz, _ptr(dh), H, _ptr(dweight), _ptr(dweight_f32), lddw, int(accumulate), ws.data_ptr(), ws.numel(),
                                     T, V, H, torch._C._cuda_getCurrentRawStream(dev.index))
     return dh
 
@@ -241,9 +262,10 @@ def _topk_targets(hidden, ids, teacher_logp, T):
     return ids.shape[1]
 
 
-def linear_topk_kl_fwd(hidden, weight, ids, teacher_logp, temperature: float = 1.0, renormalize: bool = False):
+def linear_topk_kl_fwd(hidden, weight, ids, teacher_logp, temperature: float = 1.0, renormalize: bool = False, logits=None):
     """ids (T,K) int32, teacher_logp (T,K) f32 -> (kl (T,) f32, lse (T,) f32, logq (T,K) f32): kl = sum_k p_k (log p_k - log q[ids_k]) with
-    p = exp(teacher_logp), or its softmax over the row's entries; entries with an id outside [0, V) are absent (st_linear_topk_kl_fwd)."""
+    p = exp(teacher_logp), or its softmax over the row's entries; entries with an id outside [0, V) are absent (st_linear_topk_kl_fwd).
+    logits: as linear_logprob_fwd."""
     T, V, H, ldh, ldw = _head_operands(hidden, weight, temperature)
     K = _topk_targets(hidden, ids, teacher_logp, T)
     dev = hidden.device
@@ -251,26 +273,28 @@ def linear_topk_kl_fwd(hidden, weight, ids, teacher_logp, temperature: float = 1
         kl = torch.empty(T, dtype=F32, device=dev)
         lse = torch.empty(T, dtype=F32, device=dev)
         logq = torch.empty(T, K, dtype=F32, device=dev)
+        z, ldz = _kept_logits(logits, T, V, dev)
         if T:
             ws = _head_workspace(T, V, H, K, 0, dev)
             lib().st_linear_topk_kl_fwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, ids.data_ptr(), teacher_logp.data_ptr(), K, int(renormalize),
-                                        1.0 / temperature, kl.data_ptr(), lse.data_ptr(), logq.data_ptr(), ws.data_ptr(), ws.numel(), T, V, H,
+                                        1.0 / temperature, kl.data_ptr(), lse.data_ptr(), logq.data_ptr(), z, ldz, ws.data_ptr(), ws.numel(), T, V, H,
                                         torch._C._cuda_getCurrentRawStream(dev.index))
     return kl, lse, logq
 
 
 def linear_topk_kl_bwd(hidden, weight, ids, teacher_logp, lse, logq, g, temperature: float = 1.0, renormalize: bool = False, *, want_dhidden=True,
-                       dweight=None, dweight_f32=None, accumulate=False):
-    """Gradients of sum(g * kl); outputs as linear_logprob_bwd."""
+                       dweight=None, dweight_f32=None, accumulate=False, logits=None):
+    """Gradients of sum(g * kl); outputs and logits as linear_logprob_bwd."""
     T, V, H, ldh, ldw = _head_operands(hidden, weight, temperature)
     K = _topk_targets(hidden, ids, teacher_logp, T)
     dev = hidden.device
     _vec(lse, F32, (T,), dev, "lse"); _vec(logq, F32, (T, K), dev, "logq"); _vec(g, F32, (T,), dev, "g")
     with _current(dev):
         dh, lddw = _head_grads(hidden, weight, want_dhidden, dweight, dweight_f32, accumulate)
+        z, ldz = _kept_logits(logits, T, V, dev)
         ws = _head_workspace(T, V, H, K, 1, dev)
         lib().st_linear_topk_kl_bwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, ids.data_ptr(), teacher_logp.data_ptr(), K, int(renormalize),
-                                    1.0 / temperature, lse.data_ptr(), logq.data_ptr(), g.data_ptr(), _ptr(dh), H, _ptr(dweight), _ptr(dweight_f32), lddw,
+                                    1.0 / temperature, lse.data_ptr(), logq.data_ptr(), g.data_ptr(), z, ldz, _ptr(dh), H, _ptr(dweight), _ptr(dweight_f32), lddw,
                                     int(accumulate), ws.data_ptr(), ws.numel(), T, V, H, torch._C._cuda_getCurrentRawStream(dev.index))
     return dh
 

@@ -222,6 +222,68 @@ def test_row_tiles_of_the_weight_stream(T, H):
     test_linear_topk_kl_forward_and_gradients(T, H, 519, 40, 1.0, True)
 
 
+@pytest.mark.parametrize("T,V", [(1, 5), (31, 333), (33, 257), (64, 1000), (96, 701), (128, 640), (129, 701), (160, 4001), (161, 999), (256, 700), (257, 1111), (700, 3000)])
+def test_kept_logits_give_the_same_bits(T, V):
+    """Logits read back and logits formed again: outputs and gradients are equal, and only what has to be kept is allocated."""
+    from verl.utils import torch_functional as VF
+    H, K = 192, 7
+    g, h, w, lab, gr = make(T, H, V, T + V)
+    lab[torch.rand(T, device="cuda", generator=g) < 0.2] = -100
+    h[lab < 0] = float("nan")
+    ids = torch.randint(0, V, (T, K), device="cuda", generator=g)
+    ids[lab < 0] = -1
+    a = torch.log_softmax(torch.randn(T, K, device="cuda", generator=g), 1)
+    for fn in (lambda x, y, keep: VF.linear_log_probs(x, y, lab, 0.7, keep_logits=keep), lambda x, y, keep: VF.linear_topk_kl(x, y, ids, a, 0.7, True, keep_logits=keep)):
+        outs = []
+        need = T * ((V + 63) // 64 * 64) * 4
+        for keep in (0, need - 1, need, 8 << 30):
+            hh, ww = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+            out = fn(hh, ww, keep)
+            assert (out.grad_fn.saved_tensors[-1] is not None) == (keep >= need)
+            outs.append((out.detach(),) + torch.autograd.grad(out, (hh, ww), gr))
+            with pytest.raises(RuntimeError):                      # what was kept went with the backward
+                out.grad_fn.saved_tensors
+        live = lab >= 0
+        for o in outs[1:]:
+            assert torch.equal(o[0][live], outs[0][0][live]) and torch.equal(o[1], outs[0][1]) and torch.equal(o[2], outs[0][2])
+        assert torch.isfinite(outs[0][1]).all() and torch.isfinite(outs[0][2]).all()
+        with torch.no_grad():
+            assert torch.equal(fn(h, w, 8 << 30)[live], outs[0][0][live])
+
+
+def test_kept_logits_of_several_pieces_and_in_a_captured_graph():
+    from spatialthinker_amd import ops
+    from verl.utils import torch_functional as VF
+    T, H, V = 2100, 64, 150001
+    g, h, w, lab, gr = make(T, H, V, 5)
+    outs = []
+    for keep in (0, 1 << 31):
+        hh, ww = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        lp = VF.linear_log_probs(hh, ww, lab, keep_logits=keep)
+        outs.append((lp,) + torch.autograd.grad(lp, (hh, ww), gr))
+    assert all(torch.equal(x, y) for x, y in zip(*outs))
+    del outs
+    T, V = 150, 3000
+    g, h, w, lab, gr = make(T, H, V, 6)
+
+    def step():
+        z = ops.head_logits_buffer(T, V, h.device)
+        logp, lse = ops.linear_logprob_fwd(h, w, lab, logits=z)
+        dw = torch.empty_like(w)
+        return logp, ops.linear_logprob_bwd(h, w, lab, logp, lse, gr, dweight=dw, logits=z), dw
+    step()
+    torch.cuda.synchronize()
+    gph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gph):
+        out = step()
+    for _ in range(3):
+        h.copy_(torch.randn(T, H, device="cuda", generator=g).to(BF16))
+        want = [t.clone() for t in step()]
+        gph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, want))
+
+
 def test_gradients_against_differences():
     """Central differences along random directions: <dh, h+ - h-> against the change of sum(g out), for steps that bf16 holds exactly.  The third-order
     rest of a difference of width e |h| (logits move by < 0.03) is below 1e-4 of the change's scale; 2 % covers it, the bf16 gradients (2^-8 per

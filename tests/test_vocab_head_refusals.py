@@ -82,19 +82,34 @@ def test_c_entries_return_einval_before_any_launch():
     for T, V, H, K in ((-1, 10, 64, 0), (8, 0, 64, 0), (8, 10, 0, 0), (8, 10, 65, 0), (8, 10, 64, 1025), (8, 10, 64, -1), (8, (1 << 21) + 1, 64, 0)):
         assert L.st_linear_head_workspace_bytes.raw(T, V, H, K, 1, at, None) == -22
     p = 1 << 20                                                    # never touched: every call below is refused
-    fwd = lambda h=p, ldh=64, w=p, ldw=64, lab=p, it=1.0, ws=p, nb=1 << 40, T=8, V=1000, H=64: L.st_linear_logprob_fwd.raw(
-        h, ldh, w, ldw, lab, it, p, p, ws, nb, T, V, H, None)
+    fwd = lambda h=p, ldh=64, w=p, ldw=64, lab=p, it=1.0, ws=p, nb=1 << 40, T=8, V=1000, H=64, z=None, ldz=0: L.st_linear_logprob_fwd.raw(
+        h, ldh, w, ldw, lab, it, p, p, z, ldz, ws, nb, T, V, H, None)
     for bad in (dict(h=None), dict(w=None), dict(lab=None), dict(ldh=63), dict(ldw=68), dict(ldh=56), dict(ldw=1 << 22), dict(h=p + 2), dict(w=p + 8),
-                dict(it=0.0), dict(it=-1.0), dict(it=math.inf), dict(it=math.nan), dict(ws=None), dict(nb=small // 1000), dict(T=-1), dict(V=0), dict(H=65)):
+                dict(it=0.0), dict(it=-1.0), dict(it=math.inf), dict(it=math.nan), dict(ws=None), dict(nb=small // 1000), dict(T=-1), dict(V=0), dict(H=65),
+                dict(z=p + 4, ldz=1024), dict(z=p, ldz=1023), dict(z=p, ldz=1022), dict(z=p, ldz=1020)):
         assert fwd(**bad) == -22, bad
-    bwd = lambda dh=p, lddh=64, db=None, df=None, lddw=64, acc=0, ws=p, nb=1 << 40: L.st_linear_logprob_bwd.raw(
-        p, 64, p, 64, p, p, p, p, 1.0, dh, lddh, db, df, lddw, acc, ws, nb, 8, 1000, 64, None)
+    bwd = lambda dh=p, lddh=64, db=None, df=None, lddw=64, acc=0, ws=p, nb=1 << 40, z=None, ldz=0: L.st_linear_logprob_bwd.raw(
+        p, 64, p, 64, p, p, p, p, 1.0, z, ldz, dh, lddh, db, df, lddw, acc, ws, nb, 8, 1000, 64, None)
     for bad in (dict(dh=p + 2), dict(lddh=63), dict(lddh=60), dict(db=p, df=p), dict(db=p, acc=1), dict(db=p, lddw=66), dict(df=p, lddw=62), dict(df=p + 4),
-                dict(ws=None), dict(nb=small - 1)):
+                dict(ws=None), dict(nb=small - 1), dict(z=p + 8, ldz=1024), dict(z=p, ldz=1000)):
         assert bwd(**bad) == -22, bad
-    kl = lambda K=4, ids=p, a=p, ws=p, T=8: L.st_linear_topk_kl_fwd.raw(p, 64, p, 64, ids, a, K, 0, 1.0, p, p, p, ws, 1 << 40, T, 1000, 64, None)
+    kl = lambda K=4, ids=p, a=p, ws=p, T=8: L.st_linear_topk_kl_fwd.raw(p, 64, p, 64, ids, a, K, 0, 1.0, p, p, p, None, 0, ws, 1 << 40, T, 1000, 64, None)
     for bad in (dict(K=0), dict(K=1025), dict(ids=None), dict(a=None), dict(ws=None), dict(K=1024, T=1 << 21)):
         assert kl(**bad) == -22, bad
     top = lambda z=p, ldl=1000, k=5, it=1.0, ws=p, nb=1 << 40, T=8, V=1000: L.st_topk_logprob.raw(z, ldl, k, it, p, p, p, ws, nb, T, V, None)
     for bad in (dict(z=None), dict(z=p + 1), dict(ldl=999), dict(k=0), dict(k=257), dict(k=6, V=5, ldl=5), dict(it=0.0), dict(T=-1), dict(V=0)):
         assert top(**bad) == -22, bad
+
+
+def test_kept_logits_buffers():
+    from spatialthinker_amd import ops
+    h, w, lab = args(T=4, V=70)
+    good = ops.head_logits_buffer(4, 70, h.device)
+    assert good.shape == (4, 128) and good.dtype == torch.float32
+    for bad in (good.double(), good.to(BF16)):
+        with pytest.raises(TypeError):
+            ops._kept_logits(bad, 4, 70, h.device)
+    for bad in (good[:3], good[:, :64], good[0], good[:1].expand(4, 128), torch.zeros(4, 130)[:, :128], torch.zeros(4, 132)[:, 1:129]):
+        with pytest.raises(ValueError):
+            ops._kept_logits(bad, 4, 70, h.device)
+    assert ops._kept_logits(None, 4, 70, h.device) == (None, 0) and ops._kept_logits(torch.zeros(4, 132)[:, :128], 4, 70, h.device)[1] == 132

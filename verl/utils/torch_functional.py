@@ -132,14 +132,15 @@ def _once(ctx):
 
 
 class _LinearLogProbs(torch.autograd.Function):
-    """log-probs of given tokens from hidden states and head weight, the logits never stored (st_linear_logprob_fwd / _bwd).  The backward forms
-    the logits again, piece by piece of the vocabulary; only the gradients that autograd asks for are computed."""
+    """log-probs of given tokens from hidden states and head weight (st_linear_logprob_fwd / _bwd).  Unless the forward has kept the logits, the backward
+    forms them again, piece by piece of the vocabulary; only the gradients that autograd asks for are computed."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, labels, temperature):
+    def forward(ctx, hidden, weight, labels, temperature, keep):
         from spatialthinker_amd import ops
-        logp, lse = ops.linear_logprob_fwd(hidden, weight, labels, temperature)
-        ctx.save_for_backward(hidden, weight, labels, logp, lse)
+        logits = ops.head_logits_buffer(hidden.shape[0], weight.shape[0], hidden.device) if keep else None
+        logp, lse = ops.linear_logprob_fwd(hidden, weight, labels, temperature, logits)
+        ctx.save_for_backward(hidden, weight, labels, logp, lse, logits)
         ctx.temperature = temperature
         return logp
 
@@ -147,19 +148,20 @@ class _LinearLogProbs(torch.autograd.Function):
     def backward(ctx, grad_out):
         from spatialthinker_amd import ops
         _once(ctx)
-        hidden, weight, labels, logp, lse = ctx.saved_tensors
+        hidden, weight, labels, logp, lse, logits = ctx.saved_tensors
         dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if ctx.needs_input_grad[1] else None
         dh = ops.linear_logprob_bwd(hidden, weight, labels, logp, lse, grad_out.contiguous().float(), ctx.temperature,
-                                    want_dhidden=ctx.needs_input_grad[0], dweight=dw)
-        return dh, dw, None, None
+                                    want_dhidden=ctx.needs_input_grad[0], dweight=dw, logits=logits)
+        return dh, dw, None, None, None
 
 
 class _LinearTopkKL(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, ids, teacher, temperature, renormalize):
+    def forward(ctx, hidden, weight, ids, teacher, temperature, renormalize, keep):
         from spatialthinker_amd import ops
-        kl, lse, logq = ops.linear_topk_kl_fwd(hidden, weight, ids, teacher, temperature, renormalize)
-        ctx.save_for_backward(hidden, weight, ids, teacher, lse, logq)
+        logits = ops.head_logits_buffer(hidden.shape[0], weight.shape[0], hidden.device) if keep else None
+        kl, lse, logq = ops.linear_topk_kl_fwd(hidden, weight, ids, teacher, temperature, renormalize, logits)
+        ctx.save_for_backward(hidden, weight, ids, teacher, lse, logq, logits)
         ctx.temperature, ctx.renormalize = temperature, renormalize
         return kl
 
@@ -167,11 +169,11 @@ class _LinearTopkKL(torch.autograd.Function):
     def backward(ctx, grad_out):
         from spatialthinker_amd import ops
         _once(ctx)
-        hidden, weight, ids, teacher, lse, logq = ctx.saved_tensors
+        hidden, weight, ids, teacher, lse, logq, logits = ctx.saved_tensors
         dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if ctx.needs_input_grad[1] else None
         dh = ops.linear_topk_kl_bwd(hidden, weight, ids, teacher, lse, logq, grad_out.contiguous().float(), ctx.temperature, ctx.renormalize,
-                                    want_dhidden=ctx.needs_input_grad[0], dweight=dw)
-        return dh, dw, None, None, None, None
+                                    want_dhidden=ctx.needs_input_grad[0], dweight=dw, logits=logits)
+        return dh, dw, None, None, None, None, None
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
@@ -189,24 +191,32 @@ def _flat(t: torch.Tensor, dtype: torch.dtype, device: torch.device) -> torch.Te
     return t.to(device=device, dtype=dtype).contiguous().view(-1)
 
 
-def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
-    """log_probs_from_logits(hidden @ weight^T / temperature, labels) without the logits: hidden (..., H), weight (V, H) (the head), labels (...)
-    -> (...) fp32, differentiable in hidden and weight.  At V = 152 064 the logits of 8192 rows are 2.5 GB; here the backward keeps
-    one piece of the vocabulary's gradient at a time (0.5 GiB at most) next to fp32 partial sums of hidden's, and the logits stay in fp32.  A label outside [0, V) (padding, -100) marks a row that is not
-    scored: 0, and no gradient from it.  H must be a multiple of 64; GPU tensors only."""
+def _keep(hidden: torch.Tensor, weight: torch.Tensor, keep_logits: int) -> bool:
+    return torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad) and hidden.shape[0] * ((weight.shape[0] + 63) // 64 * 64) * 4 <= keep_logits
+
+
+def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, temperature: float = 1.0, keep_logits: int = 8 << 30) -> torch.Tensor:
+    """log_probs_from_logits(hidden @ weight^T / temperature, labels) as one operator: hidden (..., H), weight (V, H) (the head), labels (...)
+    -> (...) fp32, differentiable in hidden and weight.  The logits stay in fp32 and are kept for the backward only while
+    they take at most `keep_logits` bytes (8 GiB of the card's 288: 14 122 rows of V = 152 064); beyond that, or with 0, the backward forms them again,
+    a piece of the vocabulary at a time (the gradient of one piece: 0.5 GiB at most, next to fp32 partial sums of hidden's), which takes 4 to 25 % more
+    time for forward and backward together.  Without a gradient nothing is kept.  Both ways give the same bits.
+    A label outside [0, V) (padding, -100) marks a row that is not scored: 0, and no gradient from it.  H must be a multiple of 64; GPU tensors only."""
     if labels.shape != hidden.shape[:-1]:
         raise ValueError(f"labels {tuple(labels.shape)} do not match hidden {tuple(hidden.shape)}")
-    out = _LinearLogProbs.apply(_rows16(hidden), _rows16(weight), _flat(labels, torch.int64, hidden.device), float(temperature))
+    h, w = _rows16(hidden), _rows16(weight)
+    out = _LinearLogProbs.apply(h, w, _flat(labels, torch.int64, hidden.device), float(temperature), _keep(h, w, keep_logits))
     return out if labels.dim() == 1 else out.view(labels.shape)
 
 
 def linear_topk_kl(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor, teacher_log_probs: torch.Tensor, temperature: float = 1.0,
-                   renormalize: bool = False) -> torch.Tensor:
-    """Distillation from a teacher's top log-probs (top_log_probs), per row, without the student's logits:
+                   renormalize: bool = False, keep_logits: int = 8 << 30) -> torch.Tensor:
+    """Distillation from a teacher's top log-probs (top_log_probs), per row, straight from the student's hidden states:
         kl[t] = sum_k p_k (log p_k - log softmax(hidden_t @ weight^T / temperature)[id_k]),   p = exp(teacher_log_probs)
     hidden (..., H), weight (V, H), teacher_ids / teacher_log_probs (..., K) -> (...) fp32, differentiable in hidden and weight (the teacher is a
     constant).  renormalize: p is scaled to sum 1 over the row's entries; without it the mass outside the teacher's top K counts for nothing.
-    Entries with an id outside [0, V) are absent; a row of such entries gives 0 and no gradient.  K <= 1024."""
+    Entries with an id outside [0, V) are absent; a row of such entries gives 0 and no gradient.  K <= 1024.
+    keep_logits: as linear_log_probs."""
     if teacher_ids.shape[:-1] != hidden.shape[:-1] or teacher_ids.shape != teacher_log_probs.shape:
         raise ValueError(f"teacher ids {tuple(teacher_ids.shape)} / log-probs {tuple(teacher_log_probs.shape)} do not match hidden {tuple(hidden.shape)}")
     k = teacher_ids.shape[-1]
@@ -214,7 +224,8 @@ def linear_topk_kl(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torc
         teacher_ids = teacher_ids.clamp(-1, 0x7fffffff).to(torch.int32)
     ids = _flat(teacher_ids, torch.int32, hidden.device).view(-1, k)
     a = _flat(teacher_log_probs.detach(), torch.float32, hidden.device).view(-1, k)
-    out = _LinearTopkKL.apply(_rows16(hidden), _rows16(weight), ids, a, float(temperature), bool(renormalize))
+    h, w = _rows16(hidden), _rows16(weight)
+    out = _LinearTopkKL.apply(h, w, ids, a, float(temperature), bool(renormalize), _keep(h, w, keep_logits))
     return out if hidden.dim() == 2 else out.view(hidden.shape[:-1])
 
 
