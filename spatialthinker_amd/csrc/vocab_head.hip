@@ -4,7 +4,7 @@
 //   log-prob of given tokens:          logp_t = z[t][label_t] - lse_t
 //   distillation from top log-probs:   kl_t = sum_k p_tk (log p_tk - (z[t][id_tk] - lse_t)),  p from the teacher's k log-probs of the row
 // Both gradients have one form: d[t][v] = c_t exp(z[t][v] - lse_t) + (sparse targets), dh = d W, dW = d^T h, so both share every product:
-//   forward   head_tile_kernel<STATS>   z tile in registers -> per row (max, sum 2^(z - max)) of 128 columns; then head_lse_kernel
+//   forward   head_tile_kernel<STATS>   z tile in registers -> per row (max, sum 2^(z - max) - 1) of 128 columns; then head_lse_kernel
 //   backward  per piece of the vocabulary: head_tile_kernel<DLOGITS> forms the tile again and writes d (bf16) into a bounded workspace, or
 //             head_d_kernel writes it from kept logits; head_dh_kernel adds d W into fp32 slabs, head_dw_kernel writes d^T h
 // Kept logits cost the forward their write and save the backward one of its three products (forward + backward, 152 064 x 3584: 16 rows 745 -> 621 us,
@@ -19,6 +19,15 @@
 #define VH_LN2 0.6931471805599453f
 
 __device__ __forceinline__ float vh_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Statistics of a set of logits (in base 2): x = the largest, y = sum 2^(z - x) - 1.  The largest one's own term is exactly 1 and left out of the sum,
+// because the log-prob of a nearly certain token is -log(1 + y): next to a 1 a small y would keep few of its digits.  Empty: (-inf, -1).
+__device__ __forceinline__ float2 vh_join(float2 a, float2 b) {
+    const float m = fmaxf(a.x, b.x);
+    if (m == -INFINITY) return make_float2(m, a.y + b.y + 1.f);      // empty, or NaN kept
+    const float ra = a.x == m ? a.y : (1.f + a.y) * vh_exp2(a.x - m);
+    return make_float2(m, ra + (b.x == m && a.x != m ? b.y : (1.f + b.y) * vh_exp2(b.x - m)));
+}
 
 // workgroup -> tile: each XCD walks a contiguous range of tiles in groups of 8 tile-rows (A and B panels shared in its L2)
 __device__ __forceinline__ void vh_tile(int bid, int tiles_m, int tiles_n, int& tm, int& tn) {
@@ -63,7 +72,7 @@ __device__ __forceinline__ void vh_store_image(const char* smem, uint16_t* __res
 // ------------------------------------------------------------------------------------------------------------------------------------
 // Logit tile of 256 rows x 256 vocabulary columns.  A lane owns 8 rows (mi*16 + (lane & 15)) and, of each, 4 columns of every 16-column
 // tile ni, so row statistics reduce inside the lane first and over the four lanes of a row last.
-// STATS: part[tn*2 + wn][m] = (max, sum) in base 2 of the 128 columns of a wave; zlab[m] = the label's logit, or z2[m][k] = the logit of target k
+// STATS: part[tn*2 + wn][m] = the statistics (vh_join) of the 128 columns of a wave; zlab[m] = the label's logit, or z2[m][k] = the logit of target k
 // from the tile's list of targets (head_bucket_kernel): from the same accumulators as the statistics, so that a target that is its row's maximum
 // has exactly the maximum's value.
 // KEEP: z[m][n] = h_m . w_n in fp32 as well, straight from the accumulators (64-byte runs; V = 152 064, H = 3584, 4096 rows: 416 us for 2.5 GB).
@@ -144,8 +153,25 @@ __global__ __launch_bounds__(256) void head_tile_kernel(const uint16_t* __restri
                 for (int r = 0; r < 4; ++r) s += vh_exp2(fmaf(acc[ni][mi][r], sc, -sub));
             s += __shfl_xor(s, 16, 64);
             s += __shfl_xor(s, 32, 64);
+            float rest = s - 1.f;                                    // (nothing but -inf: -1)
+            if (__any(s < 1.5f && m2 != -INFINITY)) {                // a row with one large logit among these 128: the others' sum by itself
+                float o = 0.f, ties = -1.f;
+#pragma unroll
+                for (int ni = 0; ni < 8; ++ni)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float x = acc[ni][mi][r];
+                        if (x == mx) ties += 1.f; else o += vh_exp2(fmaf(x, sc, -sub));
+                    }
+                ties += lane < 16 ? 0.f : 1.f;                       // (the -1 once per row)
+                o += __shfl_xor(o, 16, 64);
+                o += __shfl_xor(o, 32, 64);
+                ties += __shfl_xor(ties, 16, 64);
+                ties += __shfl_xor(ties, 32, 64);
+                if (m2 != -INFINITY) rest = o + ties;
+            }
             if (m < T) {
-                if (lane < 16) part[(int64_t)(tn * 2 + wn) * T + m] = make_float2(m2, s);
+                if (lane < 16) part[(int64_t)(tn * 2 + wn) * T + m] = make_float2(m2, rest);
                 if (labels) {
                     const int64_t lab = labels[m] - (n0 + wn * 128);
                     if (lab >= 0 && lab < 128) {                     // one lane of the row owns the label's column
@@ -314,14 +340,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t*
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             const float m2 = mx * sc, sub = m2 == -INFINITY ? 0.f : m2;
-            float s = 0.f;
+            float o = 0.f, ties = lane < 16 ? -1.f : 0.f;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s += vh_exp2(fmaf(acc[i][j][r], sc, -sub));
-            s += __shfl_xor(s, 16, 64);
-            s += __shfl_xor(s, 32, 64);
-            if (lane < 16) red[wave * BT + m] = make_float2(m2, s);
+                for (int r = 0; r < 4; ++r) {
+                    const float x = acc[i][j][r];
+                    if (x == mx) ties += 1.f; else o += vh_exp2(fmaf(x, sc, -sub));
+                }
+            o += __shfl_xor(o, 16, 64);
+            o += __shfl_xor(o, 32, 64);
+            ties += __shfl_xor(ties, 16, 64);
+            ties += __shfl_xor(ties, 32, 64);
+            if (lane < 16) red[wave * BT + m] = make_float2(m2, m2 != -INFINITY ? o + ties : o - 1.f);
             if (labels && m < T) {
                 const int64_t lab = labels[m] - col0;
 #pragma unroll
@@ -335,11 +366,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t*
         for (int m = threadIdx.x; m < min(BT, T); m += NT) {
             float2 a = red[m];
 #pragma unroll
-            for (int wv = 1; wv < WAVES; ++wv) {
-                const float2 b = red[wv * BT + m];
-                const float mn = fmaxf(a.x, b.x);
-                a = make_float2(mn, mn != -INFINITY ? a.y * vh_exp2(a.x - mn) + b.y * vh_exp2(b.x - mn) : a.y + b.y);
-            }
+            for (int wv = 1; wv < WAVES; ++wv) a = vh_join(a, red[wv * BT + m]);
             part[(int64_t)blockIdx.x * T + m] = a;
         }
     } else {
@@ -446,7 +473,7 @@ __global__ __launch_bounds__(256) void head_d_kernel(const float* __restrict__ z
     }
 }
 
-// (max, sum) partials -> lse (natural log), stat = (max, log2 sum); logp = label logit - lse for rows with a label inside the vocabulary, 0 for the others.
+// partial statistics (vh_join) -> lse (natural log), stat = (max, log2 sum); logp = label logit - lse for rows with a label inside the vocabulary, 0 for the others.
 // 16 rows x 64 slices per workgroup: 16 consecutive lanes read 128 contiguous bytes of one partial row.  Bound: reading the partials, 8 B per row and
 // 128 columns (4096 rows, V = 152 064: 39 MB in 15 us).
 __global__ __launch_bounds__(1024) void head_lse_kernel(const float2* __restrict__ part, int n_parts, const float* __restrict__ zlab,
@@ -455,29 +482,19 @@ __global__ __launch_bounds__(1024) void head_lse_kernel(const float2* __restrict
     __shared__ float2 red[64][17];
     const int r = threadIdx.x & 15, sl = threadIdx.x >> 4;
     const int row = blockIdx.x * 16 + r;
-    float m = -INFINITY, s = 0.f;
+    float2 a = make_float2(-INFINITY, -1.f);
     if (row < T)
 #pragma unroll 4
-        for (int p = sl; p < n_parts; p += 64) {
-            const float2 v = part[(int64_t)p * T + row];
-            const float mn = fmaxf(m, v.x);
-            if (mn != -INFINITY) s = s * vh_exp2(m - mn) + v.y * vh_exp2(v.x - mn);
-            else s += v.y;                                           // 0, or NaN kept
-            m = mn;
-        }
-    red[sl][r] = make_float2(m, s);
+        for (int p = sl; p < n_parts; p += 64) a = vh_join(a, part[(int64_t)p * T + row]);
+    red[sl][r] = a;
     __syncthreads();
     for (int o = 32; o > 0; o >>= 1) {
-        if (sl < o) {
-            const float2 a = red[sl][r], b = red[sl + o][r];
-            const float mn = fmaxf(a.x, b.x);
-            red[sl][r] = make_float2(mn, mn != -INFINITY ? a.y * vh_exp2(a.x - mn) + b.y * vh_exp2(b.x - mn) : a.y + b.y);
-        }
+        if (sl < o) red[sl][r] = vh_join(red[sl][r], red[sl + o][r]);
         __syncthreads();
     }
     if (sl == 0 && row < T) {
         const float2 v = red[0][r];
-        const float ls = log2f(v.y);
+        const float ls = log1pf(v.y) * VH_LOG2E;
         lse[row] = (v.x + ls) * VH_LN2;
         if (stat) stat[row] = make_float2(v.x, ls);
         if (labels) {                                                // (z - max) - log sum: exact where the label is the maximum, so a log-prob near 0
@@ -493,22 +510,18 @@ __global__ __launch_bounds__(1024) void head_lse_few_kernel(const float2* __rest
                                                            float2* __restrict__ stat, int T, int V) {
     __shared__ float2 red[16];
     const int row = blockIdx.x, lane = threadIdx.x & 63;
-    float2 a = make_float2(-INFINITY, 0.f);
-    auto join = [](float2 x, float2 y) {
-        const float m = fmaxf(x.x, y.x);
-        return make_float2(m, m != -INFINITY ? x.y * vh_exp2(x.x - m) + y.y * vh_exp2(y.x - m) : x.y + y.y);
-    };
-    for (int p = threadIdx.x; p < n_parts; p += 1024) a = join(a, part[(int64_t)p * T + row]);
+    float2 a = make_float2(-INFINITY, -1.f);
+    for (int p = threadIdx.x; p < n_parts; p += 1024) a = vh_join(a, part[(int64_t)p * T + row]);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) a = join(a, make_float2(__shfl_xor(a.x, o, 64), __shfl_xor(a.y, o, 64)));
+    for (int o = 32; o > 0; o >>= 1) a = vh_join(a, make_float2(__shfl_xor(a.x, o, 64), __shfl_xor(a.y, o, 64)));
     if (lane == 0) red[threadIdx.x >> 6] = a;
     __syncthreads();
     if (threadIdx.x < 64) {
         a = red[lane & 15];
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) a = join(a, make_float2(__shfl_xor(a.x, o, 64), __shfl_xor(a.y, o, 64)));
+        for (int o = 8; o > 0; o >>= 1) a = vh_join(a, make_float2(__shfl_xor(a.x, o, 64), __shfl_xor(a.y, o, 64)));
         if (lane == 0) {
-            const float ls = log2f(a.y);
+            const float ls = log1pf(a.y) * VH_LOG2E;
             lse[row] = (a.x + ls) * VH_LN2;
             if (stat) stat[row] = make_float2(a.x, ls);
             if (labels) {

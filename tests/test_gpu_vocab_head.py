@@ -88,6 +88,30 @@ def test_linear_log_probs_forward_and_gradients(T, H, V, temperature):
     assert (dh[~live] == 0).all()
 
 
+@pytest.mark.parametrize("T", [1, 40, 100, 150, 200, 300])
+def test_log_probs_of_nearly_certain_tokens_keep_their_digits(T):
+    """logp = -log(1 + y), y = sum exp(z_v - z_label) down to 1e-12: each term's relative error is that of its exponent, at most 2 ez + 2^-20 (exp2, log1p
+    and the sums of positive terms included), and so is logp's, however small it is."""
+    from verl.utils import torch_functional as VF
+    H, V = 64, 1003
+    g, h, w, lab, gr = make(T, H, V, 31 + T)
+    scale = torch.linspace(4.0, 18.0, T, device="cuda") if T > 1 else torch.tensor([9.0], device="cuda")
+    h = (scale[:, None] * w[lab].float()).to(BF16)
+    z, ez, _ = errors64(h, w, 1.0)
+    rest = (z - z.gather(1, lab[:, None])).scatter(1, lab[:, None], -math.inf).exp().sum(1)
+    want = -torch.log1p(rest)
+    got = VF.linear_log_probs(h, w, lab)
+    assert want.max() > -1e-4 and ((got.to(F64) - want).abs() <= want.abs() * (2 * ez + 2.0 ** -20)).all(), ((got.to(F64) - want).abs() / want.abs()).max()
+    ids = lab.to(torch.int32)[:, None].contiguous()                # a teacher that is certain: kl = -logp
+    kl = VF.linear_topk_kl(h, w, ids, torch.zeros(T, 1, device="cuda"))
+    assert ((kl.to(F64) + want).abs() <= want.abs() * (2 * ez + 2.0 ** -20)).all()
+    tied = w.clone()                                               # two equal maxima: log 2 each, and nothing lost
+    other = (lab + 1) % V
+    tied[other] = w[lab]
+    z = h.to(F64) @ tied.to(F64).t()
+    assert ((VF.linear_log_probs(h, tied, lab).to(F64) - (z.gather(1, lab[:, None])[:, 0] - torch.logsumexp(z, 1))).abs() <= 2 * ez + 2.0 ** -20).all()
+
+
 def test_more_than_one_piece_of_the_vocabulary():
     """T = 2100 rows leave 127 488 columns per piece: V = 150 001 takes two, the second one ending inside a tile."""
     from verl.utils import torch_functional as VF
