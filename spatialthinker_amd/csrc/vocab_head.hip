@@ -429,7 +429,7 @@ __global__ __launch_bounds__(256) void head_d_kernel(const float* __restrict__ z
                                                      uint16_t* __restrict__ d, int64_t ldd, int T64, uint16_t* __restrict__ dt, int TP) {
     constexpr int CB = 64 * 2 + 16;
     __shared__ __attribute__((aligned(16))) char img[FEW ? 128 * CB : 16];
-    const int n0 = blockIdx.x * 128, r0 = blockIdx.y * 64, c = (threadIdx.x & 15) * 8, rr = threadIdx.x >> 4;
+    const int nb = (int)((ldd + 127) >> 7), r0 = (int)(blockIdx.x / nb) * 64, n0 = (int)(blockIdx.x % nb) * 128, c = (threadIdx.x & 15) * 8, rr = threadIdx.x >> 4;
     const bool in = n0 + c < ldd;
     f32x4 v[4][2];
     VhRow ri[4];
@@ -1306,7 +1306,7 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
         const int64_t ldd = up(kv, 64);
         const uint16_t* wp = w + (int64_t)v0 * ldw;
         if (z) {
-            const dim3 grid(st_cdiv(ldd, 128), p.T64 / 64);
+            const dim3 grid(st_cdiv(ldd, 128) * (p.T64 / 64));
             if (p.few) hipLaunchKernelGGL(head_d_kernel<true>, grid, dim3(256), 0, s, z + v0, ldz, rows, T, kv, sc, v0, d, ldd, p.T64, dt, p.TP);
             else hipLaunchKernelGGL(head_d_kernel<false>, grid, dim3(256), 0, s, z + v0, ldz, rows, T, kv, sc, v0, d, ldd, p.T64, dt, p.TP);
             ST_CHECK_LAUNCH();

@@ -308,6 +308,26 @@ def test_kept_logits_of_several_pieces_and_in_a_captured_graph():
         assert all(torch.equal(x, y) for x, y in zip(out, want))
 
 
+@pytest.mark.parametrize("keep", [0, 8 << 30])
+def test_millions_of_rows_over_a_small_vocabulary(keep):
+    """More row blocks than a grid has in its second and third dimension."""
+    from verl.utils import torch_functional as VF
+    T, H, V = 65535 * 64 + 100, 64, 5
+    g, h, w, lab, gr = make(T, H, V, 77)
+    hh = h.clone().requires_grad_(True)
+    lp = VF.linear_log_probs(hh, w, lab, keep_logits=keep)
+    assert (lp.grad_fn.saved_tensors[-1] is not None) == (keep > 0)
+    dh, = torch.autograd.grad(lp, hh, gr)
+    rows = torch.tensor([0, 63, 64, 255, 256, T // 2, T - 101, T - 100, T - 65, T - 64, T - 1], device="cuda")
+    z, ez, el = errors64(h[rows], w, 1.0)
+    lse = torch.logsumexp(z, 1)
+    want = z.gather(1, lab[rows][:, None])[:, 0] - lse
+    assert ((lp[rows].to(F64) - want).abs() <= ez + el + U32 * want.abs()).all()
+    gt, q = gr[rows].to(F64)[:, None], (z - lse[:, None]).exp()
+    d = (-gt * q).scatter_add(1, lab[rows][:, None], gt)
+    check_grads(h[rows], w, d, UB * d.abs() + gt.abs() * q * (ez + el + 2.0 ** -20)[:, None], dh[rows], None, UB)
+
+
 def test_gradients_against_differences():
     """Central differences along random directions: <dh, h+ - h-> against the change of sum(g out), for steps that bf16 holds exactly.  The third-order
     rest of a difference of width e |h| (logits move by < 0.03) is below 1e-4 of the change's scale; 2 % covers it, the bf16 gradients (2^-8 per
