@@ -299,17 +299,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t*
     const int col0 = n0 + wave * 32 + fk * 4;                        // column of (i, r): col0 + i*16 + r
     if constexpr (!DLOGITS) {
         constexpr int ROWB = 128 * 4 + 16;
-        if (z) {
-#pragma unroll
-            for (int j = 0; j < MT; ++j) {
-                if (j * 16 + fr >= T) continue;
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (col0 + i * 16 < ldz) *reinterpret_cast<f32x4*>(z + (int64_t)(j * 16 + fr) * ldz + col0 + i * 16) = acc[i][j];
-            }
-        }
         const int e0 = tg.start ? tg.start[n0 >> 8] : 0, e1 = tg.start ? tg.start[(n0 >> 8) + 1] : 0;
-        for (int p = 0; p < BN / 128 && e1 > e0; ++p) {              // the tile through LDS, 128 columns at a time
+        for (int p = 0; p < BN / 128 && (e1 > e0 || z); ++p) {       // the tile through LDS, 128 columns at a time
             if (wave >> 2 == p) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -323,6 +314,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t*
                 if ((col >> 7) == (((n0 >> 7) + p) & 1))
                     tg.z2[(int64_t)row * tg.K + (it >> 16)] = sc * *reinterpret_cast<const float*>(smem + row * ROWB + (col & 127) * 4);
             }
+            if (z)                                                   // kept logits leave in runs of 512 bytes
+                for (int i = threadIdx.x; i < T * 32; i += NT) {
+                    const int row = i >> 5, c = (i & 31) * 4, col = n0 + p * 128 + c;
+                    if (col < ldz) *reinterpret_cast<f32x4*>(z + (int64_t)row * ldz + col) = *reinterpret_cast<const f32x4*>(smem + row * ROWB + c * 4);
+                }
             __syncthreads();
         }
         float2* red = reinterpret_cast<float2*>(smem);               // [wave][row]

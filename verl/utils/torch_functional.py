@@ -4,9 +4,9 @@ Host bookkeeping on (batch, length) tensors — masked_mean, get_response_mask, 
 torch.  The heavy entries are the HIP library behind the reference's own signatures, so code written against the reference imports
 and runs unchanged:
   log_probs_from_logits(logits, labels)   :34-66    -> autograd.Function over st_logprob_fwd / st_logprob_bwd
-  linear_log_probs(hidden, weight, labels)          -> the same log-probs from the head's inputs, no logits kept (st_linear_logprob_fwd / _bwd)
+  linear_log_probs(hidden, weight, labels)          -> the same log-probs straight from the head's inputs (st_linear_logprob_fwd / _bwd)
   top_log_probs(logits, k)                          -> a teacher's k largest log-probs of every row (st_topk_logprob)
-  linear_topk_kl(hidden, weight, ids, log_probs)    -> distillation from them, no logits kept (st_linear_topk_kl_fwd / _bwd)
+  linear_topk_kl(hidden, weight, ids, log_probs)    -> distillation from them, likewise (st_linear_topk_kl_fwd / _bwd)
   AnyPrecisionAdamW(params, lr, ...)      :201-329  -> torch.optim.Optimizer whose step() is st_adamw_kahan_step per parameter
   get_constant_schedule_with_warmup(...)  :187-197  -> LambdaLR with the same multiplier
 The training engine (spatialthinker_amd/actor.py) calls the same kernels on its flat buffers directly."""
