@@ -33,7 +33,7 @@ __device__ __forceinline__ float tk_value(int order) {
 }
 __device__ __forceinline__ uint64_t tk_key(int order, uint32_t id) { return ((uint64_t)(uint32_t)(order + 32768) << 32) | (0xffffffffu - id); }
 
-#define TK_BINS 1024                           // orders told apart below the largest candidate when the list is ranked
+#define TK_BINS 1024                           // orders told apart below the largest candidate when the list is ranked; the last bin holds all that lie lower
 
 template <int NT> struct TkShared {
     uint64_t cand[TK_CAP(NT) + 16];
@@ -121,7 +121,7 @@ template <int NT> __device__ __forceinline__ void tk_rank(TkShared<NT>& sh, int 
             if (threadIdx.x == 0) sh.count = 0;
             __syncthreads();
             for (int j = threadIdx.x; j < n; j += NT)
-                if (most - (int)(sh.cand[j] >> 32) <= last) sh.best[atomicAdd(&sh.count, 1)] = sh.cand[j];
+                if (min(most - (int)(sh.cand[j] >> 32), TK_BINS - 1) <= last) sh.best[atomicAdd(&sh.count, 1)] = sh.cand[j];   // clamped as counted: `left` of them
             __syncthreads();
             for (int j = threadIdx.x; j < left; j += NT) sh.cand[j] = sh.best[j];
             n = left;

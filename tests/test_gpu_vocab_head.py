@@ -413,6 +413,27 @@ def test_top_log_probs_adversarial_orders(T):
         check_top(z[i:i + 1].expand(T, V).contiguous(), k if i != 5 else 256)
 
 
+@pytest.mark.parametrize("T,V", [(1, 152064), (24, 152064), (600, 50001), (3, 300), (7, 400), (5, 1000)])
+@pytest.mark.parametrize("k", [10, 16, 20, 32, 48, 64, 96, 128, 256])
+def test_top_log_probs_with_a_kth_value_far_below_the_largest(T, V, k):
+    """Rows whose k-th largest lies more than 1023 bf16 steps (8 octaves, or a change of sign) below the largest: a few large logits over a bulk that is
+    negative, tiny, zero or -inf.  One slice and joined; as few candidates as one short row has, and as many as a vocabulary leaves."""
+    print(f"case T={T} V={V} k={k}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(T + V + k)
+    bulks = [lambda n: -6.0 + torch.randn(n, device="cuda", generator=g), lambda n: 0.03 * torch.rand(n, device="cuda", generator=g),
+             lambda n: -12.0 * torch.rand(n, device="cuda", generator=g), lambda n: 1e-30 * torch.randn(n, device="cuda", generator=g),
+             lambda n: torch.zeros(n, device="cuda"), lambda n: torch.full((n,), -1.0, device="cuda"), lambda n: torch.full((n,), -math.inf, device="cuda")]
+    rows = []
+    for t in range(max(T, 3 * len(bulks))):
+        z = bulks[t % len(bulks)](V)
+        p = (1, 5, k - 1)[t // len(bulks) % 3]
+        z[torch.randperm(V, device="cuda", generator=g)[:p]] = 8.0 + 4.0 * torch.rand(p, device="cuda", generator=g)
+        rows.append(z.to(BF16))
+    z = torch.stack(rows)
+    for i in range(0, z.shape[0], T):
+        check_top(z[i:i + T], k)
+
+
 def test_top_log_probs_pitch_alignment_and_special_rows():
     from spatialthinker_amd import ops
     g = torch.Generator(device="cuda").manual_seed(2)
