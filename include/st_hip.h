@@ -69,7 +69,7 @@ int st_logprob_bwd(st_bf16* logits, int64_t ldl, const int64_t* labels, const fl
  *   - workspace: st_linear_head_workspace_bytes(T, V, H, K (0 for labels), backward) bytes, 16-byte aligned, contents irrelevant.  Nothing is kept in it between
  *     calls: calls on several streams and captured graphs need one each.  backward != 0 covers any subset of the gradients.
  *   - logits: NULL, or a (T, ldz >= V rounded up to 64) fp32 buffer, 16-byte aligned, ldz % 4 == 0, in which the forward leaves h . w (before the
- *     temperature) for the backward of the same call; without it the backward forms them again, a piece of the vocabulary at a time.  Both ways
+ *     temperature) for the backward of the same call (columns from V rounded up to 64 on are left as they were); without it the backward forms them again, a piece of the vocabulary at a time.  Both ways
  *     give the same bits.
  *   - the same inputs give the same bits. */
 int st_linear_head_workspace_bytes(int T, int V, int H, int K, int backward, int64_t* bytes_host, st_stream_t stream);

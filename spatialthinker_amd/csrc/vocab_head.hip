@@ -18,6 +18,9 @@
 #define VH_LOG2E 1.4426950408889634f
 #define VH_LN2 0.6931471805599453f
 
+// columns of a kept-logits row: V rounded up to 64, whatever the row pitch (what lies behind them is the caller's)
+__device__ __forceinline__ int vh_cols64(int V) { return (V + 63) & ~63; }
+
 __device__ __forceinline__ float vh_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Statistics of a set of logits (in base 2): x = the largest, y = sum 2^(z - x) - 1.  The largest one's own term is exactly 1 and left out of the sum,
@@ -105,7 +108,7 @@ __global__ __launch_bounds__(256) void head_tile_kernel(const uint16_t* __restri
                 if (m >= T) continue;
 #pragma unroll
                 for (int ni = 0; ni < 8; ++ni)
-                    if (col0 + ni * 16 < ldz) *reinterpret_cast<f32x4*>(z + (int64_t)m * ldz + col0 + ni * 16) = acc[ni][mi];
+                    if (col0 + ni * 16 < vh_cols64(V)) *reinterpret_cast<f32x4*>(z + (int64_t)m * ldz + col0 + ni * 16) = acc[ni][mi];
             }
         }
         const int e0 = tg.start ? tg.start[tm * (tiles_n + 1) + tn] : 0, e1 = tg.start ? tg.start[tm * (tiles_n + 1) + tn + 1] : 0;
@@ -317,7 +320,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t*
             if (z)                                                   // kept logits leave in runs of 512 bytes
                 for (int i = threadIdx.x; i < T * 32; i += NT) {
                     const int row = i >> 5, c = (i & 31) * 4, col = n0 + p * 128 + c;
-                    if (col < ldz) *reinterpret_cast<f32x4*>(z + (int64_t)row * ldz + col) = *reinterpret_cast<const f32x4*>(smem + row * ROWB + c * 4);
+                    if (col < vh_cols64(V)) *reinterpret_cast<f32x4*>(z + (int64_t)row * ldz + col) = *reinterpret_cast<const f32x4*>(smem + row * ROWB + c * 4);
                 }
             __syncthreads();
         }

@@ -275,6 +275,30 @@ def test_kept_logits_give_the_same_bits(T, V):
             assert torch.equal(fn(h, w, 8 << 30)[live], outs[0][0][live])
 
 
+@pytest.mark.parametrize("T,V", [(1, 5), (20, 70), (64, 129), (65, 70), (100, 300), (150, 70), (150, 257), (161, 70), (300, 70), (300, 577)])
+def test_kept_logits_in_a_part_of_a_wider_buffer(T, V):
+    """Kept logits as columns of a wider buffer, first and last columns of it: what lies in front of and behind the view is left alone, and the backward
+    reads the view (bits as without kept logits)."""
+    from spatialthinker_amd import ops
+    print(f"case T={T} V={V}", flush=True)
+    H, wide, cols = 64, 1024, (V + 63) // 64 * 64
+    g, h, w, lab, gr = make(T, H, V, T + V)
+    logp, lse = ops.linear_logprob_fwd(h, w, lab)
+    dw = torch.empty(V, H, dtype=BF16, device="cuda")
+    dh = ops.linear_logprob_bwd(h, w, lab, logp, lse, gr, dweight=dw)
+    for at in (0, 192, wide - cols):
+        buf = torch.full((T + 1, wide), 7.0, device="cuda")
+        view = buf[:T, at:at + cols]
+        assert view.stride(0) == wide
+        out = ops.linear_logprob_fwd(h, w, lab, logits=view)
+        assert torch.equal(out[0], logp) and torch.equal(out[1], lse)
+        assert (buf[:, :at] == 7.0).all() and (buf[:, at + cols:] == 7.0).all() and (buf[T] == 7.0).all()
+        z, ez, _ = errors64(h, w, 1.0)
+        assert ((view[:, :V].to(F64) - z).abs() <= ez[:, None]).all()
+        dwz = torch.empty_like(dw)
+        assert torch.equal(ops.linear_logprob_bwd(h, w, lab, logp, lse, gr, dweight=dwz, logits=view), dh) and torch.equal(dwz, dw)
+
+
 def test_kept_logits_of_several_pieces_and_in_a_captured_graph():
     from spatialthinker_amd import ops
     from verl.utils import torch_functional as VF
