@@ -71,6 +71,7 @@ int st_logprob_bwd(st_bf16* logits, int64_t ldl, const int64_t* labels, const fl
  *   - logits: NULL, or a (T, ldz >= V rounded up to 64) fp32 buffer, 16-byte aligned, ldz % 4 == 0, in which the forward leaves h . w (before the
  *     temperature) for the backward of the same call (columns from V rounded up to 64 on are left as they were); without it the backward forms them again, a piece of the vocabulary at a time.  Both ways
  *     give the same bits.
+ *   - a row with a NaN or +inf logit (given, or beyond fp32) has NaN results; -inf logits are probabilities of 0.
  *   - the same inputs give the same bits. */
 int st_linear_head_workspace_bytes(int T, int V, int H, int K, int backward, int64_t* bytes_host, st_stream_t stream);
 /* logp[t] = z[t][labels[t]] - lse[t], lse[t] = log sum_v exp z[t][v].  A label outside [0, V) marks a row that is not scored: logp 0 (lse is

@@ -171,7 +171,7 @@ __global__ __launch_bounds__(256) void head_tile_kernel(const uint16_t* __restri
                 o += __shfl_xor(o, 32, 64);
                 ties += __shfl_xor(ties, 16, 64);
                 ties += __shfl_xor(ties, 32, 64);
-                if (m2 != -INFINITY) rest = o + ties;
+                if (s < 1.5f && m2 != -INFINITY) rest = o + ties;      // (s is the same in a row's four lanes: no row depends on the others of its wave)
             }
             if (m < T) {
                 if (lane < 16) part[(int64_t)(tn * 2 + wn) * T + m] = make_float2(m2, rest);
@@ -351,7 +351,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t*
             o += __shfl_xor(o, 32, 64);
             ties += __shfl_xor(ties, 16, 64);
             ties += __shfl_xor(ties, 32, 64);
-            if (lane < 16) red[wave * BT + m] = make_float2(m2, m2 != -INFINITY ? o + ties : o - 1.f);
+            // +inf, given or overflowed: NaN, as inf - inf makes it in the sum of all terms
+            if (lane < 16) red[wave * BT + m] = make_float2(m2, m2 == INFINITY ? NAN : m2 != -INFINITY ? o + ties : o - 1.f);
             if (labels && m < T) {
                 const int64_t lab = labels[m] - col0;
 #pragma unroll

@@ -158,6 +158,48 @@ def test_fp32_weight_gradient_and_single_gradients(T, accumulate):
     assert (pitched[:, H:] == 7.0).all()                           # behind the rows: untouched
 
 
+@pytest.mark.parametrize("T", [3, 40, 70, 100, 150, 200, 300])
+def test_rows_do_not_depend_on_their_neighbours_and_infinite_logits_give_nan(T):
+    """Every third row is watched; the rows between are flat, then nearly certain, then overflow to a +inf logit.  The watched rows' outputs keep their bits,
+    and a row with a +inf logit has NaN log-probs (what inf - inf gives in log_softmax) whatever stands beside it and however many rows there are."""
+    from spatialthinker_amd import ops
+    H, V, K = 64, 1003, 3
+    g, h, w, lab, gr = make(T, H, V, 13 + T)
+    h[:, 0] = 0
+    w[:, 0] = 0
+    w[5, 0] = 1e20                                                 # times 1e20: beyond fp32 in column 5 only
+    ids = torch.randint(0, V, (T, K), device="cuda", generator=g, dtype=torch.int32)
+    a = torch.log_softmax(torch.randn(T, K, device="cuda", generator=g), 1)
+    watched = torch.arange(T, device="cuda") % 3 == 1
+    lab[0] = 5
+    outs = []
+    for kind in ("flat", "certain", "infinite"):
+        x = h.clone()
+        if kind == "flat":
+            x[~watched] *= 0.01
+        if kind == "certain":
+            x[~watched] = (12.0 * w[(lab[~watched] + 7) % V].float()).masked_fill(torch.arange(H, device="cuda") == 0, 0.0).to(BF16)
+        if kind == "infinite":
+            x[~watched, 0] = 1e20
+        logp, lse = ops.linear_logprob_fwd(x, w, lab)
+        kl, lse2, logq = ops.linear_topk_kl_fwd(x, w, ids, a)
+        outs.append([t[watched] for t in (logp, lse, kl, logq)])
+        for t in (logp, lse, kl):
+            assert (torch.isnan(t[~watched]).all() if kind == "infinite" else torch.isfinite(t).all()), kind
+        assert all(torch.isfinite(t).all() for t in outs[-1])
+        assert all(torch.equal(x0, x1) for x0, x1 in zip(outs[0], outs[-1])), kind
+    x = h.clone()
+    x[:, 0] = -1e20                                                # -inf in column 5: its probability is 0, nothing else changes
+    logp, lse = ops.linear_logprob_fwd(x, w, lab)
+    z = (h.to(F64) @ w.to(F64).t())
+    z[:, 5] = -math.inf
+    _, ez, el = errors64(h[:, 1:], w[:, 1:], 1.0)
+    want = torch.log_softmax(z, 1).gather(1, lab[:, None])[:, 0]
+    assert torch.equal(torch.isneginf(logp), torch.isneginf(want)) and torch.isneginf(logp[0])
+    ok = torch.isfinite(want)
+    assert ((logp.to(F64) - want).abs() <= ez + el + U32 * want.abs())[ok].all()
+
+
 @pytest.mark.parametrize("op", ["labels", "topk"])
 def test_rows_without_a_gradient_may_hold_anything(op):
     """Unscored rows with NaN / infinite hidden states: the other rows' results have the same bits as with zeros there."""
