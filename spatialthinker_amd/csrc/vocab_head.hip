@@ -248,7 +248,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t*
     const int nk = H / 64, fr = lane & 15, fk = lane >> 4;
     // K-step kt reads k = (kt + turn) % nk: rows at a pitch of whole 4 KiB meet in a few memory channels where all workgroups stand at the same k
     // (V = 100 000, H = 2048: 8 rows 89 -> 79 us, 100 rows 107 -> 90; H = 4096: 168 -> 141, 200 -> 157; at other pitches 0 to 3 % slower, so not there)
-    const int turn = (ldw & 2047) == 0 ? (int)blockIdx.x % nk : 0;
+    // (counted from the vocabulary's first column, so that a piece of it sums in the order of the whole)
+    const int turn = (ldw & 2047) == 0 ? (int)(v0 / BN + blockIdx.x) % nk : 0;
     auto stage = [&](int kt) {
         char* dst = smem + (kt % SLOTS) * SLOT;
         const int k = (kt + turn < nk ? kt + turn : kt + turn - nk) * 64;

@@ -341,6 +341,27 @@ def test_kept_logits_in_a_part_of_a_wider_buffer(T, V):
         assert torch.equal(ops.linear_logprob_bwd(h, w, lab, logp, lse, gr, dweight=dwz, logits=view), dh) and torch.equal(dwz, dw)
 
 
+def test_kept_logits_give_the_same_bits_over_pieces_of_a_pitched_weight():
+    """130 rows leave 1 398 016 columns per piece; weight rows at a pitch of 4 KiB are summed from another K-step on per column block, which has to be the
+    same one in a piece as in the whole vocabulary."""
+    from spatialthinker_amd import ops
+    T, H, V = 130, 192, 1400003
+    g = torch.Generator(device="cuda").manual_seed(9)
+    h = torch.empty(T, H, device="cuda", dtype=BF16).normal_(generator=g)
+    w = torch.empty(V, 2048, device="cuda", dtype=BF16)[:, :H]
+    w.copy_(torch.empty(V, H, device="cuda", dtype=BF16).normal_(0.0, 0.3, generator=g))
+    lab = torch.randint(0, V, (T,), device="cuda", generator=g)
+    lab[:40] = V - 1 - lab[:40] % 1000                             # targets in the second piece
+    gr = torch.randn(T, device="cuda", generator=g)
+    z = ops.head_logits_buffer(T, V, h.device)
+    logp, lse = ops.linear_logprob_fwd(h, w, lab, logits=z)
+    grads = []
+    for kept in (z, None):
+        dw = torch.empty(V, H, dtype=BF16, device="cuda")
+        grads.append((ops.linear_logprob_bwd(h, w, lab, logp, lse, gr, dweight=dw, logits=kept), dw))
+    assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][1], grads[1][1])
+
+
 def test_kept_logits_of_several_pieces_and_in_a_captured_graph():
     from spatialthinker_amd import ops
     from verl.utils import torch_functional as VF
