@@ -159,9 +159,9 @@ def _head_operands(hidden, weight, temperature):
     _positive(temperature)
     ldh, ldw = hidden.stride(0), weight.stride(0)
     if T and (hidden.data_ptr() & 15 or ldh & 7 or not H <= ldh < 1 << 22):
-        raise ValueError(f"hidden: rows must be 16-byte aligned and not overlap (stride {ldh})")
+        raise ValueError(f"hidden: rows must be 16-byte aligned, not overlap and lie less than 2^22 elements apart (stride {ldh})")
     if weight.data_ptr() & 15 or ldw & 7 or not H <= ldw < 1 << 22:
-        raise ValueError(f"weight: rows must be 16-byte aligned and not overlap (stride {ldw})")
+        raise ValueError(f"weight: rows must be 16-byte aligned, not overlap and lie less than 2^22 elements apart (stride {ldw})")
     if not hidden.is_cuda:
         _p(hidden)
     if weight.device != hidden.device:

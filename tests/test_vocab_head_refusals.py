@@ -113,3 +113,17 @@ def test_kept_logits_buffers():
         with pytest.raises(ValueError):
             ops._kept_logits(bad, 4, 70, h.device)
     assert ops._kept_logits(None, 4, 70, h.device) == (None, 0) and ops._kept_logits(torch.zeros(4, 132)[:, :128], 4, 70, h.device)[1] == 132
+
+
+def test_rows_at_any_pitch_reach_the_kernels():
+    """The last position of each sequence, whose rows lie a whole sequence apart (here 2^22 elements, more than the kernels address): copied, not refused.
+    What is refused here is only the CPU tensor behind it."""
+    from verl.utils import torch_functional as VF
+    last = torch.zeros(2, 2048, 2048, dtype=BF16)[:, -1]
+    assert last.stride(0) == 1 << 22
+    with pytest.raises(RuntimeError, match="not on a GPU"):
+        VF.linear_log_probs(last, torch.zeros(10, 2048, dtype=BF16), torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="not on a GPU"):
+        VF.linear_log_probs(torch.zeros(2, 2048, dtype=BF16), torch.zeros(2, 2048, 2048, dtype=BF16)[:, -1], torch.zeros(2, dtype=torch.int64))
+    near = torch.zeros(2, 2048, 2048 - 8, dtype=BF16)[:, -1]
+    assert VF._rows16(near) is near                                # a pitch below it is used as it lies

@@ -177,12 +177,12 @@ class _LinearTopkKL(torch.autograd.Function):
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t as (rows, width) bf16 with contiguous 16-byte aligned rows: itself where it is that, else a differentiable cast / view / copy."""
+    """t as (rows, width) bf16 with contiguous 16-byte aligned rows at a pitch below 2^22: itself where it is that, else a differentiable cast / view / copy."""
     if t.dtype != torch.bfloat16:
         t = t.to(torch.bfloat16)
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    if t.shape[0] == 0 or (t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0):
+    if t.shape[0] == 0 or (t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.shape[1] <= t.stride(0) < 1 << 22 and t.data_ptr() % 16 == 0):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
