@@ -127,3 +127,11 @@ def test_rows_at_any_pitch_reach_the_kernels():
         VF.linear_log_probs(torch.zeros(2, 2048, dtype=BF16), torch.zeros(2, 2048, 2048, dtype=BF16)[:, -1], torch.zeros(2, dtype=torch.int64))
     near = torch.zeros(2, 2048, 2048 - 8, dtype=BF16)[:, -1]
     assert VF._rows16(near) is near                                # a pitch below it is used as it lies
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64])
+def test_teacher_ids_of_every_integer_type(dtype):
+    from verl.utils import torch_functional as VF
+    h, w, _ = args()
+    with pytest.raises(RuntimeError, match="not on a GPU"):
+        VF.linear_topk_kl(h, w, torch.ones(4, 3, dtype=dtype), torch.zeros(4, 3))
