@@ -135,3 +135,10 @@ def test_teacher_ids_of_every_integer_type(dtype):
     h, w, _ = args()
     with pytest.raises(RuntimeError, match="not on a GPU"):
         VF.linear_topk_kl(h, w, torch.ones(4, 3, dtype=dtype), torch.zeros(4, 3))
+
+
+def test_no_teacher_entries_at_all_is_an_argument_error():
+    from verl.utils import torch_functional as VF
+    h, w, _ = args()
+    with pytest.raises(ValueError, match="ids"):
+        VF.linear_topk_kl(h, w, torch.zeros(4, 0, dtype=torch.int32), torch.zeros(4, 0))

@@ -220,6 +220,8 @@ def linear_topk_kl(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torc
     if teacher_ids.shape[:-1] != hidden.shape[:-1] or teacher_ids.shape != teacher_log_probs.shape:
         raise ValueError(f"teacher ids {tuple(teacher_ids.shape)} / log-probs {tuple(teacher_log_probs.shape)} do not match hidden {tuple(hidden.shape)}")
     k = teacher_ids.shape[-1]
+    if k == 0:
+        raise ValueError(f"teacher ids: at least one entry per row, got {tuple(teacher_ids.shape)}")
     if teacher_ids.dtype != torch.int32:                         # int64 ids that int32 cannot hold must stay outside [0, V)
         teacher_ids = teacher_ids.to(torch.int64).clamp(-1, 0x7fffffff).to(torch.int32)
     ids = _flat(teacher_ids, torch.int32, hidden.device).view(-1, k)
