@@ -142,3 +142,17 @@ def test_no_teacher_entries_at_all_is_an_argument_error():
     h, w, _ = args()
     with pytest.raises(ValueError, match="ids"):
         VF.linear_topk_kl(h, w, torch.zeros(4, 0, dtype=torch.int32), torch.zeros(4, 0))
+
+
+def test_top_log_probs_of_overlapping_rows_and_single_columns():
+    """Expanded logits and a vocabulary of one token in any layout are copied; the kernel entry itself goes on refusing them."""
+    from spatialthinker_amd import ops
+    from verl.utils import torch_functional as VF
+    shared = torch.zeros(1, 50, dtype=BF16).expand(3, 50)
+    column = torch.zeros(3, 4, dtype=BF16)[:, 1:2].t().contiguous().t()
+    assert column.stride(-1) != 1
+    for z, k in ((shared, 3), (column, 1), (torch.zeros(40, dtype=BF16).as_strided((3, 20), (4, 1)), 2)):
+        with pytest.raises(ValueError):
+            ops.topk_logprob(z, k)
+        with pytest.raises(RuntimeError, match="not on a GPU"):
+            VF.top_log_probs(z, k)

@@ -240,8 +240,8 @@ def top_log_probs(logits: torch.Tensor, k: int, temperature: float = 1.0):
     z = logits if logits.dtype == torch.bfloat16 else logits.to(torch.bfloat16)
     if z.dim() != 2:
         z = z.reshape(-1, z.shape[-1])
-    if z.stride(-1) != 1:
-        z = z.contiguous()
+    if z.stride(-1) != 1 or (z.shape[0] > 1 and z.stride(0) < z.shape[1]):
+        z = z.clone(memory_format=torch.contiguous_format)
     ids, logp, lse = ops.topk_logprob(z, int(k), float(temperature))
     if logits.dim() == 2:
         return ids, logp, lse
