@@ -570,6 +570,28 @@ def test_teacher_to_student_run():
     assert (ww.grad.to(F64) - wd.grad).norm() <= 3 * UB * wd.grad.norm()
 
 
+@pytest.mark.parametrize("op", ["labels", "topk"])
+def test_outputs_may_be_changed_in_place(op):
+    """Masking the result in place, one- and two-dimensional: the gradient of the masked result, as out of place."""
+    from verl.utils import torch_functional as VF
+    T, H, V, K = 66, 64, 500, 4
+    g, h, w, lab, gr = make(T, H, V, 4)
+    ids = torch.randint(0, V, (T, K), device="cuda", generator=g)
+    a = torch.log_softmax(torch.randn(T, K, device="cuda", generator=g), 1)
+    mask = torch.rand(T, device="cuda", generator=g) < 0.3
+    for shape in ((T,), (6, T // 6)):
+        grads = []
+        for inplace in (False, True):
+            hh, ww = h.view(*shape, H).clone().requires_grad_(True), w.clone().requires_grad_(True)
+            if op == "labels":
+                out = VF.linear_log_probs(hh, ww, lab.view(shape))
+            else:
+                out = VF.linear_topk_kl(hh, ww, ids.view(*shape, K), a.view(*shape, K))
+            out = out.masked_fill_(mask.view(shape), 0.0).mul_(2.0) if inplace else out.masked_fill(mask.view(shape), 0.0) * 2.0
+            grads.append(torch.autograd.grad(out, (hh, ww), gr.view(shape)))
+        assert all(torch.equal(x, y) for x, y in zip(*grads))
+
+
 def test_empty_batches_and_fp32_inputs():
     from verl.utils import torch_functional as VF
     w = torch.randn(300, 64, device="cuda", requires_grad=True)                    # fp32 leaf: cast inside, fp32 gradient back

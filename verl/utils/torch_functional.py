@@ -140,7 +140,8 @@ class _LinearLogProbs(torch.autograd.Function):
         from spatialthinker_amd import ops
         logits = ops.head_logits_buffer(hidden.shape[0], weight.shape[0], hidden.device) if keep else None
         logp, lse = ops.linear_logprob_fwd(hidden, weight, labels, temperature, logits)
-        ctx.save_for_backward(hidden, weight, labels, logp, lse, logits)
+        # (a copy: the caller may mask or scale its log-probs in place, as log_probs_from_logits lets it)
+        ctx.save_for_backward(hidden, weight, labels, logp.clone() if any(ctx.needs_input_grad) else logp, lse, logits)
         ctx.temperature = temperature
         return logp
 
