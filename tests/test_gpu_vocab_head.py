@@ -158,6 +158,39 @@ def test_fp32_weight_gradient_and_single_gradients(T, accumulate):
     assert (pitched[:, H:] == 7.0).all()                           # behind the rows: untouched
 
 
+@pytest.mark.parametrize("T", [129, 160, 161, 192, 193, 256])
+@pytest.mark.parametrize("H", [64, 192, 448])
+def test_weight_gradient_of_129_to_256_rows_over_a_large_vocabulary(T, H):
+    """From 32 513 columns on (two row blocks of 256 per compute unit) these row counts have a weight-gradient kernel of their own: all of its row tiles and
+    outputs, column ranges that are uneven or fewer than three, a vocabulary that ends inside a tile, logits kept and formed again, a pitched result."""
+    from spatialthinker_amd import ops
+    V, temperature = 33001, 0.8
+    print(f"case T={T} H={H} V={V}", flush=True)
+    g, h, w, lab, gr = make(T, H, V, T + H, pitch_h=8, pitch_w=24)
+    dead = torch.rand(T, device="cuda", generator=g) < 0.1
+    lab[dead] = -100
+    h[dead] = float("nan")
+    z, ez, el = errors64(h.masked_fill(dead[:, None], 0.0), w, temperature)
+    kept = ops.head_logits_buffer(T, V, h.device)
+    logp, lse = ops.linear_logprob_fwd(h, w, lab, temperature, logits=kept)
+    gt = torch.where(dead, 0.0, gr.to(F64))[:, None] / temperature
+    q = (z - torch.logsumexp(z, 1, keepdim=True)).exp()
+    d = (-gt * q).scatter_add(1, lab.clamp(min=0)[:, None], gt)
+    derr = UB * d.abs() + gt.abs() * q * (ez + el + 2.0 ** -20)[:, None]
+    hx = h.masked_fill(dead[:, None], 0.0)
+    before = torch.randn(V, H, device="cuda", generator=g)
+    for logits in (kept, None):
+        for dtype, accumulate in ((BF16, False), (torch.float32, False), (torch.float32, True)):
+            buf = torch.full((V + 1, H + 16), 7.0, dtype=dtype, device="cuda")
+            out = buf[:V, :H]
+            if accumulate:
+                out.copy_(before)
+            how = dict(dweight=out) if dtype == BF16 else dict(dweight_f32=out, accumulate=accumulate)
+            dh = ops.linear_logprob_bwd(h, w, lab, logp, lse, gr, temperature, logits=logits, **how)
+            check_grads(hx, w, d, derr, dh, out, UB if dtype == BF16 else U32, before if accumulate else None)
+            assert (buf[:, H:] == 7.0).all() and (buf[V] == 7.0).all()
+
+
 @pytest.mark.parametrize("T", [3, 40, 70, 100, 150, 200, 300])
 def test_rows_do_not_depend_on_their_neighbours_and_infinite_logits_give_nan(T):
     """Every third row is watched; the rows between are flat, then nearly certain, then overflow to a +inf logit.  The watched rows' outputs keep their bits,
