@@ -1163,7 +1163,7 @@ Plan head_plan(int T, int V, int H, int K) {                         // K: targe
     p.start = p.stat + up((int64_t)T * 8, 256);
     p.list = p.start + (K ? up((int64_t)st_cdiv(T, 256) * (st_cdiv(V, 256) + 1) * 4, 256) : 0);
     p.fwd_bytes = p.list + up((int64_t)T * K * 4, 256);
-    // d of one piece: at most 512 MiB
+    // d of one piece: at most 512 MiB; beyond 2^20 rows the 256 columns (or the fewer that there are) of one tile
     const int64_t max_cols = std::max<int64_t>(256, ((int64_t)512 << 20) / 2 / p.T64 / 256 * 256);
     p.pieces = st_cdiv(V, max_cols);
     p.piece = (int)up(st_cdiv(V, p.pieces), 256);
@@ -1178,7 +1178,8 @@ Plan head_plan(int T, int V, int H, int K) {                         // K: targe
         const int64_t cost = (int64_t)st_cdiv((int64_t)tiles * s, ncu) * (st_cdiv(nkt, s) + 14) + 2 * s;
         if (cost < best) { best = cost; p.split = s; }
     }
-    // beside dw in one launch: no slice longer than half of what a CU has to do (~8 and ~14 K-steps for the rest of a dw and a dh tile)
+    // beside dw in one launch: no slice longer than half of what a CU has to do (~8 and ~14 K-steps for the rest of a dw and a dh tile).  That ends below
+    // some 2.2 tiles per CU and one slab more (150 MiB and one T x H): the slabs need no limit of their own
     p.split_both = 1;
     if (!p.few) {
         const int64_t dw_steps = (int64_t)st_cdiv(std::min(V, p.piece), 256) * st_cdiv(H, 256) * (p.T64 / 64 + 8);
@@ -1190,9 +1191,10 @@ Plan head_plan(int T, int V, int H, int K) {                         // K: targe
     p.scale = up((int64_t)T * (int64_t)sizeof(VhRow), 256);
     p.hz = p.scale + up((int64_t)T * 4, 256);
     p.hzt = p.hz;                                                    // one of the two
+    const int64_t d_bytes = up((int64_t)p.T64 * std::min<int64_t>(p.piece, up(V, 64)) * 2, 256);        // the largest row pitch of d is that of the first piece
     p.d = p.hz + up((int64_t)p.T64 * H * 2, 256);
-    p.dt = p.d + up((int64_t)p.T64 * p.piece * 2, 256);
-    p.slab = p.dt + (p.few ? up((int64_t)p.T64 * p.piece * 2, 256) : 0);
+    p.dt = p.d + d_bytes;
+    p.slab = p.dt + (p.few ? d_bytes : 0);
     p.bwd_bytes = p.slab + up((int64_t)std::max(p.split, p.split_both) * T * H * 4, 256);
     return p;
 }

@@ -156,3 +156,25 @@ def test_top_log_probs_of_overlapping_rows_and_single_columns():
             ops.topk_logprob(z, k)
         with pytest.raises(RuntimeError, match="not on a GPU"):
             VF.top_log_probs(z, k)
+
+
+def test_workspace_is_what_the_rows_need():
+    """d of a piece takes at most 512 MiB or, beyond 2^20 rows, 256 columns per row, and never more columns than the vocabulary has; the partial sums of dh
+    one fp32 T x H and at most 512 MiB more."""
+    from spatialthinker_amd.lib import lib
+    n = ctypes.c_int64(0)
+
+    def need(T, V, H):
+        assert lib().st_linear_head_workspace_bytes.raw(T, V, H, 0, 1, ctypes.addressof(n), None) == 0
+        return n.value
+    up = lambda x, a: (x + a - 1) // a * a
+    for T in (1, 64, 65, 128, 129, 256, 257, 1000, 4096, 8192, 65536, 1 << 20, 65535 * 64 + 100):
+        for V in (1, 5, 64, 65, 300, 32513, 152064, 1 << 21):
+            for H in (64, 2048, 8192):
+                rows = up(T, 64)
+                d = min(max(512 << 20, rows * 512), rows * up(V, 64) * 2)
+                fixed = 20 * T + rows * H * 2 + T * H * 4 + (2 if T <= 128 else 1) * d
+                slabs = need(T, V, H) - fixed
+                assert slabs <= (512 << 20) + 256 * 8, (T, V, H, slabs)
+    few = need(65535 * 64 + 100, 5, 64)
+    assert few <= (65535 * 64 + 100) * (20 + 128 + 256 + 128) + 64 * 300 + 256 * 8    # 64 columns of d, not a tile's 256
