@@ -629,7 +629,7 @@ __global__ __launch_bounds__(256) void head_dh_kernel(const uint16_t* __restrict
 // w is contraction-major: its fragments are LDS transpose reads (image and swizzle as the contraction-major operands of gemm_asm4.hip).  Four
 // waves of 64 columns, all rows each; the vocabulary is cut into slices so that every CU has two workgroups.  Bound: the weight stream (3584 x 152 064:
 // 16 rows 186 us = 5.9 TB/s, 128 rows 244 us = 4.5).
-template <int MT, int SLOTS, bool ACCUM>
+template <int MT, int SLOTS>
 __global__ __launch_bounds__(256, 2) void head_dh_few_kernel(const uint16_t* __restrict__ d, int64_t ldd, const uint16_t* __restrict__ w, int64_t ldw, int T,
                                                             int kv, int H, int tiles_n, int per, float* __restrict__ slab) {
     constexpr int BT = 16 * MT, WB = 32 * 512, SLOT = WB + BT * 64, DC = BT / 64;
@@ -710,10 +710,7 @@ __global__ __launch_bounds__(256, 2) void head_dh_few_kernel(const uint16_t* __r
         for (int i = 0; i < 4; ++i) {
             const int n = n0 + wave * 64 + i * 16 + fk * 4;
             if (n >= H) continue;
-            float4* q = reinterpret_cast<float4*>(out + (int64_t)m * H + n);
-            float4 o = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
-            if constexpr (ACCUM) { const float4 c = *q; o.x += c.x; o.y += c.y; o.z += c.z; o.w += c.w; }
-            *q = o;
+            *reinterpret_cast<f32x4*>(out + (int64_t)m * H + n) = acc[i][j];
         }
     }
 }
@@ -1266,8 +1263,9 @@ int head_stats(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, c
     return 0;
 }
 
-int launch_dh_few(const uint16_t* d, int64_t ldd, const uint16_t* w, int64_t ldw, int T, int kv, int H, int tiles_n, const Plan& p, bool accumulate,
-                  float* slab, hipStream_t s) {
+// (few rows: the whole vocabulary is one piece, so there is nothing to add to)
+static_assert(((int64_t)512 << 20) / 2 / VH_FEW >= VH_MAX_V, "few rows need one piece");
+int launch_dh_few(const uint16_t* d, int64_t ldd, const uint16_t* w, int64_t ldw, int T, int kv, int H, int tiles_n, const Plan& p, float* slab, hipStream_t s) {
     const int nkt = st_cdiv(kv, 32), per = st_cdiv(nkt, p.split);
     const dim3 grid(tiles_n * st_cdiv(nkt, per));
     auto go = [&](auto kern, int smem) {
@@ -1277,11 +1275,11 @@ int launch_dh_few(const uint16_t* d, int64_t ldd, const uint16_t* w, int64_t ldw
     };
     constexpr int S64 = 4 * (32 * 512 + 64 * 64), S128 = 3 * (32 * 512 + 128 * 64);
     if (p.T64 == 64) {
-        allow_lds<head_dh_few_kernel<4, 4, false>>(S64); allow_lds<head_dh_few_kernel<4, 4, true>>(S64);
-        return accumulate ? go(head_dh_few_kernel<4, 4, true>, S64) : go(head_dh_few_kernel<4, 4, false>, S64);
+        allow_lds<head_dh_few_kernel<4, 4>>(S64);
+        return go(head_dh_few_kernel<4, 4>, S64);
     }
-    allow_lds<head_dh_few_kernel<8, 3, false>>(S128); allow_lds<head_dh_few_kernel<8, 3, true>>(S128);
-    return accumulate ? go(head_dh_few_kernel<8, 3, true>, S128) : go(head_dh_few_kernel<8, 3, false>, S128);
+    allow_lds<head_dh_few_kernel<8, 3>>(S128);
+    return go(head_dh_few_kernel<8, 3>, S128);
 }
 
 // the pieces of a backward pass behind the row coefficients; `sparse` finishes d at the targets of a piece
@@ -1343,7 +1341,7 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
             continue;
         }
         if (dh && p.few) {
-            const int rc = launch_dh_few(d, ldd, wp, ldw, T, kv, H, th, p, i > 0, slab, s);
+            const int rc = launch_dh_few(d, ldd, wp, ldw, T, kv, H, th, p, slab, s);
             if (rc) return rc;
         } else if (dh) {
             const dim3 grid(tm * th * slices);
