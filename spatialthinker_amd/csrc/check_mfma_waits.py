@@ -4,15 +4,21 @@ result needs (the compiler inserts these for its own MFMAs only).   check_mfma_w
 
 Every path of that many wait states behind each MFMA is followed, through branches on both sides.  An instruction counts one state, s_nop N counts N + 1, and
 another MFMA the passes for which the earlier one holds the matrix pipe.  A later MFMA may read or overwrite the result: the hardware orders
-these."""
+these.  Without an llvm-objdump (ROCm's own, or one on the PATH) nothing is checked and a warning says so."""
 import os
 import re
+import shutil
 import subprocess
 import sys
 import tempfile
 
 LLVM = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "llvm", "bin")
 STATES, PASSES = 8, 4                        # 16x16x32 bf16: result -> VALU / memory instruction; the next MFMA waits 4 for the matrix pipe
+
+
+def objdump():
+    """The llvm-objdump to use, or None."""
+    return shutil.which(os.path.join(LLVM, "llvm-objdump")) or shutil.which("llvm-objdump")
 
 
 def registers(text):
@@ -25,14 +31,15 @@ def registers(text):
 
 def functions(obj):
     """{name: [(address, instruction, operands, branch target or None)]} of the device code in an object."""
+    tool = objdump()
     with tempfile.TemporaryDirectory() as d:
         copy = os.path.join(d, "o.o")
         with open(obj, "rb") as f, open(copy, "wb") as g:
             g.write(f.read())
-        subprocess.run([os.path.join(LLVM, "llvm-objdump"), "--offloading", copy], check=True, stdout=subprocess.DEVNULL)
+        subprocess.run([tool, "--offloading", copy], check=True, stdout=subprocess.DEVNULL)
         out, name = {}, None
         for code in sorted(f for f in os.listdir(d) if "amdgcn" in f):
-            text = subprocess.run([os.path.join(LLVM, "llvm-objdump"), "-d", os.path.join(d, code)], check=True, stdout=subprocess.PIPE, text=True).stdout
+            text = subprocess.run([tool, "-d", os.path.join(d, code)], check=True, stdout=subprocess.PIPE, text=True).stdout
             for line in text.splitlines():
                 m = re.match(r"[0-9a-f]+ <(.+)>:$", line)
                 if m:
@@ -75,6 +82,9 @@ def early(code):
 
 
 def main(objects):
+    if objdump() is None:
+        print("check_mfma_waits.py: warning: no llvm-objdump in %s or on the PATH: wait states not checked" % LLVM, file=sys.stderr)
+        return 0
     failed = 0
     for obj in objects:
         for name, code in functions(obj).items():

@@ -59,3 +59,20 @@ def test_the_built_kernels_have_their_waits(check):
     seen = check.functions(objs[1])
     assert sum(any(op.startswith("v_mfma") for _, op, _, _ in code) for code in seen.values()) >= 10
     assert check.main(objs) == 0
+
+
+def test_a_machine_without_objdump_builds_and_says_what_was_not_checked(check, monkeypatch, capsys, tmp_path):
+    monkeypatch.setattr(check, "LLVM", str(tmp_path))
+    monkeypatch.setenv("PATH", str(tmp_path))
+    assert check.main([str(tmp_path / "any.o")]) == 0
+    err = capsys.readouterr().err
+    assert "llvm-objdump" in err and str(tmp_path) in err and "not checked" in err
+
+
+def test_an_objdump_on_the_path_will_do(check, monkeypatch, tmp_path):
+    tool = tmp_path / "llvm-objdump"
+    tool.write_text("#!/bin/sh\nexit 0\n")
+    tool.chmod(0o755)
+    monkeypatch.setattr(check, "LLVM", str(tmp_path / "nothing"))
+    monkeypatch.setenv("PATH", str(tmp_path))
+    assert check.objdump() == str(tool)
