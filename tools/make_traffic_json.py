@@ -1,5 +1,6 @@
-"""profiles/r04_gemm_traffic.json (r03_… in round 3) from the PMC passes of tools/bench_traffic.sh.
-    python tools/make_traffic_json.py <pmc FETCH json> <pmc WRITE json> <bench line of the FETCH pass> <out.json>
+"""profiles/gemm_traffic.json from the PMC passes of tools/bench_traffic.sh.
+    python tools/make_traffic_json.py <pmc FETCH json> <pmc WRITE json> <bench line of the FETCH pass> <out.json> [<decode FETCH json> <decode WRITE json> [iterations [note]]]
+A counter file may be several joined by '+': a kernel's counters come from the last one that has it.
 FETCH_SIZE / WRITE_SIZE are reported in KiB; FETCH_SIZE is doubled (MI355X_MICROARCH.md, HBM section: on gfx950 it counts 128-byte
 requests as 64 bytes for wide coalesced reads).  Training GEMM class = the 256x256 tiles (4-wave asm tile, 8-wave tile in its TN /
 SwiGLU forms) and the 128x128 kernel; decode iteration = everything replayed from the decode hipGraph."""
@@ -9,8 +10,17 @@ import sys
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 fetch, write, bench_line, out = sys.argv[1:5]
-F, W = json.load(open(fetch)), json.load(open(write))
-DF, DW = (json.load(open(sys.argv[5])), json.load(open(sys.argv[6]))) if len(sys.argv) > 6 else ({}, {})     # decode probe (tools/gen_flat.py 40 64 8)
+
+
+def load(paths):
+    res = {}
+    for p in paths.split("+"):
+        res.update(json.load(open(p)))
+    return res
+
+
+F, W = load(fetch), load(write)
+DF, DW = (load(sys.argv[5]), load(sys.argv[6])) if len(sys.argv) > 6 else ({}, {})     # decode probe (tools/gen_flat.py 40 64 8)
 line = json.loads(open(bench_line).read().strip().splitlines()[-1])
 
 
@@ -60,5 +70,7 @@ res = {"kernel_source_sha16": bench.gemm_source_sha(), "command": "rocprofv3 --k
        "decode_command": "rocprofv3 --kernel-trace --pmc {FETCH_SIZE | WRITE_SIZE} -- python3 tools/gen_flat.py 6 64 8   (from the repo root; 512 live rows, 1102-token prompts, 2 x 5 decode iterations)",
        "decode_top_kernels": dict(sorted(dec_kernels.items(), key=lambda kv: -kv[1])[:6]),
        "top_kernels": dict(sorted(per_kernel.items(), key=lambda kv: -kv[1]["launches"] * kv[1]["hbm_bytes_per_launch"])[:6])}
+if len(sys.argv) > 8:
+    res["counters"] = sys.argv[8]
 json.dump(res, open(out, "w"), indent=1)
 print(json.dumps(res)[:600])
