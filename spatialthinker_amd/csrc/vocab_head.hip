@@ -988,7 +988,6 @@ __global__ __launch_bounds__(256, OUT_BF16 ? 2 : 1) void head_dw_mid_kernel(cons
 // Distillation from k teacher log-probs per row.
 // ------------------------------------------------------------------------------------------------------------------------------------
 #define VH_MAX_K 1024
-#define VH_MID_SPLIT 3                                               // column ranges of head_dw_mid_kernel: 594 row blocks alone are 1.2 rounds of two per CU
 
 #define VH_FEW 128                                                   // rows up to which the weight stream bounds the products
 #define VH_MAX_V (1 << 21)                                           // column tiles fit the counters of head_bucket_kernel
@@ -1282,6 +1281,19 @@ int launch_dh_few(const uint16_t* d, int64_t ldd, const uint16_t* w, int64_t ldw
     return go(head_dh_few_kernel<8, 3>, S128);
 }
 
+// Column ranges of head_dw_mid_kernel for `blocks` row blocks: the launch takes whole rounds of two workgroups per CU, each as long as its range, so the
+// count with the fewest rounds per range, and of equals the lowest (a range loads its d again).  MI355X, dW alone at 150 / 200 rows, us for 1, 2, 3
+// ranges: V = 33 001 (129 blocks: 3) H = 2048 82 67 57 / 96 79 66, H = 3584 125 98 80 / 148 117 98; 50 257 (197 blocks: 2) H = 2048 85 77 85 / 99 84 93,
+// H = 3584 130 104 121 / 150 124 137; 128 256 (501 blocks: 1) H = 1024 115 103 111 / 125 116 123, H = 2048 164 223 189 / 170 237 208, H = 3584 231 234
+// 232 / 274 283 273; 152 064 (594 blocks: 3) H = 2048 221 264 210 / 235 280 230, H = 3584 331 286 273 / 362 338 331.  4 and 6 were nowhere better
+// by more than 1 %.
+int mid_ranges(int blocks) {
+    int best = 1, cost = 6 * st_cdiv(blocks, 2 * st_num_cus());
+    for (int n = 2; n <= 3; ++n)
+        if (const int c = 6 / n * st_cdiv(blocks * n, 2 * st_num_cus()); c < cost) { cost = c; best = n; }
+    return best;
+}
+
 // the pieces of a backward pass behind the row coefficients; `sparse` finishes d at the targets of a piece
 template <class F>
 int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, float sc, const float* z, int64_t ldz, uint16_t* dh, int64_t lddh, uint16_t* dwb, float* dwf,
@@ -1361,7 +1373,7 @@ int head_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw
 #undef VH_DW_FEW
             }
             else if (mid) {
-                const int smem = p.T64 * 128 + 4 * 64 * 144, mid_cols = (int)up(st_cdiv(H, VH_MID_SPLIT), 64);
+                const int smem = p.T64 * 128 + 4 * 64 * 144, mid_cols = (int)up(st_cdiv(H, mid_ranges(tv)), 64);
 #define VH_DW_MID(KS, OB, AC) do { allow_lds<head_dw_mid_kernel<KS, OB, AC>>(smem); \
         hipLaunchKernelGGL((head_dw_mid_kernel<KS, OB, AC>), dim3(tv, st_cdiv(H, mid_cols)), dim3(256), smem, s, d, ldd, hz, kv, H, mid_cols, ob, of, lddw); } while (0)
                 if (p.T64 == 192) { if (dwb) VH_DW_MID(6, true, false); else if (accumulate) VH_DW_MID(6, false, true); else VH_DW_MID(6, false, false); }

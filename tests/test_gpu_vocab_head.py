@@ -158,13 +158,19 @@ def test_fp32_weight_gradient_and_single_gradients(T, accumulate):
     assert (pitched[:, H:] == 7.0).all()                           # behind the rows: untouched
 
 
+@pytest.mark.parametrize("T,H,V", [(150, 192, 50257), (250, 448, 50257), (190, 192, 100001), (256, 320, 100001), (140, 320, 140003), (200, 192, 140003)])
+def test_column_ranges_of_the_weight_gradient(T, H, V):
+    """Two, one and three column ranges (197, 391 and 547 row blocks on 256 compute units)."""
+    test_weight_gradient_of_129_to_256_rows_over_a_large_vocabulary(T, H, V)
+
+
 @pytest.mark.parametrize("T", [129, 160, 161, 192, 193, 256])
 @pytest.mark.parametrize("H", [64, 192, 448])
-def test_weight_gradient_of_129_to_256_rows_over_a_large_vocabulary(T, H):
+def test_weight_gradient_of_129_to_256_rows_over_a_large_vocabulary(T, H, V=33001):
     """From 32 513 columns on (two row blocks of 256 per compute unit) these row counts have a weight-gradient kernel of their own: all of its row tiles and
     outputs, column ranges that are uneven or fewer than three, a vocabulary that ends inside a tile, logits kept and formed again, a pitched result."""
     from spatialthinker_amd import ops
-    V, temperature = 33001, 0.8
+    temperature = 0.8
     print(f"case T={T} H={H} V={V}", flush=True)
     g, h, w, lab, gr = make(T, H, V, T + H, pitch_h=8, pitch_w=24)
     dead = torch.rand(T, device="cuda", generator=g) < 0.1
