@@ -268,6 +268,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t*
     for (int kt = 0; kt < nk; ++kt) {
         // this step's copies have landed; up to SLOTS - 2 younger steps stay in flight (the last steps have none to count)
         if (kt + SLOTS - 2 < nk) vh_wait_vm<(SLOTS - 2) * (4 + HC)>(); else vh_wait_vm<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // nothing to wait for where the compiler puts the last products before the barrier
         __builtin_amdgcn_s_barrier();                                // ... for every wave, and every wave has read the slot that is filled next
         asm volatile("" ::: "memory");
         if (kt + SLOTS - 1 < nk) stage(kt + SLOTS - 1);
