@@ -81,8 +81,8 @@ __device__ __forceinline__ void vh_store_image(const char* smem, uint16_t* __res
 // KEEP: z[m][n] = h_m . w_n in fp32 as well, straight from the accumulators (64-byte runs; V = 152 064, H = 3584, 4096 rows: 416 us for 2.5 GB).
 // DLOGITS: d[m][n] (bf16, pitch ldd, zero in columns [V, ldd) and rows [T, T64)).
 // Bound by the matrix pipe: the main loop is the four-wave tile of the framework's GEMM, and the epilogue has to cost little beside it.  MI355X,
-// V = 152 064, H = 3584: 4096 rows 3.05 ms = 1.46 PF/s with the join (the GEMM alone, writing logits, 3.15); 161 .. 256 rows, one row tile: 260 us
-// whatever their number, 4.2 TB/s of weights (2.3 rounds of 256 tiles: a last part round in narrower tiles was 0 to 8 % slower).
+// V = 152 064, H = 3584: 4096 rows 3.05 to 3.2 ms by card = 1.40 to 1.46 PF/s with the join (the GEMM alone, writing logits, 3.1); 161 .. 256 rows, one row
+// tile: 260 to 285 us whatever their number, 4 TB/s of weights (2.3 rounds of 256 tiles: a last part round in narrower tiles was 0 to 8 % slower).
 // ------------------------------------------------------------------------------------------------------------------------------------
 template <bool DLOGITS, bool ONE_ROW_TILE, bool KEEP = false>
 __global__ __launch_bounds__(256) void head_tile_kernel(const uint16_t* __restrict__ h, int64_t ldh, const uint16_t* __restrict__ w, int64_t ldw, int T,

@@ -201,7 +201,7 @@ def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.T
     -> (...) fp32, differentiable in hidden and weight.  The logits stay in fp32 and are kept for the backward only while
     they take at most `keep_logits` bytes (8 GiB of the card's 288: 14 122 rows of V = 152 064); beyond that, or with 0, the backward forms them again,
     a piece of the vocabulary at a time (the gradient of one piece: 0.5 GiB at most up to 2^20 rows, 512 bytes a row beyond; next to it
-    the fp32 partial sums of hidden's: one rows x H and at most 0.5 GiB), which takes 4 to 25 % more
+    the fp32 partial sums of hidden's: one rows x H and at most 0.5 GiB), which takes 4 to 27 % more
     time for forward and backward together.  Without a gradient nothing is kept.  Both ways give the same bits.
     A label outside [0, V) (padding, -100) marks a row that is not scored: 0, and no gradient from it.  H must be a multiple of 64; GPU tensors only."""
     if labels.shape != hidden.shape[:-1]:
