@@ -1430,7 +1430,7 @@ int st_linear_logprob_fwd(const st_bf16* hidden, int64_t ldh, const st_bf16* wei
     if (T == 0) return V > 0 && H > 0 && H % 64 == 0 ? 0 : ST_EINVAL;
     if (!operands_ok(hidden, ldh, weight, ldw, T, V, H, inv_temperature) || !labels || !logp || !lse || !logits_ok(logits, ldz, V)) return ST_EINVAL;
     const Plan p = head_plan(T, V, H, 0);
-    if (!workspace || workspace_bytes < p.fwd_bytes) return ST_EINVAL;
+    if (!workspace || (((uintptr_t)workspace) & 15) || workspace_bytes < p.fwd_bytes) return ST_EINVAL;
     return head_stats(hidden, ldh, weight, ldw, labels, inv_temperature * VH_LOG2E, logp, lse, VhTargets{}, logits, ldz, (char*)workspace, p, T, V, H,
                       (hipStream_t)stream);
 }
@@ -1443,7 +1443,7 @@ int st_linear_logprob_bwd(const st_bf16* hidden, int64_t ldh, const st_bf16* wei
     if (T == 0) return empty_dw(dweight_bf16, dweight_f32, lddw, accumulate, V, H, s);
     if (!operands_ok(hidden, ldh, weight, ldw, T, V, H, inv_temperature) || !labels || !logp || !lse || !g || !logits_ok(logits, ldz, V)) return ST_EINVAL;
     const Plan p = head_plan(T, V, H, 0);
-    if (!workspace || workspace_bytes < p.bwd_bytes) return ST_EINVAL;
+    if (!workspace || (((uintptr_t)workspace) & 15) || workspace_bytes < p.bwd_bytes) return ST_EINVAL;
     char* ws = (char*)workspace;
     hipLaunchKernelGGL(head_rows_label_kernel, dim3(p.few ? p.TP : p.T64), dim3(128), 0, s, hidden, ldh, labels, logp, lse, g, inv_temperature, (VhRow*)(ws + p.rows),
                        (float*)(ws + p.scale), p.few ? nullptr : (uint16_t*)(ws + p.hz), (uint16_t*)(ws + p.hzt), p.TP, T, V, H);
@@ -1459,7 +1459,7 @@ int st_linear_topk_kl_fwd(const st_bf16* hidden, int64_t ldh, const st_bf16* wei
     if (T == 0) return V > 0 && H > 0 && H % 64 == 0 ? 0 : ST_EINVAL;
     if (!operands_ok(hidden, ldh, weight, ldw, T, V, H, inv_temperature) || !ids || !teacher_logp || !kl || !lse || !logq || !logits_ok(logits, ldz, V)) return ST_EINVAL;
     const Plan p = head_plan(T, V, H, K);
-    if (!workspace || workspace_bytes < p.fwd_bytes) return ST_EINVAL;
+    if (!workspace || (((uintptr_t)workspace) & 15) || workspace_bytes < p.fwd_bytes) return ST_EINVAL;
     hipStream_t s = (hipStream_t)stream;
     const float sc = inv_temperature * VH_LOG2E;
     char* ws = (char*)workspace;
@@ -1486,7 +1486,7 @@ int st_linear_topk_kl_bwd(const st_bf16* hidden, int64_t ldh, const st_bf16* wei
     if (T == 0) return empty_dw(dweight_bf16, dweight_f32, lddw, accumulate, V, H, s);
     if (!operands_ok(hidden, ldh, weight, ldw, T, V, H, inv_temperature) || !ids || !teacher_logp || !lse || !logq || !g || !logits_ok(logits, ldz, V)) return ST_EINVAL;
     const Plan p = head_plan(T, V, H, 0);
-    if (!workspace || workspace_bytes < p.bwd_bytes) return ST_EINVAL;
+    if (!workspace || (((uintptr_t)workspace) & 15) || workspace_bytes < p.bwd_bytes) return ST_EINVAL;
     char* ws = (char*)workspace;
     hipLaunchKernelGGL(head_rows_kl_kernel, dim3(p.few ? p.TP : p.T64), dim3(128), 0, s, hidden, ldh, ids, teacher_logp, K, renormalize, lse, logq, g, inv_temperature,
                        (VhRow*)(ws + p.rows), (float*)(ws + p.scale), p.few ? nullptr : (uint16_t*)(ws + p.hz), (uint16_t*)(ws + p.hzt), p.TP, T, V, H);

@@ -178,3 +178,15 @@ def test_workspace_is_what_the_rows_need():
                 assert slabs <= (512 << 20) + 256 * 8, (T, V, H, slabs)
     few = need(65535 * 64 + 100, 5, 64)
     assert few <= (65535 * 64 + 100) * (20 + 128 + 256 + 128) + 64 * 300 + 256 * 8    # 64 columns of d, not a tile's 256
+
+
+def test_workspaces_that_are_not_aligned_are_refused():
+    """The kernels store 16 bytes at a time into the workspace."""
+    from spatialthinker_amd.lib import lib
+    L, p = lib(), 1 << 20                                          # never touched: every call below is refused
+    for off in (1, 4, 8):
+        ws = p + off
+        assert L.st_linear_logprob_fwd.raw(p, 64, p, 64, p, 1.0, p, p, None, 0, ws, 1 << 40, 8, 1000, 64, None) == -22
+        assert L.st_linear_logprob_bwd.raw(p, 64, p, 64, p, p, p, p, 1.0, None, 0, p, 64, None, None, 0, 0, ws, 1 << 40, 8, 1000, 64, None) == -22
+        assert L.st_linear_topk_kl_fwd.raw(p, 64, p, 64, p, p, 4, 0, 1.0, p, p, p, None, 0, ws, 1 << 40, 8, 1000, 64, None) == -22
+        assert L.st_linear_topk_kl_bwd.raw(p, 64, p, 64, p, p, 4, 0, 1.0, p, p, p, None, 0, p, 64, None, None, 0, 0, ws, 1 << 40, 8, 1000, 64, None) == -22
