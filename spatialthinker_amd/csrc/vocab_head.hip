@@ -999,8 +999,10 @@ __device__ __forceinline__ VhTeacher vh_teacher(const int32_t* __restrict__ ids,
     VhTeacher r = {0.f, 0.f};
     if (renorm) {                                                    // log p = a - log sum_k exp a over the present entries
         float m = -INFINITY, s = 0.f;
-        for (int k = lane; k < K; k += 64) if (ids[k] >= 0 && ids[k] < V) m = fmaxf(m, a[k]);
+        bool nan = false;                                            // (fmaxf passes NaN over)
+        for (int k = lane; k < K; k += 64) if (ids[k] >= 0 && ids[k] < V) { m = fmaxf(m, a[k]); nan = nan || a[k] != a[k]; }
         m = wave_max(m);
+        if (__any(nan)) { r.shift = r.total = NAN; return r; }
         if (m == -INFINITY) return r;                                // nothing present (or only zero probabilities): the row takes no part
         for (int k = lane; k < K; k += 64) if (ids[k] >= 0 && ids[k] < V) s += vh_exp2((a[k] - m) * VH_LOG2E);
         s = wave_sum(s);

@@ -319,6 +319,30 @@ def test_linear_topk_kl_forward_and_gradients(T, H, V, K, temperature, renorm):
     assert torch.isfinite(dh).all() and torch.isfinite(dw).all()
 
 
+@pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("T", [6, 200])
+def test_a_teacher_of_nan_is_not_silent(T, renorm):
+    """NaN log-probs of present entries, some or all of a row's: that row's KL and hidden gradient are NaN, the other rows' are what they are without it."""
+    from spatialthinker_amd import ops
+    H, V, K = 64, 300, 5
+    g, h, w, lab, gr = make(T, H, V, 17)
+    ids = torch.randint(0, V, (T, K), device="cuda", generator=g, dtype=torch.int32)
+    ids[:, 4] = -1
+    a = torch.log_softmax(torch.randn(T, K, device="cuda", generator=g), 1)
+    a[:, 4] = float("nan")                                         # absent: not read as a number
+    bad = a.clone()
+    bad[1, 2] = float("nan")
+    bad[4] = float("nan")
+    res = []
+    for x in (a, bad):
+        kl, lse, logq = ops.linear_topk_kl_fwd(h, w, ids, x, 1.0, renorm)
+        res.append((kl, ops.linear_topk_kl_bwd(h, w, ids, x, lse, logq, gr, 1.0, renorm)))
+    rows = torch.zeros(T, dtype=torch.bool, device="cuda")
+    rows[[1, 4]] = True
+    for good, got in zip(*res):
+        assert torch.isfinite(good).all() and torch.isnan(got[rows]).all() and torch.equal(got[~rows], good[~rows])
+
+
 @pytest.mark.parametrize("T", [32, 33, 77, 96, 97, 128, 130, 160, 161])
 @pytest.mark.parametrize("H", [64, 192, 2048])
 def test_row_tiles_of_the_weight_stream(T, H):
