@@ -22,6 +22,9 @@
 __device__ __forceinline__ int vh_cols64(int V) { return (V + 63) & ~63; }
 
 __device__ __forceinline__ float vh_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// 2^(z2 - top) of a logit that is at most `top` = its row's rounded maximum or lse: what stands above by that rounding alone (half a step of the product,
+// 2^7 and more from logits of 2^31 on) counts as equal.  NaN stays NaN (minimum, not fminf).
+__device__ __forceinline__ float vh_below(float z, float sc, float top) { return vh_exp2(__builtin_elementwise_minimum(fmaf(z, sc, -top), 0.f)); }
 
 // Statistics of a set of logits (in base 2): x = the largest, y = sum 2^(z - x) - 1.  The largest one's own term is exactly 1 and left out of the sum,
 // because the log-prob of a nearly certain token is -log(1 + y): next to a 1 a small y would keep few of its digits.  Empty: (-inf, -1).
@@ -157,21 +160,22 @@ __global__ __launch_bounds__(256) void head_tile_kernel(const uint16_t* __restri
             s += __shfl_xor(s, 16, 64);
             s += __shfl_xor(s, 32, 64);
             float rest = s - 1.f;                                    // (nothing but -inf: -1)
-            if (__any(s < 1.5f && m2 != -INFINITY)) {                // a row with one large logit among these 128: the others' sum by itself
+            const bool apart = (s < 1.5f || fabsf(m2) >= 0x1p23f) && fabsf(m2) < INFINITY;
+            if (__any(apart)) {                                      // a row with one large logit among these 128, or a rounding of its maximum that counts: the others' sum by itself
                 float o = 0.f, ties = -1.f;
 #pragma unroll
                 for (int ni = 0; ni < 8; ++ni)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float x = acc[ni][mi][r];
-                        if (x == mx) ties += 1.f; else o += vh_exp2(fmaf(x, sc, -sub));
+                        if (x == mx) ties += 1.f; else o += vh_below(x, sc, sub);
                     }
                 ties += lane < 16 ? 0.f : 1.f;                       // (the -1 once per row)
                 o += __shfl_xor(o, 16, 64);
                 o += __shfl_xor(o, 32, 64);
                 ties += __shfl_xor(ties, 16, 64);
                 ties += __shfl_xor(ties, 32, 64);
-                if (s < 1.5f && m2 != -INFINITY) rest = o + ties;      // (s is the same in a row's four lanes: no row depends on the others of its wave)
+                if (apart) rest = o + ties;                          // (s is the same in a row's four lanes: no row depends on the others of its wave)
             }
             if (m < T) {
                 if (lane < 16) part[(int64_t)(tn * 2 + wn) * T + m] = make_float2(m2, rest);
@@ -201,7 +205,7 @@ __global__ __launch_bounds__(256) void head_tile_kernel(const uint16_t* __restri
                 float o[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    float x = ri.c * vh_exp2(fmaf(acc[ni][mi][r], sc, -ri.lse2));
+                    float x = ri.c * vh_below(acc[ni][mi][r], sc, ri.lse2);
                     if (lab == ni * 16 + r) x = ri.hot;
                     o[r] = live && (inside || col0 + ni * 16 + r < V) ? x : 0.f;
                 }
@@ -268,9 +272,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t*
     for (int kt = 0; kt < nk; ++kt) {
         // this step's copies have landed; up to SLOTS - 2 younger steps stay in flight (the last steps have none to count)
         if (kt + SLOTS - 2 < nk) vh_wait_vm<(SLOTS - 2) * (4 + HC)>(); else vh_wait_vm<0>();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // nothing to wait for where the compiler puts the last products before the barrier
-        __builtin_amdgcn_s_barrier();                                // ... for every wave, and every wave has read the slot that is filled next
-        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();                                // ... for every wave, and every wave has read the slot that is filled next (the reads of
+        asm volatile("" ::: "memory");                               // a step have returned before its products; a test finds any in the built code that have not)
         if (kt + SLOTS - 1 < nk) stage(kt + SLOTS - 1);
         const char* lw = smem + (kt % SLOTS) * SLOT + wave * 32 * 128;
         const char* lh = smem + (kt % SLOTS) * SLOT + BN * 128;
@@ -353,8 +356,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t*
             o += __shfl_xor(o, 32, 64);
             ties += __shfl_xor(ties, 16, 64);
             ties += __shfl_xor(ties, 32, 64);
-            // +inf, given or overflowed: NaN, as inf - inf makes it in the sum of all terms
-            if (lane < 16) red[wave * BT + m] = make_float2(m2, m2 == INFINITY ? NAN : m2 != -INFINITY ? o + ties : o - 1.f);
+            if (lane < 16) red[wave * BT + m] = make_float2(m2, m2 != -INFINITY ? o + ties : o - 1.f);
             if (labels && m < T) {
                 const int64_t lab = labels[m] - col0;
 #pragma unroll
@@ -387,7 +389,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void head_few_kernel(const uint16_t*
                 float o[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    float x = ri.c * vh_exp2(fmaf(acc[i][j][r], sc, -ri.lse2));
+                    float x = ri.c * vh_below(acc[i][j][r], sc, ri.lse2);
                     if (lab == i * 16 + r) x = ri.hot;
                     o[r] = live && col0 + i * 16 + r < V ? x : 0.f;
                 }
@@ -453,7 +455,7 @@ __global__ __launch_bounds__(256) void head_d_kernel(const float* __restrict__ z
         float o[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            float x = ri[i].c * vh_exp2(fmaf(v[i][k >> 2][k & 3], sc, -ri[i].lse2));
+            float x = ri[i].c * vh_below(v[i][k >> 2][k & 3], sc, ri[i].lse2);
             if (lab == k) x = ri[i].hot;
             o[k] = live && n0 + c + k < V ? x : 0.f;
         }
@@ -496,7 +498,7 @@ __global__ __launch_bounds__(1024) void head_lse_kernel(const float2* __restrict
     }
     if (sl == 0 && row < T) {
         const float2 v = red[0][r];
-        const float ls = log1pf(v.y) * VH_LOG2E;
+        const float ls = v.x < INFINITY ? log1pf(v.y) * VH_LOG2E : NAN;      // +inf, given or overflowed: NaN, as inf - inf is
         lse[row] = (v.x + ls) * VH_LN2;
         if (stat) stat[row] = make_float2(v.x, ls);
         if (labels) {                                                // (z - max) - log sum: exact where the label is the maximum, so a log-prob near 0
@@ -523,7 +525,7 @@ __global__ __launch_bounds__(1024) void head_lse_few_kernel(const float2* __rest
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) a = vh_join(a, make_float2(__shfl_xor(a.x, o, 64), __shfl_xor(a.y, o, 64)));
         if (lane == 0) {
-            const float ls = log1pf(a.y) * VH_LOG2E;
+            const float ls = a.x < INFINITY ? log1pf(a.y) * VH_LOG2E : NAN;
             lse[row] = (a.x + ls) * VH_LN2;
             if (stat) stat[row] = make_float2(a.x, ls);
             if (labels) {

@@ -319,6 +319,34 @@ def test_linear_topk_kl_forward_and_gradients(T, H, V, K, temperature, renorm):
     assert torch.isfinite(dh).all() and torch.isfinite(dw).all()
 
 
+@pytest.mark.parametrize("T", [5, 40, 100, 150, 200, 300])
+@pytest.mark.parametrize("exponent", [20, 24, 27, 30, 34, 60])
+def test_logits_whose_rounding_exceeds_one_stay_finite(T, exponent):
+    """Logits of 2^exponent and more: their fp32 rounding is larger than any difference that counts, so log-probs are as good as that (ez + el), but the label
+    that is its row's maximum still has between 1 / V and all of the probability, and nothing overflows, backward included."""
+    from spatialthinker_amd import ops
+    H, V = 64, 900
+    print(f"case T={T} exponent={exponent}", flush=True)
+    g, h, w, lab, gr = make(T, H, V, 3 * T + exponent)
+    h = (h.float() * 2.0 ** exponent).to(BF16)
+    z, ez, el = errors64(h, w, 1.0)
+    lab[::2] = z.argmax(1)[::2]
+    kept = ops.head_logits_buffer(T, V, h.device)
+    logp, lse = ops.linear_logprob_fwd(h, w, lab, logits=kept)
+    assert ((lse.to(F64) - torch.logsumexp(z, 1)).abs() <= el).all()
+    want = torch.log_softmax(z, 1).gather(1, lab[:, None])[:, 0]
+    assert ((logp.to(F64) - want).abs() <= ez + el + U32 * want.abs()).all()
+    assert (logp <= 0).all() and (logp[::2] >= -math.log(V) - ez[::2]).all()
+    if exponent >= 27:                                             # two logits of a row nearer than a rounding of them: none in these rows
+        assert (logp[::2] == 0).all()
+    grads = []
+    for logits in (kept, None):
+        dw = torch.empty(V, H, dtype=BF16, device="cuda")
+        grads.append((ops.linear_logprob_bwd(h, w, lab, logp, lse, gr, dweight=dw, logits=logits), dw))
+    for x, y in zip(*grads):
+        assert torch.isfinite(x).all() and torch.equal(x, y)
+
+
 @pytest.mark.parametrize("renorm", [False, True])
 @pytest.mark.parametrize("T", [6, 200])
 def test_a_teacher_of_nan_is_not_silent(T, renorm):
