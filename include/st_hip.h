@@ -99,7 +99,7 @@ int st_linear_topk_kl_bwd(const st_bf16* hidden, int64_t ldh, const st_bf16* wei
                           int64_t workspace_bytes, int T, int V, int H, st_stream_t stream);
 /* The k <= 256 largest log-probs of each row of logits (T, V) bf16 (any row pitch >= V, no alignment beyond 2 bytes): ids (T, k) int32 in falling
  * order, equal logits by rising id (-0 equals 0); logp (T, k) = logit * inv_temperature - lse; lse (T,) = log sum_v exp(logit_v * inv_temperature).
- * -inf logits are allowed (logp -inf); a row with NaN or +inf, or of -inf alone, has NaN log-probs and distinct ids inside [0, V).
+ * -inf logits are allowed (logp -inf); a row with NaN or +inf (given, or beyond fp32 after the temperature), or of -inf alone, has NaN log-probs and distinct ids inside [0, V).
  * workspace: st_topk_logprob_workspace_bytes bytes (0 for many rows: NULL allowed), 8-byte aligned. */
 int st_topk_logprob_workspace_bytes(int T, int V, int k, int64_t* bytes_host, st_stream_t stream);
 int st_topk_logprob(const st_bf16* logits, int64_t ldl, int k, float inv_temperature, int32_t* ids, float* logp, float* lse, void* workspace,

@@ -150,7 +150,8 @@ __device__ __forceinline__ float tk_max3(float a, float b, float c) {
 __device__ __forceinline__ float2 tk_join(float2 a, float2 b) {          // (max, sum) in base 2
     const float m = fmaxf(a.x, b.x);
     if (m == -INFINITY) return make_float2(m, a.y + b.y);
-    return make_float2(m, a.y * __builtin_amdgcn_exp2f(a.x - m) + b.y * __builtin_amdgcn_exp2f(b.x - m));
+    // (an equal maximum counts 1 by comparison: the difference may be a fused one, of the product that x came from)
+    return make_float2(m, (a.x == m ? a.y : a.y * __builtin_amdgcn_exp2f(a.x - m)) + (b.x == m ? b.y : b.y * __builtin_amdgcn_exp2f(b.x - m)));
 }
 template <int NT> __device__ __forceinline__ float2 tk_block_join(TkShared<NT>& sh, float2 v) {
 #pragma unroll
@@ -164,7 +165,7 @@ template <int NT> __device__ __forceinline__ float2 tk_block_join(TkShared<NT>& 
 }
 template <int NT> __device__ __forceinline__ void tk_write(TkShared<NT>& sh, int k, float2 ms, float inv_temp, int32_t* __restrict__ ids, float* __restrict__ logp,
                                          float* __restrict__ lse) {
-    const float l = (ms.x + log2f(ms.y)) * TK_LN2;
+    const float l = ms.x < INFINITY ? (ms.x + log2f(ms.y)) * TK_LN2 : NAN;           // +inf, given or beyond fp32
     if (threadIdx.x == 0) *lse = l;
     for (int j = threadIdx.x; j < k; j += NT) {
         const uint64_t key = l == l ? sh.best[j] : 0;
@@ -193,6 +194,14 @@ __global__ __launch_bounds__(NT, 4) void topk_row_kernel(const uint16_t* __restr
     int used = 0;                                                        // granules kept, at most; the same for every thread
     int thr = TK_NONE;                                                   // values of a lower order are out
     float top = -INFINITY, m = -INFINITY, s = 0.f;                       // this thread's largest so far; base-2 maximum and sum
+    // a value's term is 2^(f by - sub), sub = m (0 while that is -inf).  From |m| = 2^30 on, where m's own rounding may be more than an exponent holds,
+    // other bf16 values lie 2^22 away at least: unscaled, by exact differences, they count 0 and equal ones 1.
+    float by = sc, sub = 0.f;
+    auto measure = [&](float f) {                                        // f: the value whose product m is
+        const bool far = fabsf(m) >= 0x1p30f;
+        by = far ? 1.f : sc;
+        sub = far ? f : m;
+    };
     bool any = false;                                                    // this thread has met a value
     __syncthreads();
     auto single = [&](int e) {                                           // one value outside the granules; the list has room for these
@@ -202,6 +211,7 @@ __global__ __launch_bounds__(NT, 4) void topk_row_kernel(const uint16_t* __restr
         if (f >= tk_value(thr)) sh.cand[atomicAdd(&sh.count, 1)] = tk_key(tk_order(x[beg + e]), (uint32_t)(beg + e));
         const float2 v = tk_join(make_float2(m, s), make_float2(f * sc, f == -INFINITY ? 0.f : f == f ? 1.f : f));
         m = v.x; s = v.y;
+        if (m > -INFINITY) measure(f);                                   // (in front of the granules: this thread's first value; behind them nothing follows)
     };
     if ((int)threadIdx.x < front) single(threadIdx.x);
     // the values of one granule per thread (where `here`) that pass the threshold -> candidates; ids above those of all candidates so far
@@ -267,11 +277,14 @@ __global__ __launch_bounds__(NT, 4) void topk_row_kernel(const uint16_t* __restr
             most = fmaxf(most, cmax[c]);
             // the exponential sum, base 2
             const float vm = cmax[c] * sc;                               // sc > 0
-            if (vm > m) { s *= __builtin_amdgcn_exp2f(m - vm); m = vm; }
-            const float sub = m == -INFINITY ? 0.f : m;
+            if (vm > m) {
+                s *= __builtin_amdgcn_exp2f(m - vm);
+                m = vm;
+                measure(cmax[c]);
+            }
             float a = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) a += __builtin_amdgcn_exp2f(fmaf(f[j], sc, -sub));
+            for (int j = 0; j < 8; ++j) a += __builtin_amdgcn_exp2f(fmaf(f[j], by, -sub));
             s += a;
         }
         top = fmaxf(top, most);

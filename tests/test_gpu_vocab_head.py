@@ -612,6 +612,25 @@ def test_top_log_probs_with_a_kth_value_far_below_the_largest(T, V, k):
         check_top(z[i:i + T], k)
 
 
+@pytest.mark.parametrize("T,V,k", [(1, 1, 1), (3, 13, 13), (64, 300, 20), (600, 5003, 64), (2, 152064, 100)])
+@pytest.mark.parametrize("exponent", [10, 24, 29, 31, 40, 100])
+def test_top_log_probs_of_huge_logits(T, V, k, exponent):
+    """Logits of 2^exponent: finite log-probs as good as their fp32 rounding, at every alignment; with a temperature that takes them beyond fp32, NaN."""
+    from spatialthinker_amd import ops
+    print(f"case T={T} V={V} k={k} exponent={exponent}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(T + V + exponent)
+    buf = (torch.randn(T, V + 9, device="cuda", generator=g) * 2.0 ** exponent).to(BF16)
+    for off in (0, 3, 8):
+        z = buf[:, off:off + V]
+        _, logp, lse = ops.topk_logprob(z, k)
+        assert torch.isfinite(lse).all() and torch.isfinite(logp).all()
+        check_top(z, k)
+        check_top(-z.abs(), k)
+        check_top(torch.where(z > 0, z, -1.0).to(BF16), k)         # huge and ordinary logits in a row
+    ids, logp, lse = ops.topk_logprob(buf[:, :V].abs() + 2.0 ** exponent, k, 2.0 ** -40 if exponent == 100 else 1.0)
+    assert torch.isnan(logp).all() == (exponent == 100) and (ids >= 0).all() and (ids < V).all()
+
+
 def test_top_log_probs_pitch_alignment_and_special_rows():
     from spatialthinker_amd import ops
     g = torch.Generator(device="cuda").manual_seed(2)
