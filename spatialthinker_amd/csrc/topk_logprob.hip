@@ -194,8 +194,8 @@ __global__ __launch_bounds__(NT, 4) void topk_row_kernel(const uint16_t* __restr
     int used = 0;                                                        // granules kept, at most; the same for every thread
     int thr = TK_NONE;                                                   // values of a lower order are out
     float top = -INFINITY, m = -INFINITY, s = 0.f;                       // this thread's largest so far; base-2 maximum and sum
-    // a value's term is 2^(f by - sub), sub = m (0 while that is -inf).  From |m| = 2^30 on, where m's own rounding may be more than an exponent holds,
-    // other bf16 values lie 2^22 away at least: unscaled, by exact differences, they count 0 and equal ones 1.
+    // a value's term is 2^(f by - sub), sub = m (0 while that is -inf).  From |m| = 2^30 on m's own rounding may be more than an exponent holds: unscaled, by
+    // exact differences, a value counts at most 1 and the largest 1, and the logarithm of the whole row's sum is below half a step of m.
     float by = sc, sub = 0.f;
     auto measure = [&](float f) {                                        // f: the value whose product m is
         const bool far = fabsf(m) >= 0x1p30f;

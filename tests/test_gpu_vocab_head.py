@@ -627,6 +627,8 @@ def test_top_log_probs_of_huge_logits(T, V, k, exponent):
         check_top(z, k)
         check_top(-z.abs(), k)
         check_top(torch.where(z > 0, z, -1.0).to(BF16), k)         # huge and ordinary logits in a row
+    check_top((buf[:, :V] * 2.0 ** -exponent).to(BF16), k, 2.0 ** -min(exponent, 60))              # ordinary logits, made huge by the temperature
+    check_top((buf[:, :V] * 2.0 ** -exponent).to(BF16), k, 1.3 * 2.0 ** -min(exponent, 60))
     ids, logp, lse = ops.topk_logprob(buf[:, :V].abs() + 2.0 ** exponent, k, 2.0 ** -40 if exponent == 100 else 1.0)
     assert torch.isnan(logp).all() == (exponent == 100) and (ids >= 0).all() and (ids < V).all()
 
